@@ -17,7 +17,8 @@
  *     (k == 1): the lookup kernels' per-block partial sums;
  *   - ouro_matmul_q on a raw TL1 payload for k >= 2 columns: x as int8
  *     digit planes for the MFMA pass;
- *   - ouro_gdn_chunk_prefill with a NULL workspace.
+ *   - ouro_gdn_chunk_prefill, ouro_kv_attend, ouro_kv_evict and
+ *     ouro_token_logprobs with a NULL workspace.
  * A weight handle (ouro_weight_upload) or ouro_matvec_q_noalloc avoids them.
  *
  * Conventions
@@ -469,6 +470,118 @@ int ouro_weight_matvec_argmax(ouro_weight_t w, const float *x, float *y,
  * NaN; *idx is a device int32.  Uses 8 KiB of per-device scratch that
  * ouro_init allocates; the call allocates nothing. */
 int ouro_finite_argmax(const float *y, size_t n, int32_t *idx, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Attention of one new token over a caller's paged key-value cache     */
+/* ------------------------------------------------------------------ */
+
+/* A paged cache, described on the host; every pointer in it is a device
+ * pointer that the caller owns.  Slot j of sequence b is token
+ * j % page_tokens of page pages[b * max_pages + j / page_tokens], and head h
+ * of token t of page p is the head_dim elements at
+ *   p * page_stride + t * token_stride + h * head_stride
+ * of k and of v: [page][token][head] and [page][head][token] pools alike.  An
+ * id outside 0 .. n_pages - 1 is a hole: its slots hold nothing, are never
+ * read or written and count as masked.  k, v and the strides in bytes are
+ * multiples of 16 (OURO_ERR_ALIGN), head_dim a multiple of 8, 8 .. 256, and
+ * page_tokens a power of two (OURO_ERR_SHAPE). */
+typedef struct ouro_kv_cache {
+    void *k, *v;
+    const int32_t *pages;                            /* [seqs][max_pages] */
+    int64_t page_stride, token_stride, head_stride;  /* elements */
+    int32_t n_pages, max_pages, page_tokens, n_head_kv, head_dim;
+    int32_t dtype;                                   /* OURO_DT_F32 or OURO_DT_BF16 */
+} ouro_kv_cache;
+
+/* What eviction goes by: the attention weight that each slot has received and
+ * the position of the token in it, for each kv head by itself (heads =
+ * n_head_kv) or for all of them together (heads = 1). */
+typedef struct ouro_kv_history {
+    float *weight;          /* [seqs][heads][slots] */
+    int32_t *pos;           /* [seqs][heads][slots] */
+    int32_t heads, slots;
+} ouro_kv_history;
+
+/* Attention of one token a sequence (the reference's run_attn keeps its cache
+ * per head on the host, qwen35.rs:1187-1210): for query head h of sequence b,
+ * over its visible slots j < lens[b] (the page there, its mask byte not 0),
+ *   s_j = scale q.k_j, out = softmax(s) v [* sigmoid(gate)], lse = ln sum e^s,
+ * with kv head h / (n_head / n_head_kv).  Where no slot is visible out = 0
+ * and lse = -inf.  What lies in slots that are not visible (NaN, infinities)
+ * changes nothing.  The rows of a sequence do not depend on the batch it is
+ * in, and the same call gives the same bits.
+ *   q, out [seqs][n_head][head_dim] of `dtype`, rows q_stride and out_stride
+ *     elements apart; gate (or NULL) as q, q_stride apart too;
+ *   k_new, v_new (or both NULL) [seqs][n_head_kv][head_dim] of `dtype`, rows
+ *     new_stride apart: the new token's, written to slot lens[b] - 1 in the
+ *     cache's type (rounded to nearest even) before it is attended to;
+ *   lens [seqs] on the device: slots in use, the new one among them (read as
+ *     0 .. max_len); max_len bounds them on the host;
+ *   mask (or NULL) [seqs] rows of max_len bytes, mask_stride apart;
+ *   lse (or NULL) [seqs][n_head];
+ *   history (or NULL, with slots >= max_len): each visible slot's weight grows
+ *     by the sum of its softmax weights over the query heads of its history
+ *     head; with k_new the new slot's weight starts at 0 and its position
+ *     becomes pos_new[b].
+ * A stride of 0 stands for rows without a gap.  Pointers and strides of
+ * `dtype` rows are multiples of 16 bytes.  n_head is a multiple of n_head_kv,
+ * seqs at most 65535.  `workspace`: ouro_kv_attend_workspace_bytes() device
+ * bytes, 16-byte aligned; NULL takes the library's. */
+size_t ouro_kv_attend_workspace_bytes(size_t seqs, size_t n_head, size_t head_dim,
+                                      size_t max_len, int with_history);
+int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history,
+                   const void *q, size_t q_stride, const void *k_new,
+                   const void *v_new, size_t new_stride, const int32_t *pos_new,
+                   const int32_t *lens, const uint8_t *mask, size_t mask_stride,
+                   const void *gate, void *out, size_t out_stride, float *lse,
+                   int dtype, size_t seqs, size_t n_head, size_t max_len,
+                   float scale, void *workspace, void *stream);
+
+/* Cuts each sequence's cache to `keep` slots by accumulated attention weight.
+ * Of a history head's n = lens[b] slots those stay that come first by
+ * (position among the `recent` newest: pos > max pos - recent; larger weight;
+ * lower slot); a NaN weight counts least.  Slots are not shifted (attention
+ * does not depend on their order, and positions are in the history): the
+ * i-th slot below `keep` that goes is filled from the i-th slot at or above
+ * `keep` that stays, rows of k and v (of all kv heads where the history has
+ * one head) and history alike.  Sequences of at most `keep` slots stay as
+ * they are.  Slots at or above the new length are left as they were.
+ *   left (or NULL: the history itself) receives weight and pos of the slots
+ *     kept; its slots >= min(keep, max_len);
+ *   lens_out [seqs] = min(lens[b], keep), not the array lens;
+ *   slot_from (or NULL) [seqs][heads][keep]: the slot that each kept slot's
+ *     contents came from, -1 past the new length. */
+size_t ouro_kv_evict_workspace_bytes(size_t seqs, size_t heads, size_t max_len,
+                                     size_t keep);
+int ouro_kv_evict(const ouro_kv_cache *cache, const ouro_kv_history *history,
+                  const int32_t *lens, size_t seqs, size_t max_len, size_t keep,
+                  size_t recent, const ouro_kv_history *left, int32_t *lens_out,
+                  int32_t *slot_from, void *workspace, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Log probabilities of given tokens                                    */
+/* ------------------------------------------------------------------ */
+
+/* From rows of n logits (f32 or bf16, row_stride elements apart, 0: n; the
+ * head's output, where the reference samples greedily, qwen35.rs:746-757):
+ *   lse[row] = ln sum e^x;
+ *   logprob[row] = x_t - lse and rank[row] = the number of tokens ahead of t
+ *     by (larger logit, lower index), t = targets[row]; a t outside
+ *     0 .. n - 1 stands for no token: logprob 0, rank -1;
+ *   entropy[row] = -sum p ln p, in nats;
+ *   top_id, top_logprob [rows][k] (k <= 64): the k likeliest tokens in that
+ *     order, -1 and -inf where no further token has a logit above -inf.
+ * A NaN logit counts as -inf.  Where +inf logits are, they share the mass;
+ * where all are -inf, lse and the logprobs are -inf and the entropy 0.  Each
+ * output may be NULL (top_id and top_logprob only with k = 0).  n < 2^24.
+ * `workspace`: ouro_token_logprobs_workspace_bytes() device bytes, 16-byte
+ * aligned; NULL takes the library's. */
+size_t ouro_token_logprobs_workspace_bytes(size_t rows, size_t n, size_t k);
+int ouro_token_logprobs(const void *logits, int dtype, size_t rows, size_t n,
+                        size_t row_stride, const int32_t *targets, size_t k,
+                        float *logprob, int32_t *rank, float *entropy,
+                        float *lse, int32_t *top_id, float *top_logprob,
+                        void *workspace, void *stream);
 
 #ifdef __cplusplus
 }

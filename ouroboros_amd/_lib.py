@@ -48,6 +48,20 @@ class StackCard(C.Structure):
                                           "ssm_n_v_heads", "ssm_d_state")] + [("eps", C.c_float),
                                                                               ("rope_base", C.c_float)]
 
+
+
+class KvCacheDesc(C.Structure):
+    """ouro_kv_cache (include/ouro_hip.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "pages")] + \
+        [(n, C.c_int64) for n in ("page_stride", "token_stride", "head_stride")] + \
+        [(n, C.c_int32) for n in ("n_pages", "max_pages", "page_tokens", "n_head_kv", "head_dim", "dtype")]
+
+
+class KvHistoryDesc(C.Structure):
+    """ouro_kv_history (include/ouro_hip.h)."""
+    _fields_ = [("weight", C.c_void_p), ("pos", C.c_void_p), ("heads", C.c_int32), ("slots", C.c_int32)]
+
+
 # name -> (restype, argtypes); every function of include/ouro_hip.h.
 SIGNATURES = {
     "ouro_stack_create": (i32, [C.POINTER(StackCard), u32, sz, sz, sz, sz, vp]),
@@ -97,6 +111,12 @@ SIGNATURES = {
     "ouro_gdn_layer_workspace_bytes": (sz, [sz, sz, sz, sz]),
     "ouro_gdn_layer_decode": (i32, [vp] * 11 + [sz, sz, sz, sz, u32, f32, vp, vp]),
     "ouro_gdn_chunk_prefill": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, u32, f32, vp, vp]),
+    "ouro_kv_attend_workspace_bytes": (sz, [sz, sz, sz, sz, i32]),
+    "ouro_kv_attend": (i32, [vp, vp, vp, sz, vp, vp, sz, vp, vp, vp, sz, vp, vp, sz, vp, i32, sz, sz, sz, f32, vp, vp]),
+    "ouro_kv_evict_workspace_bytes": (sz, [sz, sz, sz, sz]),
+    "ouro_kv_evict": (i32, [vp, vp, vp, sz, sz, sz, sz, vp, vp, vp, vp, vp]),
+    "ouro_token_logprobs_workspace_bytes": (sz, [sz, sz, sz]),
+    "ouro_token_logprobs": (i32, [vp, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp]),
     "ouro_weight_upload": (i32, [i32, vp, sz, sz, sz, f32, sz, C.POINTER(vp)]),
     "ouro_weight_free": (i32, [vp]),
     "ouro_weight_payload": (vp, [vp]),
@@ -105,6 +125,17 @@ SIGNATURES = {
     "ouro_weight_matvec": (i32, [vp, vp, vp, vp]),
     "ouro_weight_matmul": (i32, [vp, vp, sz, vp, vp]),
 }
+
+DTYPES = {"f32": DT_F32, "bf16": DT_BF16, DT_F32: DT_F32, DT_BF16: DT_BF16}
+
+
+def dtype_code(dtype) -> int:
+    """DT_F32 / DT_BF16 of "f32" / "bf16" (or of the code itself)."""
+    try:
+        return DTYPES[dtype]
+    except (KeyError, TypeError):
+        raise ValueError(f"dtype {dtype!r}: 'f32' or 'bf16'") from None
+
 
 _LIB: C.CDLL | None = None
 

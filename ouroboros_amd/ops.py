@@ -172,3 +172,41 @@ def finite_argmax(y) -> int:
     idx = DeviceBuffer((1,), np.int32)
     call("ouro_finite_argmax", yb.ptr, yb.nbytes // yb.dtype.itemsize, idx.ptr, None)
     return int(idx.download()[0])
+
+
+def _addr(a):
+    return a.ptr if isinstance(a, DeviceBuffer) else a
+
+
+def token_logprobs(logits, rows: int, n: int, *, dtype="f32", row_stride: int = 0, targets=None, k: int = 0,
+                   logprob=None, rank=None, entropy=None, lse=None, top_id=None, top_logprob=None, workspace=None,
+                   stream=None):
+    """Log probabilities of given tokens, their rank, the entropy and the k
+    likeliest alternatives of rows of logits (ouro_token_logprobs).
+
+    With device memory (DeviceBuffer, or the address of another runtime's) the
+    outputs that are given are written, nothing is returned.  With numpy logits
+    (f32, or bf16 as uint16) everything is computed and returned as a dict of
+    numpy arrays, logprob and rank where targets are given."""
+    if not isinstance(logits, np.ndarray):
+        call("ouro_token_logprobs", _addr(logits), _lib.dtype_code(dtype), rows, n, row_stride, _addr(targets), k,
+             _addr(logprob), _addr(rank), _addr(entropy), _addr(lse), _addr(top_id), _addr(top_logprob),
+             _addr(workspace), stream)
+        return None
+    half = logits.dtype == np.uint16
+    xb, _ = _dev(logits, np.uint16 if half else np.float32)
+    if xb.nbytes < rows * n * xb.dtype.itemsize or row_stride not in (0, n):
+        raise ValueError(f"host logits are {rows} whole rows of {n}")
+    out = {"entropy": DeviceBuffer((rows,), np.float32), "lse": DeviceBuffer((rows,), np.float32)}
+    tb = None
+    if targets is not None:
+        tb, _ = _dev(targets, np.int32)
+        if tb.nbytes != rows * 4:
+            raise ValueError(f"{rows} rows need {rows} targets")
+        out.update(logprob=DeviceBuffer((rows,), np.float32), rank=DeviceBuffer((rows,), np.int32))
+    if k:
+        out.update(top_id=DeviceBuffer((rows, k), np.int32), top_logprob=DeviceBuffer((rows, k), np.float32))
+    token_logprobs(xb, rows, n, dtype="bf16" if half else "f32", targets=tb, k=k, stream=stream, **out)
+    if stream is not None:
+        call("ouro_stream_synchronize", stream)
+    return {name: b.download() for name, b in out.items()}
