@@ -46,6 +46,17 @@ int kv_check_history(const ouro_kv_history *h, int n_head_kv, size_t need, const
 
 namespace {
 
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kSplit = 256;  // slots of a workgroup
+constexpr int kQ = 16;       // query heads of a workgroup: the columns of its products
+constexpr int kJoin = 8;     // query heads that the wavefronts' outputs are joined for at a time
+
 struct AttendArgs {
     KvView c;
     const void *q, *k_new, *v_new, *gate;
@@ -54,13 +65,16 @@ struct AttendArgs {
     void *out;
     float *lse, *weight;
     int32_t *pos;
-    int64_t q_stride, new_stride, mask_stride, out_stride;
-    int32_t n_head, max_len, h_heads, h_slots;
+    float *part;   // [seqs][n_head][n_split][d]: the splits' outputs, not normalised
+    float2 *ml;    // [seqs][n_head][n_split]: their maxima (of scores times log2 e) and sums
+    float *score;  // [seqs][n_head][s_stride]: scores times log2 e, where there is a history
+    int64_t q_stride, new_stride, mask_stride, out_stride, s_stride;
+    int32_t n_head, max_len, h_heads, h_slots, n_split, q_tiles;
     float scale;
     int32_t pad;
 };
 // passed by value to kernels: the host and device passes must lay it out alike
-static_assert(sizeof(AttendArgs) == 216, "AttendArgs: kernel argument layout");
+static_assert(sizeof(AttendArgs) == 256, "AttendArgs: kernel argument layout");
 
 template <typename T>
 __device__ __forceinline__ float load1(const T *p, int64_t i) {
@@ -76,138 +90,512 @@ __device__ __forceinline__ void store1(T *p, int64_t i, float x) {
     else
         p[i] = f32_to_bf16_bits(x);
 }
-__device__ __forceinline__ float wave_sum(float v) {
+// Eight (N = 8) or four adjacent values of a row, from 16-byte aligned rows.
+template <int N, typename T>
+__device__ __forceinline__ void load_row(const T *p, float (&x)[N]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += xor_shfl(v, off);
-    return v;
+        for (int i = 0; i < N; i += 4) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x2_t v = *reinterpret_cast<const u32x2_t *>(p + i);
+            x[i] = __uint_as_float(v[0] << 16), x[i + 1] = __uint_as_float(v[0] & 0xffff0000u);
+            x[i + 2] = __uint_as_float(v[1] << 16), x[i + 3] = __uint_as_float(v[1] & 0xffff0000u);
+        }
+    }
+}
+// Two floats as bf16, rounded to nearest even, in one dword.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+}
+// x as a sum of N bf16 operands, each the rounding of what the ones before
+// leave (the differences are exact): 8 bits of the significand apiece, so three
+// hold a float whole and two hold it to 2^-17.
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8_t (&s)[N]) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+            if (k + 1 < N) {
+                r[2 * i] -= __uint_as_float(w[i] << 16);
+                r[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+        s[k] = __builtin_bit_cast(bf16x8_t, w);
+    }
+}
+// Maximum and sum over the four lanes l, l + 16, l + 32, l + 48.
+__device__ __forceinline__ float quad_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 __device__ __forceinline__ int slots_of(const AttendArgs &a, int64_t b) { return max(0, min(a.lens[b], a.max_len)); }
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-// The new token's rows into slot n - 1, its weight cleared and its position
-// noted.  One workgroup a (kv head, sequence).
-template <typename C, typename IO>
-__global__ __launch_bounds__(256) void kv_append_kernel(AttendArgs a) {
-    const int h = blockIdx.x, t = threadIdx.x;
-    const int64_t b = blockIdx.y;
-    const int n = slots_of(a, b);
-    if (!n) return;
-    const int64_t at = kv_slot(a.c, b, n - 1);
-    if (at >= 0 && t < a.c.d) {
-        const int64_t src = b * a.new_stride + static_cast<int64_t>(h) * a.c.d + t, dst = at + h * a.c.head_stride + t;
-        store1(static_cast<C *>(a.c.k), dst, load1(static_cast<const IO *>(a.k_new), src));
-        store1(static_cast<C *>(a.c.v), dst, load1(static_cast<const IO *>(a.v_new), src));
-    }
-    if (a.weight && h < a.h_heads && t == 0) {
-        const int64_t i = (b * a.h_heads + h) * a.h_slots + n - 1;
-        a.weight[i] = 0.f;
-        a.pos[i] = a.pos_new[b];
-    }
+// A head's joined output (normalised), through the gate to its place.
+template <typename IO>
+__device__ __forceinline__ void store_out(const AttendArgs &a, int64_t b, int h, int dim, float o) {
+    const int64_t i = static_cast<int64_t>(h) * a.c.d + dim;
+    if (a.gate) o *= sigmoid(load1(static_cast<const IO *>(a.gate), b * a.q_stride + i));
+    store1(static_cast<IO *>(a.out), b * a.out_stride + i, o);
+}
+__device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h, float m, float l) {
+    if (a.lse) a.lse[b * a.n_head + h] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// One workgroup a (query head, sequence): wavefront w takes slots w, w + 4,
-// ... with lane l on dims l, l + 64, .. and keeps its own running maximum,
-// sum and output; the four are joined in LDS.
-template <typename C, typename IO>
-__global__ __launch_bounds__(256) void kv_attend_kernel(AttendArgs a) {
-    __shared__ float os[4][256], ms[4], ls[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int h = blockIdx.x, d = a.c.d;
-    const int64_t b = blockIdx.y;
-    const int kvh = h / (a.n_head / a.c.n_head_kv);
-    const int n = slots_of(a, b);
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        q[i] = lane + 64 * i < d
-                   ? load1(static_cast<const IO *>(a.q), b * a.q_stride + static_cast<int64_t>(h) * d + lane + 64 * i)
-                   : 0.f;
-    float m = -INFINITY, l = 0.f;
-    for (int j = wave; j < n; j += 4) {
-        if (a.mask && !a.mask[b * a.mask_stride + j]) continue;
-        int64_t at = kv_slot(a.c, b, j);
-        if (at < 0) continue;
-        at += kvh * a.c.head_stride;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < d) s += q[i] * load1(static_cast<const C *>(a.c.k), at + lane + 64 * i);
-        s = wave_sum(s) * a.scale;
-        const float mn = fmaxf(m, s);
-        if (mn == -INFINITY) continue;
-        const float f = expf(m - mn), p = expf(s - mn);
-        m = mn;
-        l = l * f + p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < d) o[i] = o[i] * f + p * load1(static_cast<const C *>(a.c.v), at + lane + 64 * i);
-    }
-    if (lane == 0) ms[wave] = m, ls[wave] = l;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) os[wave][lane + 64 * i] = o[i];
-    __syncthreads();
-    const float M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-    float L = 0.f, f[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = ms[w] == -INFINITY ? 0.f : expf(ms[w] - M);
-        L += f[w] * ls[w];
-    }
-    const int t = threadIdx.x;
-    if (t < d) {
-        float r = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) r += f[w] * os[w][t];
-        r = L != 0.f ? r / L : 0.f;
-        const int64_t i = b * a.out_stride + static_cast<int64_t>(h) * d + t;
-        if (a.gate) r *= 1.0f / (1.0f + expf(-load1(static_cast<const IO *>(a.gate), b * a.q_stride + static_cast<int64_t>(h) * d + t)));
-        store1(static_cast<IO *>(a.out), i, r);
-    }
-    if (t == 0) a.lse[b * a.n_head + h] = M + logf(L);
-}
-
-// Adds each slot's attention weight to the history: one wavefront a slot, over
-// the query heads of its history head, by the heads' log-sum-exp.
-template <typename C, typename IO>
-__global__ __launch_bounds__(256) void kv_weight_kernel(AttendArgs a) {
-    const int lane = threadIdx.x & 63, d = a.c.d;
-    const int j = blockIdx.x * 4 + (threadIdx.x >> 6), hs = blockIdx.y;
+// One workgroup a split of kSplit slots, (kv head, tile of 16 query heads) and
+// sequence, its four wavefronts on alternate tiles of slots (32 of bf16, 16 of
+// fp32), each with its own running maximum, sum and output.
+//
+// Both products run on the matrix cores with the slots as rows of the first
+// and as the inner axis of the second, the query heads as columns:
+//   S^T[slot][head] = K Q^T, O^T[dim][head] += V^T P^T.
+// A lane of S^T holds one head (lane % 16) and slots 4 (lane / 16) + 0 .. 3 of
+// each 16, and that is the order in which V's rows are loaded, so the scores
+// become the second product's operand without leaving their registers.  A
+// bf16 row of V is loaded with eight (DP = 64: four) adjacent dims a lane, 16
+// lanes a row, and pairs of rows are merged by byte permutes into operands of
+// one dim and eight slots; fp32 operands hold one slot and need none.
+// fp32 queries and weights against a bf16 cache are split into three bf16
+// operands (exact), weights for a bf16 output into two (2^-17); everything
+// else is fp32.
+template <typename C, typename IO, int DP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 4 : DP <= 128 ? 3 : 2))) void kv_attend_split_kernel(AttendArgs a) {
+    constexpr bool kHalf = sizeof(C) == 2;
+    constexpr int TS = kHalf ? 32 : 16;                   // slots of a tile
+    constexpr int NT = TS / 16;
+    constexpr int KC = kHalf ? 8 : 4;                     // dims of a lane's 16 bytes of K
+    constexpr int NJ = DP / (4 * KC);                     // steps over the dims
+    constexpr int NQ = kHalf && sizeof(IO) == 4 ? 3 : 1;  // operands of a query
+    constexpr int NP = sizeof(IO) == 4 ? 3 : 2;           // and of a weight (bf16 cache)
+    constexpr int CH = kHalf && DP > 64 ? 8 : 4;          // adjacent dims of V a lane
+    constexpr int NB = DP / (16 * CH);
+    constexpr int NR = TS / 4;                            // slots of a lane
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // queries, then the wavefronts' outputs
+    __shared__ int64_t at[kSplit];  // element offset of each slot's row, -1 where it is not visible
+    __shared__ float sm[4][kQ], sl[4][kQ];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, g = lane >> 4;
     const int64_t b = blockIdx.z;
-    if (j >= slots_of(a, b)) return;
-    if (a.mask && !a.mask[b * a.mask_stride + j]) return;
-    const int64_t row = kv_slot(a.c, b, j);
-    if (row < 0) return;
-    const int G = a.n_head / a.h_heads, per = a.n_head / a.c.n_head_kv;
-    float w = 0.f;
-    for (int h = hs * G; h < hs * G + G; ++h) {
-        const int64_t at = row + (h / per) * a.c.head_stride;
-        float s = 0.f;
-        for (int i = lane; i < d; i += 64)
-            s += load1(static_cast<const IO *>(a.q), b * a.q_stride + static_cast<int64_t>(h) * d + i) *
-                 load1(static_cast<const C *>(a.c.k), at + i);
-        s = wave_sum(s) * a.scale;
-        if (s != -INFINITY) w += expf(s - a.lse[b * a.n_head + h]);
+    const int kvh = static_cast<int>(blockIdx.y) / a.q_tiles, qt = static_cast<int>(blockIdx.y) % a.q_tiles;
+    const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
+    const int h0 = kvh * G + qt * kQ, nq = min(kQ, G - qt * kQ);  // heads h0 .. h0 + nq - 1
+    const int j0 = static_cast<int>(blockIdx.x) * kSplit;
+    // the slots' rows: page and mask are read without waiting for the length
+    const int slot = min(j0 + tid, a.max_len - 1);
+    int64_t off = -1;
+    bool seen = true;
+    if (slot >= 0) {
+        off = kv_slot(a.c, b, slot);
+        if (a.mask) seen = a.mask[b * a.mask_stride + slot] != 0;
     }
-    if (lane == 0) a.weight[(b * a.h_heads + hs) * a.h_slots + j] += w;
+    const int n = slots_of(a, b);
+    if (j0 >= n && j0 > 0) return;  // whole workgroup; an empty sequence's first split writes its zeros
+    if (off >= 0) off += kvh * a.c.head_stride;
+    const bool live = j0 + tid < n;
+    at[tid] = live && seen ? off : -1;
+    const int fresh = a.k_new && n - 1 - j0 < kSplit ? n - 1 - j0 : -1;  // the new token's place in the split
+    if (fresh >= 0 && qt == 0) {
+        // its rows into the cache; this launch takes them from k_new and v_new
+        const int64_t to = kv_slot(a.c, b, n - 1);
+        if (tid < d && to >= 0) {
+            const int64_t src = b * a.new_stride + static_cast<int64_t>(kvh) * d + tid, dst = to + kvh * a.c.head_stride + tid;
+            store1(static_cast<C *>(a.c.k), dst, load1(static_cast<const IO *>(a.k_new), src));
+            store1(static_cast<C *>(a.c.v), dst, load1(static_cast<const IO *>(a.v_new), src));
+        }
+        if (a.weight && kvh < a.h_heads && tid == 0) {
+            const int64_t i = (b * a.h_heads + kvh) * a.h_slots + n - 1;
+            a.weight[i] = 0.f;
+            a.pos[i] = a.pos_new[b];
+        }
+    }
+    // the queries as second operands: head r, dims 4 KC j + KC g .. of step j
+    for (int i = tid; i < NJ * 64; i += 256) {
+        const int jr = i & 15, dim = (i >> 6) * (4 * KC) + ((i >> 4) & 3) * KC;
+        float x[KC];
+#pragma unroll
+        for (int e = 0; e < KC; ++e) x[e] = 0.f;
+        if (jr < nq && dim < d) load_row<KC>(static_cast<const IO *>(a.q) + b * a.q_stride + static_cast<int64_t>(h0 + jr) * d + dim, x);
+        if constexpr (kHalf) {
+            bf16x8_t s[NQ];
+            split8<NQ>(x, s);
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) reinterpret_cast<bf16x8_t *>(lds)[k * NJ * 64 + i] = s[k];
+        } else {
+            reinterpret_cast<f32x4_t *>(lds)[i] = f32x4_t{x[0], x[1], x[2], x[3]};
+        }
+    }
+    __syncthreads();
+
+    f32x4_t o[NB][CH];  // o[nb][e][i]: dim 16 CH nb + CH (4 g + i) + e of head r
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < CH; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    const C *kp = static_cast<const C *>(a.c.k), *vp = static_cast<const C *>(a.c.v);
+    const int used = min(n - j0, kSplit);
+    for (int base = TS * wave; base < used; base += 4 * TS) {
+        int64_t ka[NT], va[NR];  // rows of K (slot 16 t + r) and V (slots 16 t + 4 g + i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) ka[t] = at[base + 16 * t + r];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) va[i] = at[base + 16 * (i >> 2) + 4 * g + (i & 3)];
+        bool all = true, any = false;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) all &= va[i] >= 0, any |= va[i] >= 0;
+        all = __all(all);
+        f32x4_t sc[NT];
+        float *srow = a.score ? a.score + (b * a.n_head + h0 + r) * a.s_stride + j0 + base + 4 * g : nullptr;
+        if (!__any(any)) {
+            if (srow && r < nq)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    *reinterpret_cast<f32x4_t *>(srow + 16 * t) = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            continue;
+        }
+        // rows that are not visible: any row that is there; scores and V's
+        // values of them are replaced below
+        u32x4_t kf[NT][NJ];
+        typedef uint32_t vch_t __attribute__((ext_vector_type(CH * sizeof(C) / 4)));
+        vch_t vf[NR][NB];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const C *row = kp + (ka[t] < 0 ? 0 : ka[t]);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                kf[t][j] = *reinterpret_cast<const u32x4_t *>(row + (d == DP ? 4 * KC * j + KC * g : min(4 * KC * j + KC * g, d - KC)));
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const C *row = vp + (va[i] < 0 ? 0 : va[i]);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) vf[i][nb] = *reinterpret_cast<const vch_t *>(row + min(16 * CH * nb + CH * r, d - CH));
+        }
+        if (fresh >= base && fresh < base + TS) {
+            // the new token's row, as the cache stores it
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (base + 16 * t + r == fresh) {
+                    const IO *row = static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        float x[KC];
+                        load_row<KC>(row + min(4 * KC * j + KC * g, d - KC), x);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            if constexpr (kHalf)
+                                kf[t][j][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
+                            else
+                                kf[t][j][w] = __float_as_uint(x[w]);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (base + 16 * (i >> 2) + 4 * g + (i & 3) == fresh) {
+                    const IO *row = static_cast<const IO *>(a.v_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        float x[CH];
+                        load_row<CH>(row + min(16 * CH * nb + CH * r, d - CH), x);
+#pragma unroll
+                        for (int w = 0; w < static_cast<int>(CH * sizeof(C) / 4); ++w)
+                            if constexpr (kHalf)
+                                vf[i][nb][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
+                            else
+                                vf[i][nb][w] = __float_as_uint(x[w]);
+                    }
+                }
+        }
+        if (d != DP) {  // dims past d of a visible row count as 0, whatever stands there
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                if (4 * KC * j + KC * g >= d)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) kf[t][j] = u32x4_t{0, 0, 0, 0};
+        }
+        // the queries are read from LDS for every tile: held in registers they
+        // would take 48 of them (bf16 cache, fp32 queries, DP = 128)
+        asm volatile("" ::: "memory");
+        // S^T: sc[t][e] = score of slot base + 16 t + 4 g + e against head r
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if constexpr (kHalf) {
+#pragma unroll
+                for (int k = 0; k < NQ; ++k) {
+                    const bf16x8_t q = reinterpret_cast<const bf16x8_t *>(lds)[(k * NJ + j) * 64 + lane];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[t][j]), q, sc[t], 0, 0, 0);
+                }
+            } else {
+                const f32x4_t q = reinterpret_cast<const f32x4_t *>(lds)[j * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[0][j][e]), q[e], sc[0], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t] *= sl2;
+        if (!all) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (va[i] < 0) {
+                    sc[i >> 2][i & 3] = -INFINITY;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) vf[i][nb] = vch_t(0);
+                }
+        }
+        if (srow && r < nq)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t *>(srow + 16 * t) = sc[t];
+        // running maximum and sum of head r in base 2
+        float mx = sc[0][0];
+#pragma unroll
+        for (int i = 1; i < NR; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
+        const float mn = fmaxf(m, quad_max(mx));
+        const float mref = mn == -INFINITY ? 0.f : mn;  // no finite score yet: avoid inf - inf
+        const float corr = __builtin_amdgcn_exp2f(m - mref);
+        m = mn;
+        float ps = 0.f, p[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(sc[i >> 2][i & 3] - mref);
+            ps += p[i];
+        }
+        l = l * corr + quad_sum(ps);
+        if (!__all(corr == 1.0f)) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < CH; ++e) o[nb][e] *= corr;
+        }
+        // O^T += V^T P^T
+        if constexpr (kHalf) {
+            bf16x8_t pf[NP];
+            split8<NP>(p, pf);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < CH; ++e) {
+                    u32x4_t w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = __builtin_amdgcn_perm(vf[2 * i + 1][nb][e >> 1], vf[2 * i][nb][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int k = 0; k < NP; ++k)
+                        o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), pf[k], o[nb][e], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][nb][e]), p[i], o[nb][e], 0, 0, 0);
+        }
+    }
+
+    // the four wavefronts' outputs joined, kJoin heads at a time
+    if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
+    constexpr int OS = DP + 4;  // floats of a row: padded, so that the heads' rows start in different banks
+    float *ob = reinterpret_cast<float *>(lds);
+    const bool whole = n <= kSplit;  // the sequence's only split
+    for (int q0 = 0; q0 < nq; q0 += kJoin) {
+        __syncthreads();  // the queries, or the heads before, have been read
+        if (r >= q0 && r < min(nq, q0 + kJoin)) {
+            float *row = ob + (wave * kJoin + r - q0) * OS;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < CH; e += 4)
+                        *reinterpret_cast<f32x4_t *>(row + 16 * CH * nb + CH * (4 * g + i) + e) =
+                            f32x4_t{o[nb][e][i], o[nb][e + 1][i], o[nb][e + 2][i], o[nb][e + 3][i]};
+        }
+        __syncthreads();
+        const int dim = tid % DP;
+        for (int q = q0 + tid / DP; q < min(nq, q0 + kJoin); q += 256 / DP) {
+            const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
+            float L = 0.f, x = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
+                L += f * sl[w][q];
+                x += f * ob[(w * kJoin + q - q0) * OS + dim];
+            }
+            if (dim >= d) continue;
+            const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + blockIdx.x;
+            if (dim == 0 && a.ml) a.ml[rec] = make_float2(M, L);
+            if (whole) {
+                store_out<IO>(a, b, h0 + q, dim, M == -INFINITY ? 0.f : x / L);
+                if (dim == 0) store_lse(a, b, h0 + q, M, L);
+            } else {
+                a.part[rec * d + dim] = x;
+            }
+        }
+    }
 }
 
+// Maximum and sum of a head over its splits, by one wavefront, to every lane.
+__device__ __forceinline__ float2 join_ml(const float2 *ml, int ns) {
+    const int lane = threadIdx.x & 63;
+    float M = -INFINITY, L = 0.f;
+    for (int s = lane; s < ns; s += 64) {
+        const float2 x = ml[s];
+        const float mn = fmaxf(M, x.x);
+        if (mn != -INFINITY || x.x != x.x) {
+            L = L * __builtin_amdgcn_exp2f(M - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
+            M = mn;
+        }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        const float m2 = xor_shfl(M, off), l2 = xor_shfl(L, off), mn = fmaxf(M, m2);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        L = L * __builtin_amdgcn_exp2f(M - ref) + l2 * __builtin_amdgcn_exp2f(m2 - ref);
+        M = mn;
+    }
+    return make_float2(M, L);
+}
+
+// The splits of (head, sequence) joined: a thread takes four dims of every
+// (1024 / DP)-th split.
+template <typename IO, int DP>
+__global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a) {
+    __shared__ f32x4_t red[256];
+    const int64_t b = blockIdx.y;
+    const int h = blockIdx.x, tid = threadIdx.x, d = a.c.d;
+    const int ns = (slots_of(a, b) + kSplit - 1) / kSplit;
+    if (ns <= 1) return;  // written by its only split
+    constexpr int DL = DP / 4, NG = 256 / DL;
+    const int64_t rec = (b * a.n_head + h) * a.n_split;
+    const float2 t = join_ml(a.ml + rec, ns);
+    const float ref = t.x == -INFINITY ? 0.f : t.x;
+    const int dim = 4 * (tid % DL);
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+    if (dim < d)
+        for (int s = tid / DL; s < ns; s += NG) {
+            const float f = __builtin_amdgcn_exp2f(a.ml[rec + s].x - ref);
+            x += f * *reinterpret_cast<const f32x4_t *>(a.part + (rec + s) * d + dim);
+        }
+    red[tid] = x;
+    __syncthreads();
+    if (tid >= DP) return;
+    float o = 0.f;
+#pragma unroll
+    for (int s = 0; s < NG; ++s) o += red[s * DL + tid / 4][tid % 4];
+    if (tid < d) store_out<IO>(a, b, h, tid, t.x == -INFINITY ? 0.f : o / t.y);
+    if (tid == 0) store_lse(a, b, h, t.x, t.y);
+}
+
+// Each slot's attention weight, summed over the query heads of its history
+// head, onto the history: by the scores that the splits left and the heads'
+// joined maxima and sums.  kWSlots slots a workgroup.
+constexpr int kWSlots = 512, kWHeads = 64;
+__global__ __launch_bounds__(256) void kv_weight_kernel(AttendArgs a) {
+    __shared__ float2 ml[kWHeads];
+    const int64_t b = blockIdx.z;
+    const int hs = blockIdx.y, j0 = static_cast<int>(blockIdx.x) * kWSlots, tid = threadIdx.x;
+    const int n = slots_of(a, b);
+    if (j0 >= n) return;
+    const int ns = (n + kSplit - 1) / kSplit, G = a.n_head / a.h_heads;
+    float w[kWSlots / 256];
+#pragma unroll
+    for (int i = 0; i < kWSlots / 256; ++i) w[i] = 0.f;
+    for (int g0 = 0; g0 < G; g0 += kWHeads) {
+        const int ng = min(kWHeads, G - g0);
+        const int64_t h0 = b * a.n_head + static_cast<int64_t>(hs) * G + g0;
+        __syncthreads();
+        for (int i = tid >> 6; i < ng; i += 4) {
+            const float2 t = join_ml(a.ml + (h0 + i) * a.n_split, ns);
+            // nothing visible: every score is -inf, and 2^(-inf - 0) = 0
+            if ((tid & 63) == 0) ml[i] = t.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(t.x, 1.0f / t.y);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWSlots / 256; ++i) {
+            const int j = j0 + 256 * i + tid;
+            if (j < n)
+                for (int k = 0; k < ng; ++k) w[i] += __builtin_amdgcn_exp2f(a.score[(h0 + k) * a.s_stride + j] - ml[k].x) * ml[k].y;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kWSlots / 256; ++i) {
+        const int j = j0 + 256 * i + tid;
+        if (j < n) a.weight[(b * a.h_heads + hs) * a.h_slots + j] += w[i];
+    }
+}
+
+template <typename C, typename IO, int DP>
+int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
+    constexpr bool kHalf = sizeof(C) == 2;
+    constexpr size_t q_bytes = kHalf ? (sizeof(IO) == 4 ? 3 : 1) * DP * 32 : DP * 64;
+    constexpr size_t o_bytes = 4 * kJoin * (DP + 4) * sizeof(float);
+    constexpr size_t lds = q_bytes > o_bytes ? q_bytes : o_bytes;
+    static_assert(lds + kSplit * 8 + 2 * 4 * kQ * 4 <= 65536, "LDS without an opt-in");
+    hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP>), dim3(a.n_split, a.c.n_head_kv * a.q_tiles, seqs), dim3(256), lds, s, a);
+    int st = check_launch("kv_attend_split_kernel");
+    if (st) return st;
+    if (a.n_split > 1) {
+        hipLaunchKernelGGL((kv_attend_join_kernel<IO, DP>), dim3(a.n_head, seqs), dim3(256), 0, s, a);
+        if ((st = check_launch("kv_attend_join_kernel"))) return st;
+    }
+    if (a.weight) {
+        hipLaunchKernelGGL(kv_weight_kernel, dim3((a.max_len + kWSlots - 1) / kWSlots, a.h_heads, seqs), dim3(256), 0, s, a);
+        st = check_launch("kv_weight_kernel");
+    }
+    return st;
+}
 template <typename C, typename IO>
 int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
-    int st;
-    if (a.k_new) {
-        hipLaunchKernelGGL((kv_append_kernel<C, IO>), dim3(a.c.n_head_kv, seqs), dim3(256), 0, s, a);
-        if ((st = check_launch("kv_append_kernel"))) return st;
-    }
-    hipLaunchKernelGGL((kv_attend_kernel<C, IO>), dim3(a.n_head, seqs), dim3(256), 0, s, a);
-    if ((st = check_launch("kv_attend_kernel"))) return st;
-    if (a.weight && a.max_len) {
-        hipLaunchKernelGGL((kv_weight_kernel<C, IO>), dim3((a.max_len + 3) / 4, a.h_heads, seqs), dim3(256), 0, s, a);
-        if ((st = check_launch("kv_weight_kernel"))) return st;
-    }
-    return OURO_OK;
+    if (a.c.d <= 64) return launch_attend<C, IO, 64>(a, seqs, s);
+    if (a.c.d <= 128) return launch_attend<C, IO, 128>(a, seqs, s);
+    return launch_attend<C, IO, 256>(a, seqs, s);
 }
 
-size_t attend_ws_bytes(size_t seqs, size_t n_head) { return (seqs * n_head * sizeof(float) + 255) & ~size_t{255}; }
+// The workspace: the splits' maxima and sums, their outputs, the scores.
+struct AttendWs {
+    size_t ml, part, score, bytes;
+    int n_split;
+    int64_t s_stride;
+};
+AttendWs attend_ws(size_t seqs, size_t n_head, size_t d, size_t max_len, bool history) {
+    AttendWs w{};
+    const size_t rows = seqs * n_head, ns = max_len ? (max_len + kSplit - 1) / kSplit : 1;
+    auto up = [](size_t x) { return (x + 255) & ~size_t{255}; };
+    w.n_split = static_cast<int>(ns);
+    w.s_stride = static_cast<int64_t>((max_len + 31) / 32 * 32);  // whole tiles are stored
+    w.part = ns > 1 || history ? up(rows * ns * sizeof(float2)) : 0;
+    w.score = w.part + (ns > 1 ? up(rows * ns * d * sizeof(float)) : 0);
+    w.bytes = w.score + (history ? up(rows * w.s_stride * sizeof(float)) : 0);
+    return w;
+}
 
 }  // namespace
 }  // namespace ouro
@@ -217,10 +605,7 @@ using namespace ouro;
 extern "C" {
 
 size_t ouro_kv_attend_workspace_bytes(size_t seqs, size_t n_head, size_t head_dim, size_t max_len, int with_history) {
-    (void)head_dim;
-    (void)max_len;
-    (void)with_history;
-    return attend_ws_bytes(seqs, n_head);
+    return attend_ws(seqs, n_head, head_dim, max_len, with_history != 0).bytes;
 }
 
 int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history, const void *q, size_t q_stride,
@@ -262,10 +647,18 @@ int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history, c
         a.h_slots = history->slots;
     }
     if (!seqs) return OURO_OK;
-    if (!lse) {
-        if (!ws && !(ws = workspace(attend_ws_bytes(seqs, n_head), stream))) return OURO_ERR_HIP;
-        lse = static_cast<float *>(ws);
+    if (!max_len) a.weight = nullptr;  // no slots to weigh
+    const AttendWs w = attend_ws(seqs, n_head, d, max_len, history != nullptr);
+    if (w.bytes) {
+        if (!ws && !(ws = workspace(w.bytes, stream))) return OURO_ERR_HIP;
+        unsigned char *p = static_cast<unsigned char *>(ws);
+        a.ml = reinterpret_cast<float2 *>(p);
+        if (w.n_split > 1) a.part = reinterpret_cast<float *>(p + w.part);
+        if (history) a.score = reinterpret_cast<float *>(p + w.score);
     }
+    a.s_stride = w.s_stride;
+    a.n_split = w.n_split;
+    a.q_tiles = static_cast<int>((n_head / hkv + kQ - 1) / kQ);
     a.q = q, a.k_new = k_new, a.v_new = v_new, a.gate = gate, a.pos_new = pos_new, a.lens = lens, a.mask = mask, a.out = out, a.lse = lse;
     a.q_stride = q_stride, a.new_stride = new_stride, a.mask_stride = mask_stride, a.out_stride = out_stride;
     a.n_head = static_cast<int>(n_head), a.max_len = static_cast<int>(max_len), a.scale = scale;
