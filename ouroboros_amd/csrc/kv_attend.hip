@@ -23,8 +23,8 @@ int kv_view(const ouro_kv_cache *c, const char *what, KvView *out) {
     if (c->page_tokens < 1 || c->page_tokens > (1 << 20) || (c->page_tokens & (c->page_tokens - 1)))
         return fail(OURO_ERR_SHAPE, "%s: %d tokens a page (a power of two up to 2^20)", what, c->page_tokens);
     const int64_t unit = c->dtype == OURO_DT_F32 ? 4 : 8;  // elements in 16 bytes
-    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0)
-        return fail(OURO_ERR_SHAPE, "%s: negative stride", what);
+    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->token_stride > (1 << 24))
+        return fail(OURO_ERR_SHAPE, "%s: a negative stride, or tokens over 2^24 elements apart", what);
     if (c->page_stride % unit || c->token_stride % unit || c->head_stride % unit ||
         (reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
         return fail(OURO_ERR_ALIGN, "%s: pools and their strides must be multiples of 16 bytes", what);
@@ -152,6 +152,13 @@ __device__ __forceinline__ float quad_sum(float v) {
 __device__ __forceinline__ int slots_of(const AttendArgs &a, int64_t b) { return max(0, min(a.lens[b], a.max_len)); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
+// x, as a value that is made where this stands: what is computed from it stays
+// in the loop instead of being kept in registers throughout it.
+__device__ __forceinline__ int in_loop(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A head's joined output (normalised), through the gate to its place.
 template <typename IO>
 __device__ __forceinline__ void store_out(const AttendArgs &a, int64_t b, int h, int dim, float o) {
@@ -179,11 +186,12 @@ __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h,
 // fp32 queries and weights against a bf16 cache are split into three bf16
 // operands (exact), weights for a bf16 output into two (2^-17); everything
 // else is fp32.
-template <typename C, typename IO, int DP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 4 : DP <= 128 ? 3 : 2))) void kv_attend_split_kernel(AttendArgs a) {
+template <typename C, typename IO, int DP, bool Paged>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 4 : DP <= 128 ? 2 : 1))) void kv_attend_split_kernel(AttendArgs a) {
     constexpr bool kHalf = sizeof(C) == 2;
     constexpr int TS = kHalf ? 32 : 16;                   // slots of a tile
     constexpr int NT = TS / 16;
+    constexpr int STEP = 4 * TS;                          // slots of a step of the four wavefronts
     constexpr int KC = kHalf ? 8 : 4;                     // dims of a lane's 16 bytes of K
     constexpr int NJ = DP / (4 * KC);                     // steps over the dims
     constexpr int NQ = kHalf && sizeof(IO) == 4 ? 3 : 1;  // operands of a query
@@ -192,28 +200,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
     constexpr int NB = DP / (16 * CH);
     constexpr int NR = TS / 4;                            // slots of a lane
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // queries, then the wavefronts' outputs
-    __shared__ int64_t at[kSplit];  // element offset of each slot's row, -1 where it is not visible
+    __shared__ int32_t page_of[Paged ? kSplit / 16 : kSplit];  // of each 16 slots, or of each
+    __shared__ uint32_t vis[kSplit / 32];                      // visible slots
     __shared__ float sm[4][kQ], sl[4][kQ];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int64_t b = blockIdx.z;
     const int kvh = static_cast<int>(blockIdx.y) / a.q_tiles, qt = static_cast<int>(blockIdx.y) % a.q_tiles;
     const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
     const int h0 = kvh * G + qt * kQ, nq = min(kQ, G - qt * kQ);  // heads h0 .. h0 + nq - 1
     const int j0 = static_cast<int>(blockIdx.x) * kSplit;
-    // the slots' rows: page and mask are read without waiting for the length
-    const int slot = min(j0 + tid, a.max_len - 1);
-    int64_t off = -1;
-    bool seen = true;
-    if (slot >= 0) {
-        off = kv_slot(a.c, b, slot);
-        if (a.mask) seen = a.mask[b * a.mask_stride + slot] != 0;
+    // the slots' pages and mask are read without waiting for the length
+    int32_t page = -1;
+    bool seen = false;
+    if (j0 + tid < a.max_len) {
+        page = a.c.pages[b * a.c.max_pages + ((j0 + tid) >> a.c.page_shift)];
+        if (page >= a.c.n_pages) page = -1;
+        seen = page >= 0 && (!a.mask || a.mask[b * a.mask_stride + j0 + tid] != 0);
     }
     const int n = slots_of(a, b);
     if (j0 >= n && j0 > 0) return;  // whole workgroup; an empty sequence's first split writes its zeros
-    if (off >= 0) off += kvh * a.c.head_stride;
-    const bool live = j0 + tid < n;
-    at[tid] = live && seen ? off : -1;
+    {
+        const uint64_t bits = __ballot(seen && j0 + tid < n);
+        if (lane == 0) vis[2 * wave] = static_cast<uint32_t>(bits), vis[2 * wave + 1] = static_cast<uint32_t>(bits >> 32);
+        // a hole's rows are never used, but read: from page 0, which is there
+        if (!Paged || (tid & 15) == 0) page_of[Paged ? tid >> 4 : tid] = max(page, 0);
+    }
     const int fresh = a.k_new && n - 1 - j0 < kSplit ? n - 1 - j0 : -1;  // the new token's place in the split
     if (fresh >= 0 && qt == 0) {
         // its rows into the cache; this launch takes them from k_new and v_new
@@ -254,80 +266,106 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
         for (int e = 0; e < CH; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const float sl2 = a.scale * 1.4426950408889634f;
-    const C *kp = static_cast<const C *>(a.c.k), *vp = static_cast<const C *>(a.c.v);
+    const C *const kp = static_cast<const C *>(a.c.k) + kvh * a.c.head_stride;
+    const C *const vp = static_cast<const C *>(a.c.v) + kvh * a.c.head_stride;
     const int used = min(n - j0, kSplit);
-    for (int base = TS * wave; base < used; base += 4 * TS) {
-        int64_t ka[NT], va[NR];  // rows of K (slot 16 t + r) and V (slots 16 t + 4 g + i)
+    typedef uint32_t vch_t __attribute__((ext_vector_type(CH * sizeof(C) / 4)));
+    u32x4_t kf[NT][NJ];
+    vch_t vf[NR][NB];
+    // Element offset of a slot's row.  Page ids are held to 0 .. n_pages - 1
+    // and 16 slots from a multiple of 16 stay in their page, so that every row
+    // that is read is a row of the pool, visible or not; the scores and V's
+    // values of those that are not are replaced below.
+    auto row_of = [&](int pg, int slot) {
+        return static_cast<int64_t>(min(max(pg, 0), a.c.n_pages - 1)) * a.c.page_stride +
+               static_cast<int64_t>(slot & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
+    };
+    // a lane's places in 16 rows, in bytes (the host checks that they fit);
+    // chunks past d are read from the row's last chunk
+    constexpr int kSize = sizeof(C);
+    const uint32_t row_bytes = static_cast<uint32_t>(a.c.token_stride) * kSize;
+    auto load_k = [&](int base) {
+        uint32_t off[NJ];
+        const uint32_t first = static_cast<uint32_t>(in_loop(r)) * row_bytes;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) ka[t] = at[base + 16 * t + r];
-#pragma unroll
-        for (int i = 0; i < NR; ++i) va[i] = at[base + 16 * (i >> 2) + 4 * g + (i & 3)];
-        bool all = true, any = false;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) all &= va[i] >= 0, any |= va[i] >= 0;
-        all = __all(all);
-        f32x4_t sc[NT];
-        float *srow = a.score ? a.score + (b * a.n_head + h0 + r) * a.s_stride + j0 + base + 4 * g : nullptr;
-        if (!__any(any)) {
-            if (srow && r < nq)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    *reinterpret_cast<f32x4_t *>(srow + 16 * t) = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            continue;
-        }
-        // rows that are not visible: any row that is there; scores and V's
-        // values of them are replaced below
-        u32x4_t kf[NT][NJ];
-        typedef uint32_t vch_t __attribute__((ext_vector_type(CH * sizeof(C) / 4)));
-        vch_t vf[NR][NB];
+        for (int j = 0; j < NJ; ++j) off[j] = first + min(4 * KC * j + KC * g, d - KC) * kSize;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const C *row = kp + (ka[t] < 0 ? 0 : ka[t]);
+            const int s = base + 16 * t;
+            if constexpr (Paged) {
+                const char *row = reinterpret_cast<const char *>(kp + row_of(__builtin_amdgcn_readfirstlane(page_of[s >> 4]), j0 + s));
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-                kf[t][j] = *reinterpret_cast<const u32x4_t *>(row + (d == DP ? 4 * KC * j + KC * g : min(4 * KC * j + KC * g, d - KC)));
+                for (int j = 0; j < NJ; ++j) kf[t][j] = *reinterpret_cast<const u32x4_t *>(row + off[j]);
+            } else {
+                const C *row = kp + row_of(page_of[s + r], j0 + s + r);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) kf[t][j] = *reinterpret_cast<const u32x4_t *>(row + min(4 * KC * j + KC * g, d - KC));
+            }
         }
+    };
+    auto load_v = [&](int base) {
+        uint32_t off[NB];
+        const uint32_t first = 4 * static_cast<uint32_t>(in_loop(g)) * row_bytes;
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const C *row = vp + (va[i] < 0 ? 0 : va[i]);
+        for (int nb = 0; nb < NB; ++nb) off[nb] = first + min(16 * CH * nb + CH * r, d - CH) * kSize;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) vf[i][nb] = *reinterpret_cast<const vch_t *>(row + min(16 * CH * nb + CH * r, d - CH));
-        }
-        if (fresh >= base && fresh < base + TS) {
-            // the new token's row, as the cache stores it
+        for (int t = 0; t < NT; ++t) {
+            const int s = base + 16 * t;
+            if constexpr (Paged) {
+                const char *row = reinterpret_cast<const char *>(vp + row_of(__builtin_amdgcn_readfirstlane(page_of[s >> 4]), j0 + s));
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                if (base + 16 * t + r == fresh) {
-                    const IO *row = static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        float x[KC];
-                        load_row<KC>(row + min(4 * KC * j + KC * g, d - KC), x);
+                    for (int nb = 0; nb < NB; ++nb)
+                        vf[4 * t + i][nb] = *reinterpret_cast<const vch_t *>(row + static_cast<uint64_t>(i) * row_bytes + off[nb]);
+            } else {
 #pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            if constexpr (kHalf)
-                                kf[t][j][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
-                            else
-                                kf[t][j][w] = __float_as_uint(x[w]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int q = s + 4 * g + i;
+                    const C *row = vp + row_of(page_of[q], j0 + q);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) vf[4 * t + i][nb] = *reinterpret_cast<const vch_t *>(row + min(16 * CH * nb + CH * r, d - CH));
                 }
-#pragma unroll
-            for (int i = 0; i < NR; ++i)
-                if (base + 16 * (i >> 2) + 4 * g + (i & 3) == fresh) {
-                    const IO *row = static_cast<const IO *>(a.v_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        float x[CH];
-                        load_row<CH>(row + min(16 * CH * nb + CH * r, d - CH), x);
-#pragma unroll
-                        for (int w = 0; w < static_cast<int>(CH * sizeof(C) / 4); ++w)
-                            if constexpr (kHalf)
-                                vf[i][nb][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
-                            else
-                                vf[i][nb][w] = __float_as_uint(x[w]);
-                    }
-                }
+            }
         }
+    };
+    // the new token's row, as the cache stores it, over what was loaded of its slot
+    auto fresh_rows = [&](int base) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (base + 16 * t + r == fresh) {
+                const IO *row = static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float x[KC];
+                    load_row<KC>(row + min(4 * KC * j + KC * in_loop(g), d - KC), x);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        if constexpr (kHalf)
+                            kf[t][j][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
+                        else
+                            kf[t][j][w] = __float_as_uint(x[w]);
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (base + 16 * (i >> 2) + 4 * g + (i & 3) == fresh) {
+                const IO *row = static_cast<const IO *>(a.v_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float x[CH];
+                    load_row<CH>(row + min(16 * CH * nb + CH * in_loop(r), d - CH), x);
+#pragma unroll
+                    for (int w = 0; w < static_cast<int>(CH * sizeof(C) / 4); ++w)
+                        if constexpr (kHalf)
+                            vf[i][nb][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
+                        else
+                            vf[i][nb][w] = __float_as_uint(x[w]);
+                }
+            }
+    };
+    f32x4_t sc[NT];  // sc[t][e]: score of slot base + 16 t + 4 g + e against head r
+    auto scores = [&] {
         if (d != DP) {  // dims past d of a visible row count as 0, whatever stands there
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
@@ -335,10 +373,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
 #pragma unroll
                     for (int t = 0; t < NT; ++t) kf[t][j] = u32x4_t{0, 0, 0, 0};
         }
-        // the queries are read from LDS for every tile: held in registers they
-        // would take 48 of them (bf16 cache, fp32 queries, DP = 128)
-        asm volatile("" ::: "memory");
-        // S^T: sc[t][e] = score of slot base + 16 t + 4 g + e against head r
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -360,19 +394,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t] *= sl2;
-        if (!all) {
+    };
+    // the tile's scores into the running maximum and sum of head r (in base 2)
+    // and its rows of V into the output
+    auto output = [&](int base) {
+        uint32_t seen_now = __builtin_amdgcn_readfirstlane(vis[base >> 5]);
+        if (TS == 16) seen_now = (seen_now >> (base & 31)) & 0xffffu;
+        if (seen_now != (TS == 32 ? 0xffffffffu : 0xffffu)) {
 #pragma unroll
             for (int i = 0; i < NR; ++i)
-                if (va[i] < 0) {
+                if (!((seen_now >> (16 * (i >> 2) + 4 * g + (i & 3))) & 1)) {
                     sc[i >> 2][i & 3] = -INFINITY;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) vf[i][nb] = vch_t(0);
                 }
         }
-        if (srow && r < nq)
+        if (a.score && r < nq) {
+            float *srow = a.score + (b * a.n_head + h0 + in_loop(r)) * a.s_stride + j0 + base + 4 * g;
 #pragma unroll
             for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t *>(srow + 16 * t) = sc[t];
-        // running maximum and sum of head r in base 2
+        }
         float mx = sc[0][0];
 #pragma unroll
         for (int i = 1; i < NR; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
@@ -393,7 +434,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
 #pragma unroll
                 for (int e = 0; e < CH; ++e) o[nb][e] *= corr;
         }
-        // O^T += V^T P^T
         if constexpr (kHalf) {
             bf16x8_t pf[NP];
             split8<NP>(p, pf);
@@ -418,6 +458,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
                     for (int e = 0; e < 4; ++e)
                         o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][nb][e]), p[i], o[nb][e], 0, 0, 0);
         }
+    };
+    if (int base = TS * wave; base < used) {
+        load_k(base);
+        load_v(base);
+        for (;; base += STEP) {
+            if (fresh >= base && fresh < base + TS) fresh_rows(base);
+            scores();
+            if (base + STEP >= used) break;
+            load_k(base + STEP);
+            output(base);
+            load_v(base + STEP);
+        }
+        output(base);
     }
 
     // the four wavefronts' outputs joined, kJoin heads at a time
@@ -428,18 +481,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
     for (int q0 = 0; q0 < nq; q0 += kJoin) {
         __syncthreads();  // the queries, or the heads before, have been read
         if (r >= q0 && r < min(nq, q0 + kJoin)) {
-            float *row = ob + (wave * kJoin + r - q0) * OS;
+            float *row = ob + (wave * kJoin + r - q0) * OS + 4 * g;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < CH; e += 4)
-                        *reinterpret_cast<f32x4_t *>(row + 16 * CH * nb + CH * (4 * g + i) + e) =
-                            f32x4_t{o[nb][e][i], o[nb][e + 1][i], o[nb][e + 2][i], o[nb][e + 3][i]};
+                for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * (CH * nb + e)) = o[nb][e];
         }
         __syncthreads();
         const int dim = tid % DP;
+        const int place = dim / (16 * CH) * (16 * CH) + dim % CH * 16 + dim % (16 * CH) / CH;  // of dim in a row of ob
         for (int q = q0 + tid / DP; q < min(nq, q0 + kJoin); q += 256 / DP) {
             const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
             float L = 0.f, x = 0.f;
@@ -447,7 +497,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
             for (int w = 0; w < 4; ++w) {
                 const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
                 L += f * sl[w][q];
-                x += f * ob[(w * kJoin + q - q0) * OS + dim];
+                x += f * ob[(w * kJoin + q - q0) * OS + place];
             }
             if (dim >= d) continue;
             const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + blockIdx.x;
@@ -487,12 +537,8 @@ __device__ __forceinline__ float2 join_ml(const float2 *ml, int ns) {
 // The splits of (head, sequence) joined: a thread takes four dims of every
 // (1024 / DP)-th split.
 template <typename IO, int DP>
-__global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a) {
-    __shared__ f32x4_t red[256];
-    const int64_t b = blockIdx.y;
-    const int h = blockIdx.x, tid = threadIdx.x, d = a.c.d;
-    const int ns = (slots_of(a, b) + kSplit - 1) / kSplit;
-    if (ns <= 1) return;  // written by its only split
+__device__ __forceinline__ void join_splits(const AttendArgs &a, int64_t b, int h, int ns, f32x4_t *red) {
+    const int tid = threadIdx.x, d = a.c.d;
     constexpr int DL = DP / 4, NG = 256 / DL;
     const int64_t rec = (b * a.n_head + h) * a.n_split;
     const float2 t = join_ml(a.ml + rec, ns);
@@ -518,12 +564,8 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a) {
 // head, onto the history: by the scores that the splits left and the heads'
 // joined maxima and sums.  kWSlots slots a workgroup.
 constexpr int kWSlots = 512, kWHeads = 64;
-__global__ __launch_bounds__(256) void kv_weight_kernel(AttendArgs a) {
-    __shared__ float2 ml[kWHeads];
-    const int64_t b = blockIdx.z;
-    const int hs = blockIdx.y, j0 = static_cast<int>(blockIdx.x) * kWSlots, tid = threadIdx.x;
-    const int n = slots_of(a, b);
-    if (j0 >= n) return;
+__device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int hs, int j0, int n, float2 *ml) {
+    const int tid = threadIdx.x;
     const int ns = (n + kSplit - 1) / kSplit, G = a.n_head / a.h_heads;
     float w[kWSlots / 256];
 #pragma unroll
@@ -552,6 +594,22 @@ __global__ __launch_bounds__(256) void kv_weight_kernel(AttendArgs a) {
     }
 }
 
+// What the splits left brought together: workgroups 0 .. joins - 1 of a
+// sequence take a head's output each, the others kWSlots slots of a history
+// head.
+template <typename IO, int DP>
+__global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, int joins) {
+    __shared__ f32x4_t red[256];
+    const int64_t b = blockIdx.y;
+    const int x = static_cast<int>(blockIdx.x), n = slots_of(a, b);
+    if (x < joins) {
+        if (n > kSplit) join_splits<IO, DP>(a, b, x, (n + kSplit - 1) / kSplit, red);  // else its only split wrote it
+    } else {
+        const int hs = (x - joins) % a.h_heads, j0 = (x - joins) / a.h_heads * kWSlots;
+        if (j0 < n) add_weights(a, b, hs, j0, n, reinterpret_cast<float2 *>(red));
+    }
+}
+
 template <typename C, typename IO, int DP>
 int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
     constexpr bool kHalf = sizeof(C) == 2;
@@ -559,16 +617,18 @@ int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
     constexpr size_t o_bytes = 4 * kJoin * (DP + 4) * sizeof(float);
     constexpr size_t lds = q_bytes > o_bytes ? q_bytes : o_bytes;
     static_assert(lds + kSplit * 8 + 2 * 4 * kQ * 4 <= 65536, "LDS without an opt-in");
-    hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP>), dim3(a.n_split, a.c.n_head_kv * a.q_tiles, seqs), dim3(256), lds, s, a);
+    const dim3 grid(a.n_split, a.c.n_head_kv * a.q_tiles, seqs);
+    if (a.c.page_shift >= 4)
+        hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP, true>), grid, dim3(256), lds, s, a);
+    else
+        hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP, false>), grid, dim3(256), lds, s, a);
     int st = check_launch("kv_attend_split_kernel");
     if (st) return st;
-    if (a.n_split > 1) {
-        hipLaunchKernelGGL((kv_attend_join_kernel<IO, DP>), dim3(a.n_head, seqs), dim3(256), 0, s, a);
-        if ((st = check_launch("kv_attend_join_kernel"))) return st;
-    }
-    if (a.weight) {
-        hipLaunchKernelGGL(kv_weight_kernel, dim3((a.max_len + kWSlots - 1) / kWSlots, a.h_heads, seqs), dim3(256), 0, s, a);
-        st = check_launch("kv_weight_kernel");
+    const int joins = a.n_split > 1 ? a.n_head : 0;
+    const int64_t weights = a.weight ? static_cast<int64_t>((a.max_len + kWSlots - 1) / kWSlots) * a.h_heads : 0;
+    if (joins + weights > 0) {
+        hipLaunchKernelGGL((kv_attend_join_kernel<IO, DP>), dim3(static_cast<unsigned>(joins + weights), seqs), dim3(256), 0, s, a, joins);
+        st = check_launch("kv_attend_join_kernel");
     }
     return st;
 }
