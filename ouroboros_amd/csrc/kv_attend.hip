@@ -9,6 +9,7 @@
 #include "kv_cache.hpp"
 
 #include <cmath>
+#include <cstdlib>
 
 namespace ouro {
 
@@ -49,6 +50,7 @@ namespace {
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef short bf16x4_t __attribute__((ext_vector_type(4)));  // the builtin's type of four bf16
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -70,8 +72,8 @@ struct AttendArgs {
     float *score;  // [seqs][n_head][s_stride]: scores times log2 e, where there is a history
     int64_t q_stride, new_stride, mask_stride, out_stride, s_stride;
     int32_t n_head, max_len, h_heads, h_slots, n_split, q_tiles;
+    int32_t run;  // splits of a workgroup, one after another
     float scale;
-    int32_t pad;
 };
 // passed by value to kernels: the host and device passes must lay it out alike
 static_assert(sizeof(AttendArgs) == 256, "AttendArgs: kernel argument layout");
@@ -116,24 +118,35 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // x as a sum of N bf16 operands, each the rounding of what the ones before
 // leave (the differences are exact): 8 bits of the significand apiece, so three
 // hold a float whole and two hold it to 2^-17.
-template <int N>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8_t (&s)[N]) {
-    float r[8];
+template <int N, int M>
+__device__ __forceinline__ void split(const float (&x)[M], uint32_t (&w)[N][M / 2]) {
+    float r[M];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = x[i];
+    for (int i = 0; i < M; ++i) r[i] = x[i];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        u32x4_t w;
+    for (int k = 0; k < N; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+        for (int i = 0; i < M / 2; ++i) {
+            w[k][i] = pack_bf16(r[2 * i], r[2 * i + 1]);
             if (k + 1 < N) {
-                r[2 * i] -= __uint_as_float(w[i] << 16);
-                r[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+                r[2 * i] -= __uint_as_float(w[k][i] << 16);
+                r[2 * i + 1] -= __uint_as_float(w[k][i] & 0xffff0000u);
             }
         }
-        s[k] = __builtin_bit_cast(bf16x8_t, w);
-    }
+}
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8_t (&s)[N]) {
+    uint32_t w[N][4];
+    split<N>(x, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = __builtin_bit_cast(bf16x8_t, u32x4_t{w[k][0], w[k][1], w[k][2], w[k][3]});
+}
+template <int N>
+__device__ __forceinline__ void split4(const float (&x)[4], bf16x4_t (&s)[N]) {
+    uint32_t w[N][2];
+    split<N>(x, w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = __builtin_bit_cast(bf16x4_t, u32x2_t{w[k][0], w[k][1]});
 }
 // Maximum and sum over the four lanes l, l + 16, l + 32, l + 48.
 __device__ __forceinline__ float quad_max(float v) {
@@ -187,10 +200,9 @@ __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h,
 // operands (exact), weights for a bf16 output into two (2^-17); everything
 // else is fp32.
 template <typename C, typename IO, int DP, bool Paged>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 4 : DP <= 128 ? 2 : 1))) void kv_attend_split_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) == 2 ? (DP <= 64 ? 5 : DP <= 128 ? 4 : 2) : (DP <= 64 ? 5 : DP <= 128 ? 3 : 2)))) void kv_attend_split_kernel(AttendArgs a) {
     constexpr bool kHalf = sizeof(C) == 2;
-    constexpr int TS = kHalf ? 32 : 16;                   // slots of a tile
-    constexpr int NT = TS / 16;
+    constexpr int TS = 16;                                // slots of a tile
     constexpr int STEP = 4 * TS;                          // slots of a step of the four wavefronts
     constexpr int KC = kHalf ? 8 : 4;                     // dims of a lane's 16 bytes of K
     constexpr int NJ = DP / (4 * KC);                     // steps over the dims
@@ -199,9 +211,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
     constexpr int CH = kHalf && DP > 64 ? 8 : 4;          // adjacent dims of V a lane
     constexpr int NB = DP / (16 * CH);
     constexpr int NR = TS / 4;                            // slots of a lane
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // queries, then the wavefronts' outputs
-    __shared__ int32_t page_of[Paged ? kSplit / 16 : kSplit];  // of each 16 slots, or of each
-    __shared__ uint32_t vis[kSplit / 32];                      // visible slots
+    constexpr size_t kQBytes = kHalf ? NQ * DP * 32 : DP * 64;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // queries | the wavefronts' outputs
     __shared__ float sm[4][kQ], sl[4][kQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -209,24 +220,70 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
     const int kvh = static_cast<int>(blockIdx.y) / a.q_tiles, qt = static_cast<int>(blockIdx.y) % a.q_tiles;
     const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
     const int h0 = kvh * G + qt * kQ, nq = min(kQ, G - qt * kQ);  // heads h0 .. h0 + nq - 1
-    const int j0 = static_cast<int>(blockIdx.x) * kSplit;
-    // the slots' pages and mask are read without waiting for the length
-    int32_t page = -1;
+    const int j0 = static_cast<int>(blockIdx.x) * a.run * kSplit;
+    // Lane l of wavefront w stands for slot 16 (w + 4 (l / 16)) + l % 16 of a
+    // split: the wavefront's own tiles, so that their pages and visible slots
+    // stay in its registers.  They are read without waiting for the length.
+    const int mine = 16 * (wave + 4 * g) + r;
+    int32_t page = 0;  // held to 0 .. n_pages - 1: a hole's rows are read (of a page that is there), never used
     bool seen = false;
-    if (j0 + tid < a.max_len) {
-        page = a.c.pages[b * a.c.max_pages + ((j0 + tid) >> a.c.page_shift)];
-        if (page >= a.c.n_pages) page = -1;
-        seen = page >= 0 && (!a.mask || a.mask[b * a.mask_stride + j0 + tid] != 0);
-    }
+    auto look = [&](int slot) {
+        page = 0, seen = false;
+        if (slot < a.max_len) {
+            const int32_t id = a.c.pages[b * a.c.max_pages + (slot >> a.c.page_shift)];
+            const bool there = id >= 0 && id < a.c.n_pages;
+            if (there) page = id;
+            seen = there && (!a.mask || a.mask[b * a.mask_stride + slot] != 0);
+        }
+    };
+    look(j0 + mine);
     const int n = slots_of(a, b);
-    if (j0 >= n && j0 > 0) return;  // whole workgroup; an empty sequence's first split writes its zeros
-    {
-        const uint64_t bits = __ballot(seen && j0 + tid < n);
-        if (lane == 0) vis[2 * wave] = static_cast<uint32_t>(bits), vis[2 * wave + 1] = static_cast<uint32_t>(bits >> 32);
-        // a hole's rows are never used, but read: from page 0, which is there
-        if (!Paged || (tid & 15) == 0) page_of[Paged ? tid >> 4 : tid] = max(page, 0);
-    }
-    const int fresh = a.k_new && n - 1 - j0 < kSplit ? n - 1 - j0 : -1;  // the new token's place in the split
+    if (j0 >= n && j0 > 0) return;  // whole workgroup; an empty sequence's first run writes its zeros
+    const int end = min(n, j0 + a.run * kSplit);  // the run's slots are j0 .. end - 1
+    typedef uint32_t vch_t __attribute__((ext_vector_type(CH * sizeof(C) / 4)));
+    u32x4_t kf[NJ];
+    vch_t vf[NR][NB];
+    const C *const kp = static_cast<const C *>(a.c.k) + kvh * a.c.head_stride;
+    const C *const vp = static_cast<const C *>(a.c.v) + kvh * a.c.head_stride;
+    // Element offset of a slot's row.  16 slots from a multiple of 16 stay in
+    // their page, so that every row that is read is a row of the pool, visible
+    // or not; scores and V's values of those that are not are replaced below.
+    auto row_of = [&](int pg, int slot) {
+        return static_cast<int64_t>(pg) * a.c.page_stride +
+               static_cast<int64_t>(slot & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
+    };
+    // a lane's places in 16 rows, in bytes (the host checks that they fit);
+    // chunks past d are read from the row's last chunk
+    constexpr int kSize = sizeof(C);
+    const uint32_t row_bytes = static_cast<uint32_t>(a.c.token_stride) * kSize;
+    // the tile of 16 slots from `slot`, the wavefront's k-th of its split
+    auto load_tile = [&](int slot, int k) {
+        if constexpr (Paged) {
+            const int64_t row = row_of(__builtin_amdgcn_readlane(page, 16 * k), slot);
+            const char *kr = reinterpret_cast<const char *>(kp + row), *vr = reinterpret_cast<const char *>(vp + row);
+            const uint32_t k0 = static_cast<uint32_t>(in_loop(r)) * row_bytes, v0 = 4 * static_cast<uint32_t>(in_loop(g)) * row_bytes;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const u32x4_t *>(kr + (k0 + min(4 * KC * j + KC * g, d - KC) * kSize));
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    vf[i][nb] = *reinterpret_cast<const vch_t *>(vr + static_cast<uint64_t>(i) * row_bytes + (v0 + min(16 * CH * nb + CH * r, d - CH) * kSize));
+        } else {
+            const C *kr = kp + row_of(__shfl(page, 16 * k + r, 64), slot + r);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const u32x4_t *>(kr + min(4 * KC * j + KC * g, d - KC));
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const C *vr = vp + row_of(__shfl(page, 16 * k + 4 * g + i, 64), slot + 4 * g + i);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) vf[i][nb] = *reinterpret_cast<const vch_t *>(vr + min(16 * CH * nb + CH * r, d - CH));
+            }
+        }
+    };
+    uint64_t bits = __ballot(seen && j0 + mine < n);  // visible slots: 16 of each of the wavefront's tiles of the split
+    if (j0 + TS * wave < end) load_tile(j0 + TS * wave, 0);
+    const int fresh = a.k_new && n <= end ? n - 1 : -1;  // the new token's slot, if it is in the run
     if (fresh >= 0 && qt == 0) {
         // its rows into the cache; this launch takes them from k_new and v_new
         const int64_t to = kv_slot(a.c, b, n - 1);
@@ -266,90 +323,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
         for (int e = 0; e < CH; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const float sl2 = a.scale * 1.4426950408889634f;
-    const C *const kp = static_cast<const C *>(a.c.k) + kvh * a.c.head_stride;
-    const C *const vp = static_cast<const C *>(a.c.v) + kvh * a.c.head_stride;
-    const int used = min(n - j0, kSplit);
-    typedef uint32_t vch_t __attribute__((ext_vector_type(CH * sizeof(C) / 4)));
-    u32x4_t kf[NT][NJ];
-    vch_t vf[NR][NB];
-    // Element offset of a slot's row.  Page ids are held to 0 .. n_pages - 1
-    // and 16 slots from a multiple of 16 stay in their page, so that every row
-    // that is read is a row of the pool, visible or not; the scores and V's
-    // values of those that are not are replaced below.
-    auto row_of = [&](int pg, int slot) {
-        return static_cast<int64_t>(min(max(pg, 0), a.c.n_pages - 1)) * a.c.page_stride +
-               static_cast<int64_t>(slot & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
-    };
-    // a lane's places in 16 rows, in bytes (the host checks that they fit);
-    // chunks past d are read from the row's last chunk
-    constexpr int kSize = sizeof(C);
-    const uint32_t row_bytes = static_cast<uint32_t>(a.c.token_stride) * kSize;
-    auto load_k = [&](int base) {
-        uint32_t off[NJ];
-        const uint32_t first = static_cast<uint32_t>(in_loop(r)) * row_bytes;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) off[j] = first + min(4 * KC * j + KC * g, d - KC) * kSize;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int s = base + 16 * t;
-            if constexpr (Paged) {
-                const char *row = reinterpret_cast<const char *>(kp + row_of(__builtin_amdgcn_readfirstlane(page_of[s >> 4]), j0 + s));
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) kf[t][j] = *reinterpret_cast<const u32x4_t *>(row + off[j]);
-            } else {
-                const C *row = kp + row_of(page_of[s + r], j0 + s + r);
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) kf[t][j] = *reinterpret_cast<const u32x4_t *>(row + min(4 * KC * j + KC * g, d - KC));
-            }
-        }
-    };
-    auto load_v = [&](int base) {
-        uint32_t off[NB];
-        const uint32_t first = 4 * static_cast<uint32_t>(in_loop(g)) * row_bytes;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) off[nb] = first + min(16 * CH * nb + CH * r, d - CH) * kSize;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int s = base + 16 * t;
-            if constexpr (Paged) {
-                const char *row = reinterpret_cast<const char *>(vp + row_of(__builtin_amdgcn_readfirstlane(page_of[s >> 4]), j0 + s));
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-                        vf[4 * t + i][nb] = *reinterpret_cast<const vch_t *>(row + static_cast<uint64_t>(i) * row_bytes + off[nb]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int q = s + 4 * g + i;
-                    const C *row = vp + row_of(page_of[q], j0 + q);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) vf[4 * t + i][nb] = *reinterpret_cast<const vch_t *>(row + min(16 * CH * nb + CH * r, d - CH));
-                }
-            }
-        }
-    };
     // the new token's row, as the cache stores it, over what was loaded of its slot
-    auto fresh_rows = [&](int base) {
+    auto fresh_rows = [&](int slot) {
+        if (slot + r == fresh) {
+            const IO *row = static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (base + 16 * t + r == fresh) {
-                const IO *row = static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
+            for (int j = 0; j < NJ; ++j) {
+                float x[KC];
+                load_row<KC>(row + min(4 * KC * j + KC * in_loop(g), d - KC), x);
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    float x[KC];
-                    load_row<KC>(row + min(4 * KC * j + KC * in_loop(g), d - KC), x);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        if constexpr (kHalf)
-                            kf[t][j][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
-                        else
-                            kf[t][j][w] = __float_as_uint(x[w]);
-                }
+                for (int w = 0; w < 4; ++w)
+                    if constexpr (kHalf)
+                        kf[j][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
+                    else
+                        kf[j][w] = __float_as_uint(x[w]);
             }
+        }
 #pragma unroll
         for (int i = 0; i < NR; ++i)
-            if (base + 16 * (i >> 2) + 4 * g + (i & 3) == fresh) {
+            if (slot + 4 * g + i == fresh) {
                 const IO *row = static_cast<const IO *>(a.v_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
@@ -364,67 +356,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
                 }
             }
     };
-    f32x4_t sc[NT];  // sc[t][e]: score of slot base + 16 t + 4 g + e against head r
-    auto scores = [&] {
+    // The tile of 16 slots from `slot`, of which `now` are visible, into the
+    // running maximum, sum and output of head r; maximum and scores in base 2.
+    auto products = [&](int slot, uint32_t now) {
         if (d != DP) {  // dims past d of a visible row count as 0, whatever stands there
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
-                if (4 * KC * j + KC * g >= d)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) kf[t][j] = u32x4_t{0, 0, 0, 0};
+                if (4 * KC * j + KC * g >= d) kf[j] = u32x4_t{0, 0, 0, 0};
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        f32x4_t sc = {0.f, 0.f, 0.f, 0.f};  // sc[e]: score of slot 4 g + e against head r
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             if constexpr (kHalf) {
 #pragma unroll
-                for (int k = 0; k < NQ; ++k) {
-                    const bf16x8_t q = reinterpret_cast<const bf16x8_t *>(lds)[(k * NJ + j) * 64 + lane];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[t][j]), q, sc[t], 0, 0, 0);
-                }
+                for (int k = 0; k < NQ; ++k)
+                    sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[j]),
+                                                                 reinterpret_cast<const bf16x8_t *>(lds)[(k * NJ + j) * 64 + lane], sc, 0, 0, 0);
             } else {
                 const f32x4_t q = reinterpret_cast<const f32x4_t *>(lds)[j * 64 + lane];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[0][j][e]), q[e], sc[0], 0, 0, 0);
+                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[j][e]), q[e], sc, 0, 0, 0);
             }
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) sc[t] *= sl2;
-    };
-    // the tile's scores into the running maximum and sum of head r (in base 2)
-    // and its rows of V into the output
-    auto output = [&](int base) {
-        uint32_t seen_now = __builtin_amdgcn_readfirstlane(vis[base >> 5]);
-        if (TS == 16) seen_now = (seen_now >> (base & 31)) & 0xffffu;
-        if (seen_now != (TS == 32 ? 0xffffffffu : 0xffffu)) {
+        sc *= sl2;
+        if (now != 0xffffu) {
 #pragma unroll
             for (int i = 0; i < NR; ++i)
-                if (!((seen_now >> (16 * (i >> 2) + 4 * g + (i & 3))) & 1)) {
-                    sc[i >> 2][i & 3] = -INFINITY;
+                if (!((now >> (4 * g + i)) & 1)) {
+                    sc[i] = -INFINITY;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) vf[i][nb] = vch_t(0);
                 }
         }
-        if (a.score && r < nq) {
-            float *srow = a.score + (b * a.n_head + h0 + in_loop(r)) * a.s_stride + j0 + base + 4 * g;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t *>(srow + 16 * t) = sc[t];
-        }
-        float mx = sc[0][0];
-#pragma unroll
-        for (int i = 1; i < NR; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
-        const float mn = fmaxf(m, quad_max(mx));
+        if (a.score && r < nq)
+            *reinterpret_cast<f32x4_t *>(a.score + (b * a.n_head + h0 + in_loop(r)) * a.s_stride + slot + 4 * g) = sc;
+        const float mn = fmaxf(m, quad_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]))));
         const float mref = mn == -INFINITY ? 0.f : mn;  // no finite score yet: avoid inf - inf
         const float corr = __builtin_amdgcn_exp2f(m - mref);
         m = mn;
         float ps = 0.f, p[NR];
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(sc[i >> 2][i & 3] - mref);
+            p[i] = __builtin_amdgcn_exp2f(sc[i] - mref);
             ps += p[i];
         }
         l = l * corr + quad_sum(ps);
@@ -435,19 +408,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
                 for (int e = 0; e < CH; ++e) o[nb][e] *= corr;
         }
         if constexpr (kHalf) {
-            bf16x8_t pf[NP];
-            split8<NP>(p, pf);
+            bf16x4_t pf[NP];
+            split4<NP>(p, pf);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int e = 0; e < CH; ++e) {
-                    u32x4_t w;
+                    u32x2_t w;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 2; ++i)
                         w[i] = __builtin_amdgcn_perm(vf[2 * i + 1][nb][e >> 1], vf[2 * i][nb][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                     for (int k = 0; k < NP; ++k)
-                        o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), pf[k], o[nb][e], 0, 0, 0);
+                        o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_t, w), pf[k], o[nb][e], 0, 0, 0);
                 }
         } else {
 #pragma unroll
@@ -459,56 +432,67 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 
                         o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][nb][e]), p[i], o[nb][e], 0, 0, 0);
         }
     };
-    if (int base = TS * wave; base < used) {
-        load_k(base);
-        load_v(base);
-        for (;; base += STEP) {
-            if (fresh >= base && fresh < base + TS) fresh_rows(base);
-            scores();
-            if (base + STEP >= used) break;
-            load_k(base + STEP);
-            output(base);
-            load_v(base + STEP);
-        }
-        output(base);
-    }
-
-    // the four wavefronts' outputs joined, kJoin heads at a time
-    if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
-    constexpr int OS = DP + 4;  // floats of a row: padded, so that the heads' rows start in different banks
-    float *ob = reinterpret_cast<float *>(lds);
+    constexpr int OS = DP + 4;  // floats of an output row: padded, so that the heads' rows start in different banks
+    float *const ob = reinterpret_cast<float *>(lds + kQBytes);
     const bool whole = n <= kSplit;  // the sequence's only split
-    for (int q0 = 0; q0 < nq; q0 += kJoin) {
-        __syncthreads();  // the queries, or the heads before, have been read
-        if (r >= q0 && r < min(nq, q0 + kJoin)) {
-            float *row = ob + (wave * kJoin + r - q0) * OS + 4 * g;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * (CH * nb + e)) = o[nb][e];
-        }
-        __syncthreads();
-        const int dim = tid % DP;
-        const int place = dim / (16 * CH) * (16 * CH) + dim % CH * 16 + dim % (16 * CH) / CH;  // of dim in a row of ob
-        for (int q = q0 + tid / DP; q < min(nq, q0 + kJoin); q += 256 / DP) {
-            const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
-            float L = 0.f, x = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
-                L += f * sl[w][q];
-                x += f * ob[(w * kJoin + q - q0) * OS + place];
+    for (int s0 = j0;;) {  // the run's splits
+        for (int k = 0; k < 4; ++k) {
+            const int slot = s0 + TS * wave + STEP * k;
+            if (slot < end) {
+                if (fresh >= slot && fresh < slot + TS) fresh_rows(slot);
+                products(slot, static_cast<uint32_t>(bits >> (16 * k)) & 0xffffu);
             }
-            if (dim >= d) continue;
-            const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + blockIdx.x;
-            if (dim == 0 && a.ml) a.ml[rec] = make_float2(M, L);
-            if (whole) {
-                store_out<IO>(a, b, h0 + q, dim, M == -INFINITY ? 0.f : x / L);
-                if (dim == 0) store_lse(a, b, h0 + q, M, L);
-            } else {
-                a.part[rec * d + dim] = x;
+            if (k < 3 && slot + STEP < end) load_tile(slot + STEP, k + 1);
+        }
+        const int split = s0 / kSplit;
+        s0 += kSplit;
+        const bool more = s0 < end;
+        if (more) {  // the next split's first tile is on its way while this one's outputs are joined
+            look(s0 + mine);
+            bits = __ballot(seen && s0 + mine < n);
+            if (s0 + TS * wave < end) load_tile(s0 + TS * wave, 0);
+        }
+        // the four wavefronts' outputs joined, kJoin heads at a time
+        if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
+        for (int q0 = 0; q0 < nq; q0 += kJoin) {
+            if (q0) __syncthreads();  // the heads before have been read
+            if (r >= q0 && r < min(nq, q0 + kJoin)) {
+                float *row = ob + (wave * kJoin + in_loop(r) - q0) * OS + 4 * g;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * (CH * nb + e)) = o[nb][e];
+            }
+            __syncthreads();
+            const int dim = in_loop(tid) % DP;
+            const int place = dim / (16 * CH) * (16 * CH) + dim % CH * 16 + dim % (16 * CH) / CH;  // of dim in a row of ob
+            for (int q = q0 + tid / DP; q < min(nq, q0 + kJoin); q += 256 / DP) {
+                const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
+                float L = 0.f, x = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
+                    L += f * sl[w][q];
+                    x += f * ob[(w * kJoin + q - q0) * OS + place];
+                }
+                if (dim >= d) continue;
+                const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + split;
+                if (dim == 0 && a.ml) a.ml[rec] = make_float2(M, L);
+                if (whole) {
+                    store_out<IO>(a, b, h0 + q, dim, M == -INFINITY ? 0.f : x / L);
+                    if (dim == 0) store_lse(a, b, h0 + q, M, L);
+                } else {
+                    a.part[rec * d + dim] = x;
+                }
             }
         }
+        if (!more) break;
+        __syncthreads();  // the outputs have been read
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < CH; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 }
 
@@ -614,10 +598,9 @@ template <typename C, typename IO, int DP>
 int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
     constexpr bool kHalf = sizeof(C) == 2;
     constexpr size_t q_bytes = kHalf ? (sizeof(IO) == 4 ? 3 : 1) * DP * 32 : DP * 64;
-    constexpr size_t o_bytes = 4 * kJoin * (DP + 4) * sizeof(float);
-    constexpr size_t lds = q_bytes > o_bytes ? q_bytes : o_bytes;
-    static_assert(lds + kSplit * 8 + 2 * 4 * kQ * 4 <= 65536, "LDS without an opt-in");
-    const dim3 grid(a.n_split, a.c.n_head_kv * a.q_tiles, seqs);
+    constexpr size_t lds = q_bytes + 4 * kJoin * (DP + 4) * sizeof(float);
+    static_assert(lds + 2 * 4 * kQ * 4 <= 65536, "LDS without an opt-in");
+    const dim3 grid((a.n_split + a.run - 1) / a.run, a.c.n_head_kv * a.q_tiles, seqs);
     if (a.c.page_shift >= 4)
         hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP, true>), grid, dim3(256), lds, s, a);
     else
@@ -719,6 +702,7 @@ int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history, c
     a.s_stride = w.s_stride;
     a.n_split = w.n_split;
     a.q_tiles = static_cast<int>((n_head / hkv + kQ - 1) / kQ);
+    a.run = getenv("ORUN") ? atoi(getenv("ORUN")) : 1;
     a.q = q, a.k_new = k_new, a.v_new = v_new, a.gate = gate, a.pos_new = pos_new, a.lens = lens, a.mask = mask, a.out = out, a.lse = lse;
     a.q_stride = q_stride, a.new_stride = new_stride, a.mask_stride = mask_stride, a.out_stride = out_stride;
     a.n_head = static_cast<int>(n_head), a.max_len = static_cast<int>(max_len), a.scale = scale;
