@@ -8,8 +8,8 @@
 // and o = 0, lse = -inf where no slot is visible.
 #include "kv_cache.hpp"
 
+#include <atomic>
 #include <cmath>
-#include <cstdlib>
 
 namespace ouro {
 
@@ -57,6 +57,11 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kSplit = 256;  // slots of a workgroup
 constexpr int kQ = 16;       // query heads of a workgroup: the columns of its products
+// Caches of more bytes are read with non-temporal loads: half of the last-level
+// cache, which holds a smaller one from one call to the next where nothing else
+// comes between.  (64 sequences of up to 1025 keys, 134 MB: 37.4 -> 34.2 us; 24
+// of up to 8191 of half the width, 100 MB, called again and again: 24.9 -> 30.3)
+constexpr int64_t kKeptBytes = 128 << 20;
 constexpr int kJoin = 8;     // query heads that the wavefronts' outputs are joined for at a time
 
 struct AttendArgs {
@@ -72,8 +77,8 @@ struct AttendArgs {
     float *score;  // [seqs][n_head][s_stride]: scores times log2 e, where there is a history
     int64_t q_stride, new_stride, mask_stride, out_stride, s_stride;
     int32_t n_head, max_len, h_heads, h_slots, n_split, q_tiles;
-    int32_t run;  // splits of a workgroup, one after another
     float scale;
+    int32_t pad;
 };
 // passed by value to kernels: the host and device passes must lay it out alike
 static_assert(sizeof(AttendArgs) == 256, "AttendArgs: kernel argument layout");
@@ -165,6 +170,14 @@ __device__ __forceinline__ float quad_sum(float v) {
 __device__ __forceinline__ int slots_of(const AttendArgs &a, int64_t b) { return max(0, min(a.lens[b], a.max_len)); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
+// A load of the cache: Once = non-temporal, for caches that no cache of the
+// chip holds until the next call.
+template <bool Once, typename T>
+__device__ __forceinline__ T load_cache(const T *p) {
+    if constexpr (Once) return __builtin_nontemporal_load(p);
+    return *p;
+}
+
 // x, as a value that is made where this stands: what is computed from it stays
 // in the loop instead of being kept in registers throughout it.
 __device__ __forceinline__ int in_loop(int x) {
@@ -199,7 +212,7 @@ __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h,
 // fp32 queries and weights against a bf16 cache are split into three bf16
 // operands (exact), weights for a bf16 output into two (2^-17); everything
 // else is fp32.
-template <typename C, typename IO, int DP, bool Paged>
+template <typename C, typename IO, int DP, bool Paged, bool Once>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) == 2 ? (DP <= 64 ? 5 : DP <= 128 ? 4 : 2) : (DP <= 64 ? 5 : DP <= 128 ? 3 : 2)))) void kv_attend_split_kernel(AttendArgs a) {
     constexpr bool kHalf = sizeof(C) == 2;
     constexpr int TS = 16;                                // slots of a tile
@@ -212,7 +225,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
     constexpr int NB = DP / (16 * CH);
     constexpr int NR = TS / 4;                            // slots of a lane
     constexpr size_t kQBytes = kHalf ? NQ * DP * 32 : DP * 64;
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // queries | the wavefronts' outputs
+    constexpr int CPR = DP / KC;                          // chunks of 16 bytes of a row
+    constexpr int RK = 64 / CPR;                          // rows of a load of K
+    constexpr size_t kKRow = 16 * CPR + 16;               // bytes of a row of K in LDS: 16 rows start in different banks
+    constexpr size_t kKBytes = 16 * kKRow;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // queries | the wavefronts' rows of K, later their outputs
     __shared__ float sm[4][kQ], sl[4][kQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -220,28 +237,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
     const int kvh = static_cast<int>(blockIdx.y) / a.q_tiles, qt = static_cast<int>(blockIdx.y) % a.q_tiles;
     const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
     const int h0 = kvh * G + qt * kQ, nq = min(kQ, G - qt * kQ);  // heads h0 .. h0 + nq - 1
-    const int j0 = static_cast<int>(blockIdx.x) * a.run * kSplit;
+    const int j0 = static_cast<int>(blockIdx.x) * kSplit;
     // Lane l of wavefront w stands for slot 16 (w + 4 (l / 16)) + l % 16 of a
     // split: the wavefront's own tiles, so that their pages and visible slots
     // stay in its registers.  They are read without waiting for the length.
     const int mine = 16 * (wave + 4 * g) + r;
     int32_t page = 0;  // held to 0 .. n_pages - 1: a hole's rows are read (of a page that is there), never used
     bool seen = false;
-    auto look = [&](int slot) {
-        page = 0, seen = false;
-        if (slot < a.max_len) {
-            const int32_t id = a.c.pages[b * a.c.max_pages + (slot >> a.c.page_shift)];
-            const bool there = id >= 0 && id < a.c.n_pages;
-            if (there) page = id;
-            seen = there && (!a.mask || a.mask[b * a.mask_stride + slot] != 0);
-        }
-    };
-    look(j0 + mine);
+    if (j0 + mine < a.max_len) {
+        const int32_t id = a.c.pages[b * a.c.max_pages + ((j0 + mine) >> a.c.page_shift)];
+        const bool there = id >= 0 && id < a.c.n_pages;
+        if (there) page = id;
+        seen = there && (!a.mask || a.mask[b * a.mask_stride + j0 + mine] != 0);
+    }
     const int n = slots_of(a, b);
-    if (j0 >= n && j0 > 0) return;  // whole workgroup; an empty sequence's first run writes its zeros
-    const int end = min(n, j0 + a.run * kSplit);  // the run's slots are j0 .. end - 1
+    if (j0 >= n && j0 > 0) return;  // whole workgroup; an empty sequence's first split writes its zeros
+    const int end = min(n, j0 + kSplit);  // the split's slots are j0 .. end - 1
     typedef uint32_t vch_t __attribute__((ext_vector_type(CH * sizeof(C) / 4)));
-    u32x4_t kf[NJ];
+    u32x4_t kf[NJ];  // K: chunk kc of rows RK i + kr
     vch_t vf[NR][NB];
     const C *const kp = static_cast<const C *>(a.c.k) + kvh * a.c.head_stride;
     const C *const vp = static_cast<const C *>(a.c.v) + kvh * a.c.head_stride;
@@ -256,34 +269,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
     // chunks past d are read from the row's last chunk
     constexpr int kSize = sizeof(C);
     const uint32_t row_bytes = static_cast<uint32_t>(a.c.token_stride) * kSize;
-    // the tile of 16 slots from `slot`, the wavefront's k-th of its split
-    auto load_tile = [&](int slot, int k) {
+    const int kr = lane / CPR, kc = lane % CPR;
+    // Rows of the tile of 16 slots from `slot`, the wavefront's k-th of its
+    // split; where there is none, one line over and over, so that the loads in
+    // flight can be counted without knowing.
+    auto load_k = [&](int slot, int k, bool there) {
         if constexpr (Paged) {
-            const int64_t row = row_of(__builtin_amdgcn_readlane(page, 16 * k), slot);
-            const char *kr = reinterpret_cast<const char *>(kp + row), *vr = reinterpret_cast<const char *>(vp + row);
-            const uint32_t k0 = static_cast<uint32_t>(in_loop(r)) * row_bytes, v0 = 4 * static_cast<uint32_t>(in_loop(g)) * row_bytes;
+            const int64_t row = there ? row_of(__builtin_amdgcn_readlane(page, 16 * k), slot) : 0;
+            const char *base = reinterpret_cast<const char *>(kp + row);
+            const uint32_t step = there ? row_bytes : 0u;
+            const uint32_t off = static_cast<uint32_t>(in_loop(kr)) * step + min(KC * kc, d - KC) * kSize;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const u32x4_t *>(kr + (k0 + min(4 * KC * j + KC * g, d - KC) * kSize));
+            for (int i = 0; i < NJ; ++i)
+                kf[i] = load_cache<Once>(reinterpret_cast<const u32x4_t *>(base + static_cast<uint64_t>(RK * i) * step + off));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NJ; ++i) {
+                const int s = RK * i + kr;
+                const int64_t row = there ? row_of(__shfl(page, 16 * k + s, 64), slot + s) : 0;
+                kf[i] = load_cache<Once>(reinterpret_cast<const u32x4_t *>(kp + row + min(KC * kc, d - KC)));
+            }
+        }
+    };
+    auto load_v = [&](int slot, int k, bool there) {
+        if constexpr (Paged) {
+            const int64_t row = there ? row_of(__builtin_amdgcn_readlane(page, 16 * k), slot) : 0;
+            const char *base = reinterpret_cast<const char *>(vp + row);
+            const uint32_t step = there ? row_bytes : 0u;
+            const uint32_t off = 4 * static_cast<uint32_t>(in_loop(g)) * step;
 #pragma unroll
             for (int i = 0; i < NR; ++i)
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
-                    vf[i][nb] = *reinterpret_cast<const vch_t *>(vr + static_cast<uint64_t>(i) * row_bytes + (v0 + min(16 * CH * nb + CH * r, d - CH) * kSize));
+                    vf[i][nb] = load_cache<Once>(reinterpret_cast<const vch_t *>(
+                        base + static_cast<uint64_t>(i) * step + (off + min(16 * CH * nb + CH * r, d - CH) * kSize)));
         } else {
-            const C *kr = kp + row_of(__shfl(page, 16 * k + r, 64), slot + r);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const u32x4_t *>(kr + min(4 * KC * j + KC * g, d - KC));
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                const C *vr = vp + row_of(__shfl(page, 16 * k + 4 * g + i, 64), slot + 4 * g + i);
+                const int64_t row = there ? row_of(__shfl(page, 16 * k + 4 * g + i, 64), slot + 4 * g + i) : 0;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) vf[i][nb] = *reinterpret_cast<const vch_t *>(vr + min(16 * CH * nb + CH * r, d - CH));
+                for (int nb = 0; nb < NB; ++nb)
+                    vf[i][nb] = load_cache<Once>(reinterpret_cast<const vch_t *>(vp + row + min(16 * CH * nb + CH * r, d - CH)));
             }
         }
     };
-    uint64_t bits = __ballot(seen && j0 + mine < n);  // visible slots: 16 of each of the wavefront's tiles of the split
-    if (j0 + TS * wave < end) load_tile(j0 + TS * wave, 0);
-    const int fresh = a.k_new && n <= end ? n - 1 : -1;  // the new token's slot, if it is in the run
+    const uint64_t bits = __ballot(seen && j0 + mine < n);  // visible slots: 16 of each of the wavefront's tiles
+    load_k(j0 + TS * wave, 0, j0 + TS * wave < end);
+    load_v(j0 + TS * wave, 0, j0 + TS * wave < end);
+    const int fresh = a.k_new && n <= end ? n - 1 : -1;  // the new token's slot, if it is in the split
     if (fresh >= 0 && qt == 0) {
         // its rows into the cache; this launch takes them from k_new and v_new
         const int64_t to = kv_slot(a.c, b, n - 1);
@@ -323,22 +356,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
         for (int e = 0; e < CH; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const float sl2 = a.scale * 1.4426950408889634f;
-    // the new token's row, as the cache stores it, over what was loaded of its slot
+    // the new token's rows, as the cache stores them, over what was loaded of its slot
     auto fresh_rows = [&](int slot) {
-        if (slot + r == fresh) {
-            const IO *row = static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
+        for (int i = 0; i < NJ; ++i)
+            if (slot + RK * i + kr == fresh) {
                 float x[KC];
-                load_row<KC>(row + min(4 * KC * j + KC * in_loop(g), d - KC), x);
+                load_row<KC>(static_cast<const IO *>(a.k_new) + b * a.new_stride + static_cast<int64_t>(kvh) * d + min(KC * in_loop(kc), d - KC), x);
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
                     if constexpr (kHalf)
-                        kf[j][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
+                        kf[i][w] = pack_bf16(x[2 * w], x[2 * w + 1]);
                     else
-                        kf[j][w] = __float_as_uint(x[w]);
+                        kf[i][w] = __float_as_uint(x[w]);
             }
-        }
 #pragma unroll
         for (int i = 0; i < NR; ++i)
             if (slot + 4 * g + i == fresh) {
@@ -356,28 +387,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
                 }
             }
     };
+    // K's rows to LDS, from where they are read as operands; dims past d of a
+    // row count as 0, whatever stands there.
+    unsigned char *const kw = lds + kQBytes + wave * kKBytes;
+    auto stage_k = [&] {
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) {
+            u32x4_t x = kf[i];
+            if (KC * kc >= d) x = u32x4_t{0, 0, 0, 0};
+            *reinterpret_cast<u32x4_t *>(kw + (RK * i + kr) * kKRow + 16 * kc) = x;
+        }
+    };
     // The tile of 16 slots from `slot`, of which `now` are visible, into the
     // running maximum, sum and output of head r; maximum and scores in base 2.
     auto products = [&](int slot, uint32_t now) {
-        if (d != DP) {  // dims past d of a visible row count as 0, whatever stands there
+        // sc[e]: score of slot 4 g + e against head r, by as many chains as a query has operands
+        f32x4_t part[NQ];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-                if (4 * KC * j + KC * g >= d) kf[j] = u32x4_t{0, 0, 0, 0};
-        }
-        f32x4_t sc = {0.f, 0.f, 0.f, 0.f};  // sc[e]: score of slot 4 g + e against head r
+        for (int k = 0; k < NQ; ++k) part[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
+            const u32x4_t kx = *reinterpret_cast<const u32x4_t *>(kw + r * kKRow + 64 * j + 16 * g);
             if constexpr (kHalf) {
 #pragma unroll
                 for (int k = 0; k < NQ; ++k)
-                    sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[j]),
-                                                                 reinterpret_cast<const bf16x8_t *>(lds)[(k * NJ + j) * 64 + lane], sc, 0, 0, 0);
+                    part[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kx),
+                                                                      reinterpret_cast<const bf16x8_t *>(lds)[(k * NJ + j) * 64 + lane], part[k], 0, 0, 0);
             } else {
                 const f32x4_t q = reinterpret_cast<const f32x4_t *>(lds)[j * 64 + lane];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[j][e]), q[e], sc, 0, 0, 0);
+                for (int e = 0; e < 4; ++e) part[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kx[e]), q[e], part[0], 0, 0, 0);
             }
         }
+        f32x4_t sc = part[NQ - 1];  // the smallest first
+#pragma unroll
+        for (int k = NQ - 2; k >= 0; --k) sc += part[k];
         sc *= sl2;
         if (now != 0xffffu) {
 #pragma unroll
@@ -413,14 +457,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int e = 0; e < CH; ++e) {
-                    u32x2_t w;
+                for (int e0 = 0; e0 < CH; e0 += 4) {  // four dims' chains at a time
+                    u32x2_t w[4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        w[i] = __builtin_amdgcn_perm(vf[2 * i + 1][nb][e >> 1], vf[2 * i][nb][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            w[e][i] = __builtin_amdgcn_perm(vf[2 * i + 1][nb][(e0 + e) >> 1], vf[2 * i][nb][(e0 + e) >> 1],
+                                                            e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                     for (int k = 0; k < NP; ++k)
-                        o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_t, w), pf[k], o[nb][e], 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[nb][e0 + e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_t, w[e]), pf[k], o[nb][e0 + e], 0, 0, 0);
                 }
         } else {
 #pragma unroll
@@ -435,72 +484,57 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
     constexpr int OS = DP + 4;  // floats of an output row: padded, so that the heads' rows start in different banks
     float *const ob = reinterpret_cast<float *>(lds + kQBytes);
     const bool whole = n <= kSplit;  // the sequence's only split
-    for (int s0 = j0;;) {  // the run's splits
-        for (int k = 0; k < 4; ++k) {
-            const int slot = s0 + TS * wave + STEP * k;
-            if (slot < end) {
-                if (fresh >= slot && fresh < slot + TS) fresh_rows(slot);
-                products(slot, static_cast<uint32_t>(bits >> (16 * k)) & 0xffffu);
-            }
-            if (k < 3 && slot + STEP < end) load_tile(slot + STEP, k + 1);
+    for (int k = 0; k < 4; ++k) {
+        const int slot = j0 + TS * wave + STEP * k;
+        if (fresh >= slot && fresh < slot + TS) fresh_rows(slot);
+        stage_k();
+        const bool next = k < 3 && slot + STEP < end;
+        load_k(slot + STEP, k + 1, next);
+        if (slot < end) products(slot, static_cast<uint32_t>(bits >> (16 * k)) & 0xffffu);
+        load_v(slot + STEP, k + 1, next);
+    }
+    // the four wavefronts' outputs joined, kJoin heads at a time
+    if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
+    for (int q0 = 0; q0 < nq; q0 += kJoin) {
+        __syncthreads();  // K's rows, or the heads before, have been read
+        if (r >= q0 && r < min(nq, q0 + kJoin)) {
+            float *row = ob + (wave * kJoin + r - q0) * OS + 4 * g;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * (CH * nb + e)) = o[nb][e];
         }
-        const int split = s0 / kSplit;
-        s0 += kSplit;
-        const bool more = s0 < end;
-        if (more) {  // the next split's first tile is on its way while this one's outputs are joined
-            look(s0 + mine);
-            bits = __ballot(seen && s0 + mine < n);
-            if (s0 + TS * wave < end) load_tile(s0 + TS * wave, 0);
-        }
-        // the four wavefronts' outputs joined, kJoin heads at a time
-        if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
-        for (int q0 = 0; q0 < nq; q0 += kJoin) {
-            if (q0) __syncthreads();  // the heads before have been read
-            if (r >= q0 && r < min(nq, q0 + kJoin)) {
-                float *row = ob + (wave * kJoin + in_loop(r) - q0) * OS + 4 * g;
+        __syncthreads();
+        const int dim = tid % DP;
+        const int place = dim / (16 * CH) * (16 * CH) + dim % CH * 16 + dim % (16 * CH) / CH;  // of dim in a row of ob
+        for (int q = q0 + tid / DP; q < min(nq, q0 + kJoin); q += 256 / DP) {
+            const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
+            float L = 0.f, x = 0.f;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * (CH * nb + e)) = o[nb][e];
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
+                L += f * sl[w][q];
+                x += f * ob[(w * kJoin + q - q0) * OS + place];
             }
-            __syncthreads();
-            const int dim = in_loop(tid) % DP;
-            const int place = dim / (16 * CH) * (16 * CH) + dim % CH * 16 + dim % (16 * CH) / CH;  // of dim in a row of ob
-            for (int q = q0 + tid / DP; q < min(nq, q0 + kJoin); q += 256 / DP) {
-                const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
-                float L = 0.f, x = 0.f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
-                    L += f * sl[w][q];
-                    x += f * ob[(w * kJoin + q - q0) * OS + place];
-                }
-                if (dim >= d) continue;
-                const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + split;
-                if (dim == 0 && a.ml) a.ml[rec] = make_float2(M, L);
-                if (whole) {
-                    store_out<IO>(a, b, h0 + q, dim, M == -INFINITY ? 0.f : x / L);
-                    if (dim == 0) store_lse(a, b, h0 + q, M, L);
-                } else {
-                    a.part[rec * d + dim] = x;
-                }
+            if (dim >= d) continue;
+            const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + blockIdx.x;
+            if (dim == 0 && a.ml) a.ml[rec] = make_float2(M, L);
+            if (whole) {
+                store_out<IO>(a, b, h0 + q, dim, M == -INFINITY ? 0.f : x / L);
+                if (dim == 0) store_lse(a, b, h0 + q, M, L);
+            } else {
+                a.part[rec * d + dim] = x;
             }
         }
-        if (!more) break;
-        __syncthreads();  // the outputs have been read
-        m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int e = 0; e < CH; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 }
 
-// Maximum and sum of a head over its splits, by one wavefront, to every lane.
+// Maximum and sum of a head over its splits, by N lanes of a wavefront, to each
+// of them.
+template <int N>
 __device__ __forceinline__ float2 join_ml(const float2 *ml, int ns) {
-    const int lane = threadIdx.x & 63;
     float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < ns; s += 64) {
+    for (int s = threadIdx.x % N; s < ns; s += N) {
         const float2 x = ml[s];
         const float mn = fmaxf(M, x.x);
         if (mn != -INFINITY || x.x != x.x) {
@@ -509,7 +543,7 @@ __device__ __forceinline__ float2 join_ml(const float2 *ml, int ns) {
         }
     }
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
+    for (int off = N / 2; off >= 1; off >>= 1) {
         const float m2 = xor_shfl(M, off), l2 = xor_shfl(L, off), mn = fmaxf(M, m2);
         const float ref = mn == -INFINITY ? 0.f : mn;
         L = L * __builtin_amdgcn_exp2f(M - ref) + l2 * __builtin_amdgcn_exp2f(m2 - ref);
@@ -525,15 +559,27 @@ __device__ __forceinline__ void join_splits(const AttendArgs &a, int64_t b, int 
     const int tid = threadIdx.x, d = a.c.d;
     constexpr int DL = DP / 4, NG = 256 / DL;
     const int64_t rec = (b * a.n_head + h) * a.n_split;
-    const float2 t = join_ml(a.ml + rec, ns);
+    const int dim = 4 * (tid % DL), s0 = tid / DL;
+    // the first kAhead splits' outputs are on their way while the maxima are joined
+    constexpr int kAhead = 4;
+    f32x4_t first[kAhead];
+    float fm[kAhead];
+    const bool in = dim < d;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int s = min(s0 + i * NG, ns - 1);
+        fm[i] = a.ml[rec + s].x;
+        first[i] = *reinterpret_cast<const f32x4_t *>(a.part + (rec + s) * d + (in ? dim : 0));
+    }
+    const float2 t = join_ml<64>(a.ml + rec, ns);
     const float ref = t.x == -INFINITY ? 0.f : t.x;
-    const int dim = 4 * (tid % DL);
     f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-    if (dim < d)
-        for (int s = tid / DL; s < ns; s += NG) {
-            const float f = __builtin_amdgcn_exp2f(a.ml[rec + s].x - ref);
-            x += f * *reinterpret_cast<const f32x4_t *>(a.part + (rec + s) * d + dim);
-        }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (s0 + i * NG < ns) x += __builtin_amdgcn_exp2f(fm[i] - ref) * first[i];
+    if (in)
+        for (int s = s0 + kAhead * NG; s < ns; s += NG)
+            x += __builtin_amdgcn_exp2f(a.ml[rec + s].x - ref) * *reinterpret_cast<const f32x4_t *>(a.part + (rec + s) * d + dim);
     red[tid] = x;
     __syncthreads();
     if (tid >= DP) return;
@@ -551,30 +597,47 @@ constexpr int kWSlots = 512, kWHeads = 64;
 __device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int hs, int j0, int n, float2 *ml) {
     const int tid = threadIdx.x;
     const int ns = (n + kSplit - 1) / kSplit, G = a.n_head / a.h_heads;
-    float w[kWSlots / 256];
+    constexpr int NW = kWSlots / 256;
+    float *const out = a.weight + (b * a.h_heads + hs) * a.h_slots;
+    float w[NW], sum[NW];
 #pragma unroll
-    for (int i = 0; i < kWSlots / 256; ++i) w[i] = 0.f;
+    for (int i = 0; i < NW; ++i) {
+        const int j = j0 + 256 * i + tid;
+        w[i] = j < n ? out[j] : 0.f;
+        sum[i] = 0.f;
+    }
     for (int g0 = 0; g0 < G; g0 += kWHeads) {
         const int ng = min(kWHeads, G - g0);
         const int64_t h0 = b * a.n_head + static_cast<int64_t>(hs) * G + g0;
+        // the first heads' scores are on their way while the maxima are joined
+        constexpr int kAhead = 4;
+        float first[kAhead][NW];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (int i = 0; i < NW; ++i) first[k][i] = a.score[(h0 + min(k, ng - 1)) * a.s_stride + min(j0 + 256 * i + tid, n - 1)];
         __syncthreads();
-        for (int i = tid >> 6; i < ng; i += 4) {
-            const float2 t = join_ml(a.ml + (h0 + i) * a.n_split, ns);
+        for (int i = tid >> 4; i < ng; i += 16) {
+            const float2 t = join_ml<16>(a.ml + (h0 + i) * a.n_split, ns);
             // nothing visible: every score is -inf, and 2^(-inf - 0) = 0
-            if ((tid & 63) == 0) ml[i] = t.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(t.x, 1.0f / t.y);
+            if (tid % 16 == 0) ml[i] = t.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(t.x, 1.0f / t.y);
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kWSlots / 256; ++i) {
+        for (int i = 0; i < NW; ++i) {
             const int j = j0 + 256 * i + tid;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (k < ng) sum[i] += __builtin_amdgcn_exp2f(first[k][i] - ml[k].x) * ml[k].y;
             if (j < n)
-                for (int k = 0; k < ng; ++k) w[i] += __builtin_amdgcn_exp2f(a.score[(h0 + k) * a.s_stride + j] - ml[k].x) * ml[k].y;
+#pragma unroll 8
+                for (int k = kAhead; k < ng; ++k) sum[i] += __builtin_amdgcn_exp2f(a.score[(h0 + k) * a.s_stride + j] - ml[k].x) * ml[k].y;
         }
     }
 #pragma unroll
-    for (int i = 0; i < kWSlots / 256; ++i) {
+    for (int i = 0; i < NW; ++i) {
         const int j = j0 + 256 * i + tid;
-        if (j < n) a.weight[(b * a.h_heads + hs) * a.h_slots + j] += w[i];
+        if (j < n) out[j] = w[i] + sum[i];
     }
 }
 
@@ -598,13 +661,24 @@ template <typename C, typename IO, int DP>
 int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
     constexpr bool kHalf = sizeof(C) == 2;
     constexpr size_t q_bytes = kHalf ? (sizeof(IO) == 4 ? 3 : 1) * DP * 32 : DP * 64;
-    constexpr size_t lds = q_bytes + 4 * kJoin * (DP + 4) * sizeof(float);
-    static_assert(lds + 2 * 4 * kQ * 4 <= 65536, "LDS without an opt-in");
-    const dim3 grid((a.n_split + a.run - 1) / a.run, a.c.n_head_kv * a.q_tiles, seqs);
-    if (a.c.page_shift >= 4)
-        hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP, true>), grid, dim3(256), lds, s, a);
-    else
-        hipLaunchKernelGGL((kv_attend_split_kernel<C, IO, DP, false>), grid, dim3(256), lds, s, a);
+    constexpr size_t o_bytes = 4 * kJoin * (DP + 4) * sizeof(float), k_bytes = 4 * 16 * (DP * sizeof(C) + 16);
+    constexpr size_t lds = q_bytes + (o_bytes > k_bytes ? o_bytes : k_bytes);
+    const dim3 grid(a.n_split, a.c.n_head_kv * a.q_tiles, seqs);
+    const int64_t bytes = static_cast<int64_t>(seqs) * a.max_len * a.c.n_head_kv * a.c.d * 2 * sizeof(C);
+    const int which = (a.c.page_shift >= 4 ? 2 : 0) + (bytes > kKeptBytes);
+    using Kernel = void (*)(AttendArgs);
+    static const Kernel kernels[4] = {kv_attend_split_kernel<C, IO, DP, false, false>, kv_attend_split_kernel<C, IO, DP, false, true>,
+                                      kv_attend_split_kernel<C, IO, DP, true, false>, kv_attend_split_kernel<C, IO, DP, true, true>};
+    if (lds + 1024 > 65536) {  // one opt-in per process and kernel for more than 64 KiB of LDS (idempotent)
+        static std::atomic<bool> done[4];
+        if (!done[which].load(std::memory_order_acquire)) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernels[which]),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+            if (e != hipSuccess) return fail(OURO_ERR_HIP, "ouro_kv_attend: LDS opt-in: %s", hipGetErrorString(e));
+            done[which].store(true, std::memory_order_release);
+        }
+    }
+    hipLaunchKernelGGL(kernels[which], grid, dim3(256), lds, s, a);
     int st = check_launch("kv_attend_split_kernel");
     if (st) return st;
     const int joins = a.n_split > 1 ? a.n_head : 0;
@@ -702,7 +776,6 @@ int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history, c
     a.s_stride = w.s_stride;
     a.n_split = w.n_split;
     a.q_tiles = static_cast<int>((n_head / hkv + kQ - 1) / kQ);
-    a.run = getenv("ORUN") ? atoi(getenv("ORUN")) : 1;
     a.q = q, a.k_new = k_new, a.v_new = v_new, a.gate = gate, a.pos_new = pos_new, a.lens = lens, a.mask = mask, a.out = out, a.lse = lse;
     a.q_stride = q_stride, a.new_stride = new_stride, a.mask_stride = mask_stride, a.out_stride = out_stride;
     a.n_head = static_cast<int>(n_head), a.max_len = static_cast<int>(max_len), a.scale = scale;
