@@ -189,6 +189,7 @@ def token_logprobs(logits, rows: int, n: int, *, dtype="f32", row_stride: int = 
     (f32, or bf16 as uint16) everything is computed and returned as a dict of
     numpy arrays, logprob and rank where targets are given."""
     if not isinstance(logits, np.ndarray):
+        _lib.init()
         call("ouro_token_logprobs", _addr(logits), _lib.dtype_code(dtype), rows, n, row_stride, _addr(targets), k,
              _addr(logprob), _addr(rank), _addr(entropy), _addr(lse), _addr(top_id), _addr(top_logprob),
              _addr(workspace), stream)
