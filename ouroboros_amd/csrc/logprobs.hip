@@ -15,8 +15,8 @@ namespace ouro {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kVec = 8;                     // 16-byte vectors of a thread
-constexpr int kPart = kThreads * kVec;      // vectors of a workgroup: 32 KiB of logits
+constexpr int kLogits = 32;                 // logits of a thread
+constexpr int kPartLogits = kThreads * kLogits;
 constexpr int kSegs = kThreads / 16;        // segments of a part: 16 lanes each
 constexpr int kCap = 2048;                  // candidates that the choice of alternatives holds
 
@@ -50,6 +50,8 @@ __device__ __forceinline__ float logit(const T *x, int64_t i) {
 template <typename T>
 struct Row {
     static constexpr int VL = 16 / sizeof(T);
+    static constexpr int kVec = kLogits / VL;         // vectors of a thread
+    static constexpr int kPart = kPartLogits / VL;    // and of a part
     const T *x;
     int n, shift;
     __device__ __forceinline__ Row(const ScoreArgs &a, int64_t row) : x(static_cast<const T *>(a.x) + row * a.stride), n(a.n) {
@@ -75,13 +77,13 @@ struct Row {
         }
         return r;
     }
-    // Element e of a vector, NaN as -inf.
+    // Element e of a vector as it is, and with NaN as -inf.
+    static __device__ __forceinline__ float raw(const u32x4_t &v, int e) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(v[e]);
+        return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+    }
     static __device__ __forceinline__ float at(const u32x4_t &v, int e) {
-        float f;
-        if constexpr (sizeof(T) == 4)
-            f = __uint_as_float(v[e]);
-        else
-            f = __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+        const float f = raw(v, e);
         return f != f ? -INFINITY : f;
     }
 };
@@ -108,19 +110,13 @@ __device__ __forceinline__ void merge(float &m, float &l, float &s, float m2, fl
     m = M;
 }
 
-// What a row's sums say, written by one thread.
-template <typename T>
-__device__ __forceinline__ void finish(const ScoreArgs &a, int64_t row, float m, float l, float s, int ahead) {
+// What a row's sums say, written by one thread; g the given token, xt its logit.
+__device__ __forceinline__ void finish(const ScoreArgs &a, int64_t row, int g, float xt, float m, float l, float s, int ahead) {
     const float ln = logf(l);
-    const bool empty = m == -INFINITY;
-    const int g = a.target ? a.target[row] : -1;
-    const bool given = g >= 0 && g < a.n;
+    const bool empty = m == -INFINITY, given = g >= 0 && g < a.n;
     if (a.lse) a.lse[row] = empty ? -INFINITY : m + ln;
     if (a.entropy) a.entropy[row] = empty ? 0.f : ln - s / l;
-    if (a.logprob) {
-        const float xt = given ? logit(static_cast<const T *>(a.x) + row * a.stride, g) : 0.f;
-        a.logprob[row] = !given ? 0.f : empty ? -INFINITY : (xt == m ? 0.f : xt - m) - ln;
-    }
+    if (a.logprob) a.logprob[row] = !given ? 0.f : empty ? -INFINITY : (xt == m ? 0.f : xt - m) - ln;
     if (a.rank) a.rank[row] = given ? ahead : -1;
 }
 
@@ -130,7 +126,7 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, int64_t row, float m,
 // lanes.  A row of one part is finished here.
 template <typename T, bool Top>
 __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
-    constexpr int VL = Row<T>::VL;
+    constexpr int VL = Row<T>::VL, kVec = Row<T>::kVec, kPart = Row<T>::kPart;
     __shared__ float4 waves[kThreads / 64];
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.y;
@@ -145,29 +141,29 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
         if (x.first(q) < a.n) v[j] = x.load(q);
     }
     const int g = a.target ? a.target[row] : -1;
+    const float xt = g >= 0 && g < a.n ? logit(x.x, g) : 0.f;
     const bool given = a.rank && g >= 0 && g < a.n;
-    const float xt = given ? logit(x.x, g) : 0.f;
     float mt = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
 #pragma unroll
-        for (int e = 0; e < VL; ++e) mt = fmaxf(mt, Row<T>::at(v[j], e));
+        for (int e = 0; e < VL; ++e) mt = fmaxf(mt, Row<T>::raw(v[j], e));  // passes over a NaN
     const float ms = row16_max(mt);
     float m = fmaxf(ms, xor_shfl(ms, 16));
     m = fmaxf(m, xor_shfl(m, 32));
     float l = 0.f, s = 0.f;
-    if (m == INFINITY) {
-#pragma unroll
+    if (m == INFINITY) {  // shared by the logits that are +inf
         for (int j = 0; j < kVec; ++j)
 #pragma unroll
-            for (int e = 0; e < VL; ++e) l += Row<T>::at(v[j], e) == INFINITY ? 1.f : 0.f;
+            for (int e = 0; e < VL; ++e) l += Row<T>::raw(v[j], e) == INFINITY ? 1.f : 0.f;
     } else if (m != -INFINITY) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
             float lj = 0.f, sj = 0.f;  // short chains
 #pragma unroll
             for (int e = 0; e < VL; ++e) {
-                const float d = fmaxf(Row<T>::at(v[j], e) - m, -3e38f);  // e^d (-inf) would be 0 (-inf)
+                // the maximum takes a NaN and -inf alike to where e^d = 0 and e^d d = 0
+                const float d = fmaxf(Row<T>::raw(v[j], e) - m, -3e38f);
                 const float p = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
                 lj += p;
                 sj += p * d;
@@ -176,32 +172,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
             s += sj;
         }
     }
+    // tokens ahead, counted for the wavefront in scalar registers
     int ahead = 0;
     if (given) {
-        const int lo = x.first(q0), hi = x.first(q0 + kPart);  // the part's elements, shift aside
-        if (hi <= g) {
+        const int lo = x.first(q0), hi = x.first(q0 + kPart);  // the part's elements
+        if (xt != -INFINITY && hi <= g) {
 #pragma unroll
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
-                for (int e = 0; e < VL; ++e) ahead += Row<T>::at(v[j], e) >= xt;
-            if (xt == -INFINITY) {  // the places of no element are -inf too
-                ahead = 0;
-                for (int j = 0; j < kVec; ++j)
-                    for (int e = 0; e < VL; ++e) ahead += x.first(q0 + kThreads * j + tid) + e >= 0;
-            }
+                for (int e = 0; e < VL; ++e) ahead += __popcll(__ballot(Row<T>::raw(v[j], e) >= xt));
         } else if (lo > g) {
 #pragma unroll
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
-                for (int e = 0; e < VL; ++e) ahead += Row<T>::at(v[j], e) > xt;
+                for (int e = 0; e < VL; ++e) ahead += __popcll(__ballot(Row<T>::raw(v[j], e) > xt));
         } else {
-#pragma unroll
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
                 for (int e = 0; e < VL; ++e) {
                     const int i = x.first(q0 + kThreads * j + tid) + e;
                     const float f = Row<T>::at(v[j], e);
-                    ahead += f > xt || (f == xt && i >= 0 && i < g);
+                    ahead += __popcll(__ballot(f > xt || (f == xt && i >= 0 && i < g)));
                 }
         }
     }
@@ -221,7 +212,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
     for (int off = 32; off >= 1; off >>= 1) {
         l += xor_shfl(l, off);
         s += xor_shfl(s, off);
-        ahead += xor_shfl(ahead, off);
     }
     if ((tid & 63) == 0) waves[tid >> 6] = make_float4(m, l, s, __int_as_float(ahead));
     __syncthreads();
@@ -233,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
         ahead += __float_as_int(o.w);
     }
     if (a.parts == 1 && !a.k)
-        finish<T>(a, row, m, l, s, ahead);
+        finish(a, row, g, xt, m, l, s, ahead);
     else
         a.part[row * a.parts + blockIdx.x] = make_float4(m, l, s, __int_as_float(ahead));
 }
@@ -249,63 +239,65 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
     __shared__ unsigned long long cand[kCap];
-    __shared__ unsigned long long group[64];
+    __shared__ int32_t list[kCap];
     __shared__ unsigned long long bound;
     __shared__ float m_all, ln_all;
-    __shared__ float4 sums[kThreads / 64];
-    __shared__ int count;
-    constexpr int VL = Row<T>::VL;
+    __shared__ int n_cand, n_list;
+    constexpr int VL = Row<T>::VL, kVec = Row<T>::kVec, kPart = Row<T>::kPart;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
     const Row<T> x(a, row);
     const int ns = a.parts * kSegs;
     const unsigned long long *seg = a.seg + row * ns;
     // the groups' largest keys: thread t takes segments t, t + 256, ..: group t % 64
+    unsigned long long first = 0;  // the thread's first segment's key
     if (a.k) {
-        unsigned long long best = 0;
-        for (int i = tid; i < ns; i += kThreads) best = argmax_key_max(best, seg[i]);
+        first = tid < ns ? seg[tid] : 0ull;
+        unsigned long long best = first;
+        for (int i = tid + kThreads; i < ns; i += kThreads) best = argmax_key_max(best, seg[i]);
         cand[tid] = best;
+        __syncthreads();
     }
-    // the sums, a part a thread
-    float m = -INFINITY, l = 0.f, s = 0.f;
-    int ahead = 0;
-    for (int p = tid; p < a.parts; p += kThreads) {
-        const float4 o = a.part[row * a.parts + p];
-        if (o.x != -INFINITY) merge(m, l, s, o.x, o.y, o.z);
-        ahead += __float_as_int(o.w);
-    }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const float m2 = xor_shfl(m, off), l2 = xor_shfl(l, off), s2 = xor_shfl(s, off);
-        if (m2 != -INFINITY || m != -INFINITY) {
-            // the same order of the two on both lanes, so that they agree
-            float ma = lane & off ? m2 : m, la = lane & off ? l2 : l, sa = lane & off ? s2 : s;
-            merge(ma, la, sa, lane & off ? m : m2, lane & off ? l : l2, lane & off ? s : s2);
-            m = ma, l = la, s = sa;
-        }
-        ahead += xor_shfl(ahead, off);
-    }
-    if (lane == 0) sums[wave] = make_float4(m, l, s, __int_as_float(ahead));
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) {
-            const float4 o = sums[w];
+    if (wave == 1) {
+        // the sums, a part a lane
+        const int g = a.target ? a.target[row] : -1;
+        const float xt = g >= 0 && g < a.n ? logit(x.x, g) : 0.f;
+        float m = -INFINITY, l = 0.f, s = 0.f;
+        int ahead = 0;
+        for (int p = lane; p < a.parts; p += 64) {
+            const float4 o = a.part[row * a.parts + p];
             if (o.x != -INFINITY) merge(m, l, s, o.x, o.y, o.z);
             ahead += __float_as_int(o.w);
         }
-        finish<T>(a, row, m, l, s, ahead);
-        m_all = m;
-        ln_all = logf(l);
+        float M = m;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, xor_shfl(M, off));
+        if (M != -INFINITY) merge(m, l, s, M, 0.f, 0.f);  // against the row's maximum
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            l += xor_shfl(l, off);
+            s += xor_shfl(s, off);
+            ahead += xor_shfl(ahead, off);
+        }
+        if (lane == 0) {
+            finish(a, row, g, xt, M, l, s, ahead);
+            m_all = M;
+            ln_all = logf(l);
+        }
     }
     if (!a.k) return;
-    if (tid < 64) group[tid] = argmax_key_max(argmax_key_max(cand[tid], cand[tid + 64]), argmax_key_max(cand[tid + 128], cand[tid + 192]));
-    if (tid == 0) bound = 1;  // every logit above -inf, where fewer than k groups have one
-    __syncthreads();
-    if (tid < 64) {
-        const unsigned long long mine = group[tid];
+    if (wave == 0) {
+        const unsigned long long mine = argmax_key_max(argmax_key_max(cand[lane], cand[lane + 64]), argmax_key_max(cand[lane + 128], cand[lane + 192]));
         int before = 0;
-        for (int i = 0; i < 64; ++i) before += group[i] > mine;
+#pragma unroll 8
+        for (int i = 0; i < 64; ++i) {
+            const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine >> 32), i);
+            const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine), i);
+            before += (static_cast<unsigned long long>(hi) << 32 | lo) > mine;
+        }
+        if (lane == 0) bound = 1;  // every logit above -inf, where fewer than k groups have one
         if (mine && before == a.k - 1) bound = mine;  // keys are unique
+        if (lane == 0) n_list = n_cand = 0;
     }
     __syncthreads();
     const unsigned long long least = bound;
@@ -313,36 +305,34 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
     bool by_value = true;  // the first raise goes past the bound's own value
     int c;
     for (;;) {
+        // the segments that reach the bound, then their logits that do
+        for (int i = tid; i < ns; i += kThreads)
+            if ((i == tid ? first : seg[i]) >= cur) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < kCap) list[at] = i;
+            }
         __syncthreads();
-        if (tid == 0) count = 0;
-        __syncthreads();
-        // wavefront w looks at segments 64 w .. , and reads each that reaches the bound
-        for (int i0 = 64 * wave; i0 < ns; i0 += kThreads) {
-            const bool in = i0 + lane < ns && seg[i0 + lane] >= cur;
-            unsigned long long set = __ballot(in);
-            while (set) {
-                const int i = i0 + __ffsll(set) - 1;
-                set &= set - 1;
-                const int base = i / kSegs * kPart + i % kSegs * 16;
-                for (int u = lane; u < 16 * kVec; u += 64) {
-                    const int q = base + (u >> 4) * kThreads + (u & 15);
-                    if (x.first(q) >= a.n) continue;
-                    const u32x4_t v = x.load(q);
+        const int nl = n_list;
+        if (nl <= kCap) {
+            for (int u = tid; u < nl * 16 * kVec; u += kThreads) {
+                const int i = list[u / (16 * kVec)], w = u % (16 * kVec);
+                const int q = i / kSegs * kPart + i % kSegs * 16 + (w >> 4) * kThreads + (w & 15);
+                if (x.first(q) >= a.n) continue;
+                const u32x4_t v = x.load(q);
 #pragma unroll
-                    for (int e = 0; e < VL; ++e) {
-                        const float f = Row<T>::at(v, e);
-                        if (f == -INFINITY) continue;
-                        const unsigned long long key = argmax_key(f, static_cast<unsigned>(x.first(q) + e));
-                        if (key >= cur) {
-                            const int at = atomicAdd(&count, 1);
-                            if (at < kCap) cand[at] = key;
-                        }
+                for (int e = 0; e < VL; ++e) {
+                    const float f = Row<T>::at(v, e);
+                    if (f == -INFINITY) continue;
+                    const unsigned long long key = argmax_key(f, static_cast<unsigned>(x.first(q) + e));
+                    if (key >= cur) {
+                        const int at = atomicAdd(&n_cand, 1);
+                        if (at < kCap) cand[at] = key;
                     }
                 }
             }
         }
         __syncthreads();
-        c = count;
+        c = nl <= kCap ? n_cand : kCap + 1;  // a segment in the list has a candidate at least
         if (c <= kCap && (c >= a.k || cur == least)) break;
         if (c > kCap)
             lo = cur;
@@ -353,21 +343,23 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
         else
             cur = lo + (hi - lo) / 2;
         by_value = false;
+        __syncthreads();
+        if (tid == 0) n_list = n_cand = 0;
+        __syncthreads();
     }
     const float mm = m_all, ln = ln_all;
-    for (int i = tid; i < a.k; i += kThreads)
-        if (i >= c) {
-            a.top_id[row * a.k + i] = -1;
-            a.top_logprob[row * a.k + i] = -INFINITY;
-        }
+    for (int i = c + tid; i < a.k; i += kThreads) {
+        a.top_id[row * a.k + i] = -1;
+        a.top_logprob[row * a.k + i] = -INFINITY;
+    }
     for (int i = tid; i < c; i += kThreads) {
         const unsigned long long mine = cand[i];
         int before = 0;
         for (int j = 0; j < c; ++j) before += cand[j] > mine;
         if (before < a.k) {
-            const int id = argmax_index(mine);
-            const float f = logit(x.x, id);
-            a.top_id[row * a.k + before] = id;
+            const uint32_t u = static_cast<uint32_t>(mine >> 32);  // the logit, as argmax_key ordered it
+            const float f = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+            a.top_id[row * a.k + before] = argmax_index(mine);
             a.top_logprob[row * a.k + before] = (f == mm ? 0.f : f - mm) - ln;
         }
     }
@@ -400,8 +392,8 @@ int launch(const ScoreArgs &a, unsigned rows, hipStream_t s) {
 // Parts of a row that may start anywhere in a vector, and the workspace of a
 // launch of up to 65535 rows.
 int parts_of(size_t n, size_t size) {
-    const size_t vl = 16 / size, vectors = (n + 2 * (vl - 1)) / vl;
-    return static_cast<int>((vectors + kPart - 1) / kPart);
+    const size_t vl = 16 / size, vectors = (n + 2 * (vl - 1)) / vl, part = kPartLogits / vl;
+    return static_cast<int>((vectors + part - 1) / part);
 }
 struct ScoreWs {
     size_t seg, bytes;
@@ -423,7 +415,8 @@ using namespace ouro;
 extern "C" {
 
 size_t ouro_token_logprobs_workspace_bytes(size_t rows, size_t n, size_t k) {
-    return score_ws(rows, parts_of(n, 4), k).bytes;  // fp32 rows have the most parts
+    const int a = parts_of(n, 4), b = parts_of(n, 2);
+    return score_ws(rows, a > b ? a : b, k).bytes;
 }
 
 int ouro_token_logprobs(const void *logits, int dtype, size_t rows, size_t n, size_t row_stride, const int32_t *targets,
