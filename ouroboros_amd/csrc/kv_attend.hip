@@ -32,7 +32,7 @@ int kv_view(const ouro_kv_cache *c, const char *what, KvView *out) {
     int shift = 0;
     while ((1 << shift) < c->page_tokens) ++shift;
     *out = KvView{c->k, c->v, c->pages, c->page_stride, c->token_stride, c->head_stride,
-                  c->n_pages, c->max_pages, shift, c->n_head_kv, c->head_dim, 0};
+                  c->n_pages, c->max_pages, shift, c->n_head_kv, c->head_dim, c->dtype == OURO_DT_F32 ? 4 : 2};
     return OURO_OK;
 }
 

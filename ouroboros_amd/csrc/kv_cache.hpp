@@ -15,7 +15,7 @@ struct KvView {
     const int32_t *pages;
     int64_t page_stride, token_stride, head_stride;  // elements
     int32_t n_pages, max_pages, page_shift, n_head_kv, d;
-    int32_t pad;
+    int32_t elem;  // bytes of an element
 };
 // passed by value to kernels: the host and device passes must lay it out alike
 static_assert(sizeof(KvView) == 72, "KvView: kernel argument layout");
