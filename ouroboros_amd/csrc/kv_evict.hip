@@ -32,47 +32,61 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 // lowest, -0 as +0).
 constexpr uint32_t kGoes = 0u, kStays = 0xffffffffu, kLeast = 1u, kMost = 0xff800000u;
 __device__ __forceinline__ uint32_t weight_order(float w) {
-    if (w != w) return kLeast;
-    const uint32_t u = __float_as_uint(w == 0.f ? 0.f : w);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t u = __float_as_uint(w + 0.f);
+    return w != w ? kLeast : u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 
-// Over lanes 0 .. W - 1 of each 16 (W 4 or 16), to each of them.
-template <int W, typename F>
+// Lanes of the mask below this one.
+__device__ __forceinline__ int rank_in(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
+// Over the 16 lanes of a row of the wavefront, to each of them.
+template <typename F>
 __device__ __forceinline__ int row_join(int v, F f) {
-    if constexpr (W == 16) {
-        v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false));
-        v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));
-    }
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));
     v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false));
     return f(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false));
 }
 
-// Copies rows of k and v of one (kv head, sequence): `lanes` lanes a row, from
-// the pair `first` on in steps of `step`.
+// Copies rows of k and v of one (kv head, sequence), lanes of 16 bytes, from the
+// pair `first` on in steps of `step`.
 __device__ __forceinline__ void move_rows(const EvictArgs &a, int64_t b, int h, const int2 *move, int n, int first, int step, int lane) {
+    if (lane >= a.vecs) return;
+    const int64_t head = h * a.c.head_stride * a.c.elem + lane * 16;
+    char *k = static_cast<char *>(a.c.k) + head, *v = static_cast<char *>(a.c.v) + head;
     for (int i = first; i < n; i += step) {
         const int2 m = move[i];
-        const int64_t dst = kv_slot(a.c, b, m.x), src = kv_slot(a.c, b, m.y);
-        if (src < 0 || dst < 0 || lane >= a.vecs) continue;
-        const int64_t size = a.c.elem;
-        const char *k = static_cast<const char *>(a.c.k), *v = static_cast<const char *>(a.c.v);
-        const int64_t from = (src + h * a.c.head_stride) * size + lane * 16, to = (dst + h * a.c.head_stride) * size + lane * 16;
-        const u32x4_t x = *reinterpret_cast<const u32x4_t *>(k + from), y = *reinterpret_cast<const u32x4_t *>(v + from);
-        *reinterpret_cast<u32x4_t *>(static_cast<char *>(a.c.k) + to) = x;
-        *reinterpret_cast<u32x4_t *>(static_cast<char *>(a.c.v) + to) = y;
+        const int64_t dst = kv_slot(a.c, b, m.x) * a.c.elem, src = kv_slot(a.c, b, m.y) * a.c.elem;
+        if (src < 0 || dst < 0) continue;  // a hole
+        const u32x4_t x = *reinterpret_cast<const u32x4_t *>(k + src), y = *reinterpret_cast<const u32x4_t *>(v + src);
+        *reinterpret_cast<u32x4_t *>(k + dst) = x;
+        *reinterpret_cast<u32x4_t *>(v + dst) = y;
     }
 }
 
-// The choice of one (head, sequence) by one workgroup of W wavefronts, each
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kBinBits = 11, kBins = 1 << kBinBits, kCopies = 4;  // bins of a count, and how many lanes' counts share one
+
+// The choice of one (head, sequence) by one workgroup of 16 wavefronts, each
 // with a run of slots in order, 64 R of them in registers (longer runs are read
-// again at each pass).  The order of the last slot that stays is searched for
-// with three counts a round; counts are of ballots, and a round's are joined
-// through LDS with one barrier.  Moves: the workgroup copies the rows too.
-template <int W, int R, bool Moves>
-__global__ __launch_bounds__(W * 64) void kv_choose_kernel(EvictArgs a) {
-    constexpr int kThreads = W * 64;
-    __shared__ int4 tmp[2][W];
+// again at each pass).  The runs' blocks of 64 start so that one starts at
+// slot `keep`: what a block's slots may become is the same for all of them.  The order of the last slot that stays is found from
+// counts in bins, from the largest order down, first of all orders, then of the
+// bin that holds it.  Moves: the workgroup copies the rows too.
+//
+// Bound by instructions and barriers: a pass over 16384 slots costs a workgroup
+// 256 cycles for each instruction a slot takes, a barrier about 400.  Four rows
+// of 16384 slots and 4 heads, a workgroup each: 17 us, of which the counts in
+// bins 4, the two passes over what stays 5, loads 2.  64 rows of 1025 slots, 4
+// heads: 7.8 us with the launch.  Counting thresholds with ballots, 12 rounds of
+// three, took 33 us where the bins take 19.
+template <int R, bool Moves>
+__global__ __launch_bounds__(kThreads) void kv_choose_kernel(EvictArgs a) {
+    __shared__ int4 tmp[2][kWaves];
+    __shared__ __align__(16) int bins[kBins * kCopies];
+    __shared__ int4 found;
     const int hs = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int64_t b = blockIdx.y, row = b * a.heads + hs;
@@ -91,31 +105,33 @@ __global__ __launch_bounds__(W * 64) void kv_choose_kernel(EvictArgs a) {
             for (int j = t; j < n; j += kThreads) w_out[j] = weight[j], pos_out[j] = pos[j];
         return;
     }
+    for (int i = t; i < kBins; i += kThreads) reinterpret_cast<int4 *>(bins)[i] = make_int4(0, 0, 0, 0);
     int round = 0;
     // A wavefront's counts joined: the sums over all wavefronts, and those over
     // the ones before it.
     int4 all, before;
-    auto join = [&](int x, int y, int z) {
+    auto join = [&](int x, int y, int z) __attribute__((always_inline)) {
         int4 *buf = tmp[round++ & 1];  // a wavefront is at most one round ahead
         if (lane == 0) buf[wave] = make_int4(x, y, z, 0);
         __syncthreads();
-        const int4 o = buf[lane % W];
+        const int4 o = buf[lane % kWaves];
         auto add = [](int p, int q) { return p + q; };
-        const bool is = lane % W < wave;
-        all = make_int4(row_join<W>(o.x, add), row_join<W>(o.y, add), row_join<W>(o.z, add), 0);
-        before = make_int4(row_join<W>(is ? o.x : 0, add), row_join<W>(is ? o.y : 0, add), row_join<W>(is ? o.z : 0, add), 0);
+        const bool is = lane % kWaves < wave;
+        all = make_int4(row_join(o.x, add), row_join(o.y, add), row_join(o.z, add), 0);
+        before = make_int4(row_join(is ? o.x : 0, add), row_join(is ? o.y : 0, add), row_join(is ? o.z : 0, add), 0);
     };
-    const int run = ((n + kThreads - 1) / kThreads) * 64;  // slots of a wavefront
-    const int j0 = wave * run, end = min(n, j0 + run);
+    const int front = -keep & 63;  // places before slot 0
+    const int run = (n + front + kThreads - 1) / kThreads * 64;  // places of a wavefront
+    const int j0 = wave * run - front;
     float w[R];
-    int32_t p[R];
+    uint32_t u[R];  // the position, then how far it is behind the newest
     uint32_t o[R];
-    auto load = [&](int c) {
+    auto slot = [&](int c, int i) __attribute__((always_inline)) { return c + i * 64 < run && static_cast<uint32_t>(j0 + c + i * 64 + lane) < static_cast<uint32_t>(n); };
+    auto load = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int j = j0 + c + i * 64 + lane;
-            w[i] = 0.f, p[i] = INT32_MIN;
-            if (c + i * 64 < run && j < end) w[i] = weight[j], p[i] = pos[j];
+            w[i] = 0.f, u[i] = static_cast<uint32_t>(INT32_MIN);
+            if (slot(c, i)) w[i] = weight[j0 + c + i * 64 + lane], u[i] = pos[j0 + c + i * 64 + lane];
         }
     };
     const bool once = run <= 64 * R;
@@ -125,7 +141,7 @@ __global__ __launch_bounds__(W * 64) void kv_choose_kernel(EvictArgs a) {
     for (int c = 0; c < run; c += 64 * R) {
         if (c) load(c);
 #pragma unroll
-        for (int i = 0; i < R; ++i) newest = max(newest, p[i]);
+        for (int i = 0; i < R; ++i) newest = max(newest, static_cast<int>(u[i]));
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) newest = max(newest, xor_shfl(newest, off));
@@ -133,104 +149,128 @@ __global__ __launch_bounds__(W * 64) void kv_choose_kernel(EvictArgs a) {
         int4 *buf = tmp[round++ & 1];
         if (lane == 0) buf[wave].x = newest;
         __syncthreads();
-        newest = row_join<W>(buf[lane % W].x, [](int x, int y) { return x > y ? x : y; });
+        newest = row_join(buf[lane % kWaves].x, [](int x, int y) { return x > y ? x : y; });
     }
-    const int64_t line = static_cast<int64_t>(newest) - a.recent;
-    int news = 0;
-    for (int c = 0; c < run; c += 64 * R) {
+    // new: newest - pos < recent, a difference that 32 bits hold unsigned
+    const uint32_t recent = a.recent;
+    auto behind = [&](int c) __attribute__((always_inline)) {
         if (!once) load(c);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (c + i * 64 >= run) break;
-            news += __popcll(__ballot(j0 + c + i * 64 + lane < end && p[i] > line));
-        }
+        for (int i = 0; i < R; ++i) u[i] = slot(c, i) ? newest - u[i] : 0xffffffffu;
+    };
+    int news = 0;
+    for (int c = 0; c < run; c += 64 * R) {
+        behind(c);
+#pragma unroll
+        for (int i = 0; i < R; ++i) news += __popcll(__ballot(u[i] < recent));
     }
     join(news, 0, 0);
     // whichever class is cut: the newest alone where they fill the budget, else the others
     const bool cut = all.x >= keep;
-    auto orders = [&](int c) {
-        if (!once) load(c);
+    const uint32_t other = cut ? kGoes : kStays;
+    auto orders = [&](int c) __attribute__((always_inline)) {
+        if (!once) behind(c);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const bool is_new = p[i] > line;
-            o[i] = is_new == cut ? weight_order(w[i]) : is_new ? kStays : kGoes;
-            if (j0 + c + i * 64 + lane >= end) o[i] = kGoes;
+            o[i] = (u[i] < recent) == cut ? weight_order(w[i]) : other;
+            if (!slot(c, i)) o[i] = kGoes;
         }
     };
     if (once) orders(0);
-    // the largest order that `keep` slots reach: in lo .. hi
+    // the largest order that `keep` slots reach, in lo .. hi
     uint32_t lo = kLeast, hi = kMost;
-    int ties = 0;      // how many at the order itself stay
+    int need = cut ? keep : keep - all.x;  // slots of lo .. hi that stay
     bool exact = false;
-    while (lo < hi) {
-        const uint32_t q = max(1u, (hi - lo) >> 2), c1 = lo + q, c2 = c1 + q, c3 = c2 + q;
-        int n1 = 0, n2 = 0, n3 = 0;
+    for (;;) {
+        const int shift = max(0, 32 - static_cast<int>(__clz(hi - lo)) - kBinBits);
         for (int c = 0; c < run; c += 64 * R) {
             if (!once) orders(c);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 if (c + i * 64 >= run) break;
-                n1 += __popcll(__ballot(o[i] >= c1));
-                n2 += __popcll(__ballot(o[i] >= c2));
-                n3 += __popcll(__ballot(o[i] >= c3));
+                if (o[i] - lo <= hi - lo) atomicAdd(&bins[((hi - o[i]) >> shift) * kCopies + lane % kCopies], 1);
             }
         }
-        join(n1, n2, n3);
-        const int m1 = __builtin_amdgcn_readfirstlane(all.x), m2 = __builtin_amdgcn_readfirstlane(all.y), m3 = __builtin_amdgcn_readfirstlane(all.z);
-        if (m1 == keep || m2 == keep || m3 == keep) {  // exactly those above lo stay
-            lo = (m1 == keep ? c1 : m2 == keep ? c2 : c3) - 1;
+        __syncthreads();
+        int mine[kBins / kThreads], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kBins / kThreads; ++i) {
+            int4 *bin = reinterpret_cast<int4 *>(bins) + t * (kBins / kThreads) + i;
+            const int4 q = *bin;
+            *bin = make_int4(0, 0, 0, 0);
+            sum += mine[i] = q.x + q.y + q.z + q.w;
+        }
+        int up = sum;  // over the lanes up to this one
+        up += __builtin_amdgcn_update_dpp(0, up, 0x111, 0xf, 0xf, false);
+        up += __builtin_amdgcn_update_dpp(0, up, 0x112, 0xf, 0xf, false);
+        up += __builtin_amdgcn_update_dpp(0, up, 0x114, 0xf, 0xf, false);
+        up += __builtin_amdgcn_update_dpp(0, up, 0x118, 0xf, 0xf, false);
+        up += __builtin_amdgcn_update_dpp(0, up, 0x142, 0xa, 0xf, false);
+        up += __builtin_amdgcn_update_dpp(0, up, 0x143, 0xc, 0xf, false);
+        join(__builtin_amdgcn_readlane(up, 63), 0, 0);
+        int past = before.x + up - sum;  // in the bins of larger orders
+#pragma unroll
+        for (int i = 0; i < kBins / kThreads; ++i) {
+            if (past < need && past + mine[i] >= need) found = make_int4(t * (kBins / kThreads) + i, past, mine[i], 0);
+            past += mine[i];
+        }
+        __syncthreads();
+        const int bin = __builtin_amdgcn_readfirstlane(found.x), over = __builtin_amdgcn_readfirstlane(found.y), in = __builtin_amdgcn_readfirstlane(found.z);
+        hi -= static_cast<uint32_t>(bin) << shift;
+        const uint32_t width = (1u << shift) - 1;
+        if (hi - lo > width) lo = hi - width;
+        need -= over;
+        if (need == in) {  // those of the bin stay to the last
+            --lo;
             exact = true;
             break;
         }
-        if (m3 >= keep)
-            lo = c3;
-        else if (m2 >= keep)
-            lo = c2, hi = c3 - 1;
-        else if (m1 >= keep)
-            lo = c1, hi = c2 - 1;
-        else
-            hi = c1 - 1;
+        if (lo == hi) break;
     }
-    int tied = 0;  // those at lo in the wavefronts before
+    // of those at lo, the slots up to `last` stay
+    int last = -1;
     if (!exact) {
-        int above = 0, at = 0;
+        int at = 0;
         for (int c = 0; c < run; c += 64 * R) {
             if (!once) orders(c);
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (c + i * 64 >= run) break;
-                above += __popcll(__ballot(o[i] > lo));
-                at += __popcll(__ballot(o[i] == lo));
-            }
+            for (int i = 0; i < R; ++i) at += __popcll(__ballot(o[i] == lo));
         }
-        join(above, at, 0);
-        ties = keep - all.x;
-        tied = before.y;
+        join(at, 0, 0);
+        int seen = __builtin_amdgcn_readfirstlane(before.x);
+        if (seen < need && seen + at >= need)
+            for (int c = 0; c < run; c += 64 * R) {
+                if (!once) orders(c);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const unsigned long long is = __ballot(o[i] == lo);
+                    if (o[i] == lo && seen + rank_in(is) == need - 1) found.x = j0 + c + i * 64 + lane;
+                    seen += __popcll(is);
+                }
+            }
+        __syncthreads();
+        last = __builtin_amdgcn_readfirstlane(found.x);
     }
+    auto stays = [&](int c, int i) __attribute__((always_inline)) { return __ballot(o[i] > (i * 64 <= last - j0 - c - lane ? lo - 1 : lo)); };
     // those that go below `keep`, those that stay from it on
-    const unsigned long long below = (1ull << lane) - 1;
-    auto stays = [&](int i, int &seen) {
-        const bool is = !exact && o[i] == lo;
-        const unsigned long long bal = __ballot(is);
-        const int r = seen + __popcll(bal & below);
-        seen += __popcll(bal);
-        return o[i] > lo || (is && r < ties);
-    };
-    int holes = 0, movers = 0, seen = tied;
+    int under = 0, over = 0;
+    const int cross = keep - j0;  // the first of the run's places from `keep` on
     for (int c = 0; c < run; c += 64 * R) {
         if (!once) orders(c);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             if (c + i * 64 >= run) break;
-            const int j = j0 + c + i * 64 + lane;
-            const bool s = stays(i, seen);
-            holes += __popcll(__ballot(!s && j < end && j < keep));
-            movers += __popcll(__ballot(s && j >= keep));
+            const int s = __popcll(stays(c, i));
+            if (c + i * 64 < cross)
+                under += 64 - s;
+            else
+                over += s;
         }
     }
-    join(holes, movers, 0);
+    if (wave == 0) under -= front;
+    join(under, over, 0);
     const int moves = all.y;
-    holes = before.x, movers = before.y, seen = tied;
+    int hole = __builtin_amdgcn_readfirstlane(before.x), mover = __builtin_amdgcn_readfirstlane(before.y);
     int2 *move = a.move + row * a.most;
     for (int c = 0; c < run; c += 64 * R) {
         if (!once) orders(c);
@@ -238,16 +278,21 @@ __global__ __launch_bounds__(W * 64) void kv_choose_kernel(EvictArgs a) {
         for (int i = 0; i < R; ++i) {
             if (c + i * 64 >= run) break;
             const int j = j0 + c + i * 64 + lane;
-            const bool s = stays(i, seen);
-            const bool hole = !s && j < end && j < keep, mover = s && j >= keep;
-            const unsigned long long hb = __ballot(hole), mb = __ballot(mover);
-            if (hole) move[holes + __popcll(hb & below)].x = j;
-            if (mover) move[movers + __popcll(mb & below)].y = j;
-            holes += __popcll(hb);
-            movers += __popcll(mb);
-            if (s && j < keep) {
-                from[j] = j;
-                if (apart) w_out[j] = w[i], pos_out[j] = p[i];
+            const unsigned long long s = stays(c, i);
+            if (c + i * 64 < cross) {
+                if (s >> lane & 1) {
+                    from[j] = j;
+                    if (apart) w_out[j] = w[i], pos_out[j] = newest - u[i];
+                }
+                unsigned long long goes = ~s;
+                if (i == 0 && j0 + c < 0) goes &= ~0ull << front;
+                if (goes) {
+                    if (goes >> lane & 1) move[hole + rank_in(goes)].x = j;
+                    hole += __popcll(goes);
+                }
+            } else if (s) {
+                if (s >> lane & 1) move[mover + rank_in(s)].y = j;
+                mover += __popcll(s);
             }
         }
     }
@@ -269,7 +314,9 @@ __global__ __launch_bounds__(W * 64) void kv_choose_kernel(EvictArgs a) {
 
 constexpr int kMoveThreads = 256;
 
-// One workgroup a (kv head, sequence) and share of its moves.
+// One workgroup a (kv head, sequence) and share of its moves: bound by memory,
+// 100 MB read and written in 24 us (4.2 TB/s; a large copy reaches 4.9).  Four
+// rows in flight a lane instead of one took as long.
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(EvictArgs a) {
     const int lanes = a.vecs <= 16 ? 16 : a.vecs <= 32 ? 32 : 64;
     const int h = blockIdx.y, t = threadIdx.x;
@@ -278,7 +325,10 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(EvictArgs a) {
     move_rows(a, b, h, a.move + row * a.most, a.moves[row], blockIdx.x * groups + t / lanes, gridDim.x * groups, t % lanes);
 }
 
-constexpr size_t kFew = 64;  // moves a sequence and head up to which the choosing workgroup makes them
+// Bytes of moved rows up to which the choosing workgroup moves them itself.  64
+// sequences and 4 heads: 256 moves of 512 bytes (128 KiB) 18.1 us by it, 21.6 by
+// a second launch, one move 7.8 and 11.1; 48 and 4, up to 512 moves: 38.7 and 32.9.
+constexpr size_t kFew = 128 << 10;
 
 // Moves of a (sequence, head) at the most.
 size_t most_moves(size_t max_len, size_t keep) {
@@ -292,10 +342,16 @@ size_t evict_ws_bytes(size_t seqs, size_t heads, size_t max_len, size_t keep) {
 template <bool Moves>
 void choose(const EvictArgs &a, unsigned seqs, hipStream_t s) {
     const dim3 grid(a.heads, seqs);
-    if (a.max_len <= 2048)
-        hipLaunchKernelGGL((kv_choose_kernel<4, 8, Moves>), grid, dim3(256), 0, s, a);
+    // places of the runs: the first block may start up to 63 before slot 0.
+    // Registers for fewer of them save what the unrolled passes skip: 1025 slots
+    // 8.0 us with 2 a lane, 8.4 with 4; 4032 slots 15.2 with 4, 17.3 with 16.
+    const int places = a.max_len + 63;
+    if (places <= 2 * kThreads)
+        hipLaunchKernelGGL((kv_choose_kernel<2, Moves>), grid, dim3(kThreads), 0, s, a);
+    else if (places <= 4 * kThreads)
+        hipLaunchKernelGGL((kv_choose_kernel<4, Moves>), grid, dim3(kThreads), 0, s, a);
     else
-        hipLaunchKernelGGL((kv_choose_kernel<16, 16, Moves>), grid, dim3(1024), 0, s, a);
+        hipLaunchKernelGGL((kv_choose_kernel<16, Moves>), grid, dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
@@ -342,7 +398,7 @@ int ouro_kv_evict(const ouro_kv_cache *cache, const ouro_kv_history *history, co
     a.max_len = static_cast<int>(max_len), a.keep = static_cast<int>(keep), a.recent = static_cast<int>(recent);
     a.most = static_cast<int>(most), a.vecs = a.c.d * a.c.elem / 16;
     hipStream_t s = as_stream(stream);
-    if (most <= kFew) {
+    if (most * (heads > 1 ? 1 : a.c.n_head_kv) * a.vecs * 32 <= kFew) {
         choose<true>(a, static_cast<unsigned>(seqs), s);
         return check_launch("kv_choose_kernel");
     }
