@@ -18,6 +18,8 @@ constexpr int kThreads = 256;
 constexpr int kLogits = 32;                 // logits of a thread
 constexpr int kPartLogits = kThreads * kLogits;
 constexpr int kSegs = kThreads / 16;        // segments of a part: 16 lanes each
+constexpr int kJoin = 1024;                 // threads that join a row's parts
+constexpr int kGroups = 256;                // groups of its segments
 constexpr int kCap = 2048;                  // candidates that the choice of alternatives holds
 
 struct ScoreArgs {
@@ -124,6 +126,13 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, int64_t row, int g, f
 // maximum, then the sums against it, then the tokens ahead of the given one
 // and (Top) the largest key of each segment, that is of the vectors of 16
 // lanes.  A row of one part is finished here.
+//
+// Bound by memory once the rows fill the chip: 512 rows of 248320 fp32 logits
+// in 90 us (5.6 TB/s), 64 in 16 (4.0), 1009 rows of 32003 bf16 in 19 (3.4).  A
+// part of 8192 logits leaves each thread its 32 in registers, so that the
+// maximum is known before the first exponential and nothing is read twice; 16
+// bits hold twice as many in as many registers, but unpacked they take 183 and
+// the launch of bf16 rows 40 us.
 template <typename T, bool Top>
 __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
     constexpr int VL = Row<T>::VL, kVec = Row<T>::kVec, kPart = Row<T>::kPart;
@@ -230,41 +239,49 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
 
 // One workgroup a row: the parts' sums joined, and the k alternatives chosen.
 //
-// A lower bound of the k-th largest key: the k-th largest of 64 groups' largest
-// (a group has every 64th segment).  Few segments reach it, and only their
+// A lower bound of the k-th largest key: the k-th largest of the groups' largest
+// (a group has every 256th segment).  Few segments reach it, and only their
 // logits are read again: those at or above the bound become candidates.  Where
 // ties or a skewed row make them more than kCap, the bound is raised by
 // bisection (keys are unique, so some bound leaves k to kCap of them).  The
 // candidates' places are their ranks among each other.
+//
+// Bound by latency, a chain of loads and barriers: 6.5 us for one row of 248320
+// (31 parts) with 20 alternatives, 10 for 512 rows with 8.  1024 threads because
+// the reread segments are loads in flight: 10.8 us with 256; 256 groups because
+// with 64 and k = 64 the least of the groups' largest is the bound, which
+// hundreds of segments reach: the whole call 32 us against 17.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(kJoin) void logprobs_join_kernel(ScoreArgs a) {
     __shared__ unsigned long long cand[kCap];
     __shared__ int32_t list[kCap];
     __shared__ unsigned long long bound;
     __shared__ float m_all, ln_all;
-    __shared__ int n_cand, n_list;
+    __shared__ int n_cand, n_list, ahead_of[kGroups];
     constexpr int VL = Row<T>::VL, kVec = Row<T>::kVec, kPart = Row<T>::kPart;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
     const Row<T> x(a, row);
     const int ns = a.parts * kSegs;
     const unsigned long long *seg = a.seg + row * ns;
-    // the groups' largest keys: thread t takes segments t, t + 256, ..: group t % 64
+    // the groups' largest keys: thread t takes segments t, t + kJoin, ..: group t % 64
     unsigned long long first = 0;  // the thread's first segment's key
+    const int g = a.target ? a.target[row] : -1;
+    float4 part = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    if (wave == 1 && lane < a.parts) part = a.part[row * a.parts + lane];
     if (a.k) {
         first = tid < ns ? seg[tid] : 0ull;
         unsigned long long best = first;
-        for (int i = tid + kThreads; i < ns; i += kThreads) best = argmax_key_max(best, seg[i]);
+        for (int i = tid + kJoin; i < ns; i += kJoin) best = argmax_key_max(best, seg[i]);
         cand[tid] = best;
-        __syncthreads();
     }
+    const float xt = g >= 0 && g < a.n ? logit(x.x, g) : 0.f;
+    if (a.k) __syncthreads();
     if (wave == 1) {
         // the sums, a part a lane
-        const int g = a.target ? a.target[row] : -1;
-        const float xt = g >= 0 && g < a.n ? logit(x.x, g) : 0.f;
-        float m = -INFINITY, l = 0.f, s = 0.f;
-        int ahead = 0;
-        for (int p = lane; p < a.parts; p += 64) {
+        float m = part.x, l = part.y, s = part.z;
+        int ahead = __float_as_int(part.w);
+        for (int p = lane + 64; p < a.parts; p += 64) {
             const float4 o = a.part[row * a.parts + p];
             if (o.x != -INFINITY) merge(m, l, s, o.x, o.y, o.z);
             ahead += __float_as_int(o.w);
@@ -286,19 +303,31 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
         }
     }
     if (!a.k) return;
-    if (wave == 0) {
-        const unsigned long long mine = argmax_key_max(argmax_key_max(cand[lane], cand[lane + 64]), argmax_key_max(cand[lane + 128], cand[lane + 192]));
-        int before = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) {
-            const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine >> 32), i);
-            const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine), i);
-            before += (static_cast<unsigned long long>(hi) << 32 | lo) > mine;
-        }
-        if (lane == 0) bound = 1;  // every logit above -inf, where fewer than k groups have one
-        if (mine && before == a.k - 1) bound = mine;  // keys are unique
-        if (lane == 0) n_list = n_cand = 0;
+    // group g: the keys that threads g, g + kGroups, .. hold
+    if (tid < kGroups) {
+        unsigned long long best = cand[tid];
+#pragma unroll
+        for (int i = kGroups; i < kJoin; i += kGroups) best = argmax_key_max(best, cand[tid + i]);
+        cand[kJoin + tid] = best;
+        ahead_of[tid] = 0;
     }
+    if (tid == 0) {
+        bound = 1;  // every logit above -inf, where fewer than k groups have one
+        n_list = n_cand = 0;
+    }
+    __syncthreads();
+    const unsigned long long *group = cand + kJoin, mine = group[tid % kGroups];
+    {
+        // its rank among a quarter of the groups
+        constexpr int kShare = kGroups * kGroups / kJoin;
+        const int from = tid / kGroups * kShare;
+        int before = 0;
+#pragma unroll 16
+        for (int i = 0; i < kShare; ++i) before += group[from + i] > mine;
+        atomicAdd(&ahead_of[tid % kGroups], before);
+    }
+    __syncthreads();
+    if (tid < kGroups && mine && ahead_of[tid] == a.k - 1) bound = mine;  // keys are unique
     __syncthreads();
     const unsigned long long least = bound;
     unsigned long long lo = least, hi = ~0ull, cur = least;
@@ -306,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
     int c;
     for (;;) {
         // the segments that reach the bound, then their logits that do
-        for (int i = tid; i < ns; i += kThreads)
+        for (int i = tid; i < ns; i += kJoin)
             if ((i == tid ? first : seg[i]) >= cur) {
                 const int at = atomicAdd(&n_list, 1);
                 if (at < kCap) list[at] = i;
@@ -314,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
         __syncthreads();
         const int nl = n_list;
         if (nl <= kCap) {
-            for (int u = tid; u < nl * 16 * kVec; u += kThreads) {
+            for (int u = tid; u < nl * 16 * kVec; u += kJoin) {
                 const int i = list[u / (16 * kVec)], w = u % (16 * kVec);
                 const int q = i / kSegs * kPart + i % kSegs * 16 + (w >> 4) * kThreads + (w & 15);
                 if (x.first(q) >= a.n) continue;
@@ -348,11 +377,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(ScoreArgs a) {
         __syncthreads();
     }
     const float mm = m_all, ln = ln_all;
-    for (int i = c + tid; i < a.k; i += kThreads) {
+    for (int i = c + tid; i < a.k; i += kJoin) {
         a.top_id[row * a.k + i] = -1;
         a.top_logprob[row * a.k + i] = -INFINITY;
     }
-    for (int i = tid; i < c; i += kThreads) {
+    for (int i = tid; i < c; i += kJoin) {
         const unsigned long long mine = cand[i];
         int before = 0;
         for (int j = 0; j < c; ++j) before += cand[j] > mine;
@@ -382,7 +411,7 @@ int launch(const ScoreArgs &a, unsigned rows, hipStream_t s) {
         int st = check_launch("logprobs_part_kernel");
         if (st) return st;
         if (a.k || a.parts > 1) {
-            hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3(m), dim3(kThreads), 0, s, b);
+            hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3(m), dim3(a.k ? kJoin : 128), 0, s, b);
             if ((st = check_launch("logprobs_join_kernel"))) return st;
         }
     }
