@@ -484,7 +484,8 @@ int ouro_finite_argmax(const float *y, size_t n, int32_t *idx, void *stream);
  * id outside 0 .. n_pages - 1 is a hole: its slots hold nothing, are never
  * read or written and count as masked.  k, v and the strides in bytes are
  * multiples of 16 (OURO_ERR_ALIGN), head_dim a multiple of 8, 8 .. 256, and
- * page_tokens a power of two (OURO_ERR_SHAPE). */
+ * page_tokens a power of two up to 2^20, tokens up to 2^24 elements apart
+ * (OURO_ERR_SHAPE). */
 typedef struct ouro_kv_cache {
     void *k, *v;
     const int32_t *pages;                            /* [seqs][max_pages] */

@@ -371,7 +371,7 @@ def expected(t, w, pos, keep, recent):
 
 
 def check_evict(seed, lens, hkv, d, page, keep, recent, *, heads=None, cache=True, layout="token", weights="spread",
-                shuffled=False, apart=False, max_len=None, holes=(), extra=0, stream=None, workspace=False):
+                shuffled=False, apart=False, max_len=None, holes=(), extra=0, stream=None, workspace=False, positions=None):
     t = Setup(seed, lens, hkv, d, page, cache, layout, max_len, holes, extra * 8)
     rng, B, H = t.rng, len(lens), hkv if heads is None else heads
     slots = t.max_len + 2
@@ -385,6 +385,8 @@ def check_evict(seed, lens, hkv, d, page, keep, recent, *, heads=None, cache=Tru
     pos = np.broadcast_to(np.arange(slots, dtype=np.int32), w.shape).copy()
     if shuffled:
         pos = rng.permuted(pos * 3 - 50, axis=2)
+    if positions is not None:
+        pos = rng.choice(positions, pos.shape)
     src, w1, p1, k, v = expected(t, w, pos, keep, recent)
     c = t.open()
     hist = History(DeviceBuffer.from_host(w), DeviceBuffer.from_host(pos), H, slots)
@@ -445,6 +447,19 @@ def test_evict_holes(gpu):
 def test_evict_long(gpu, n):
     check_evict(7, (n, n - 1), 1, 8, 64, n // 5, n // 50, shuffled=True)
     check_evict(8, (n,), 1, 8, 64, n - 1, 100, weights="ties")
+
+
+@pytest.mark.parametrize("heads", [None, 1])
+@pytest.mark.parametrize("n,keep,d,cache", [(2000, 900, 80, True), (700, 340, 256, True), (700, 340, 256, False), (1100, 500, 96, False)])
+def test_evict_many_moves(gpu, heads, n, keep, d, cache):
+    check_evict(n, (n, n // 2, n - 1), 2, d, 32, keep, 30, heads=heads, cache=cache, shuffled=True, apart=d == 256, holes=[(0, 1, -1), (2, n // 32, 1 << 30)])
+
+
+@pytest.mark.parametrize("recent", [0, 1, 3, 20, 1 << 30])
+def test_evict_positions(gpu, recent):
+    """Positions from one end of their type to the other."""
+    check_evict(9, (40, 7, 1000), 2, 16, 16, 24, recent, positions=np.array([-2 ** 31, -2 ** 31 + 1, -1, 0, 1, 2 ** 31 - 2, 2 ** 31 - 1], np.int32))
+    check_evict(9, (40, 100), 2, 16, 16, 24, recent, positions=np.array([-2 ** 31, -2 ** 31 + 1], np.int32), apart=True)
 
 
 def test_evict_streams(gpu):
@@ -524,7 +539,8 @@ def test_attend_refusals(gpu, code, more):
 @pytest.mark.parametrize("code,field,x", [
     (ARG, "k", None), (ARG, "v", None), (ARG, "pages", None), (ARG, "dtype", 2), (SHAPE, "n_pages", 0), (SHAPE, "max_pages", 0),
     (SHAPE, "n_head_kv", 0), (SHAPE, "head_dim", 0), (SHAPE, "head_dim", 12), (SHAPE, "head_dim", 264), (SHAPE, "page_tokens", 0),
-    (SHAPE, "page_tokens", 48), (SHAPE, "page_stride", -8), (ALIGN, "token_stride", 130), (ALIGN, "head_stride", 4), (ALIGN, "k", "odd"),
+    (SHAPE, "page_tokens", 48), (SHAPE, "page_stride", -8), (ALIGN, "token_stride", 130), (SHAPE, "token_stride", (1 << 24) + 8),
+    (ALIGN, "head_stride", 4), (ALIGN, "k", "odd"),
 ])
 def test_cache_refusals(gpu, code, field, x):
     t, c, b = small()
