@@ -78,7 +78,7 @@ struct AttendArgs {
     int64_t q_stride, new_stride, mask_stride, out_stride, s_stride;
     int32_t n_head, max_len, h_heads, h_slots, n_split, q_tiles;
     float scale;
-    int32_t pad;
+    int32_t w_slots;  // slots of a workgroup that adds weights: 512 or 256
 };
 // passed by value to kernels: the host and device passes must lay it out alike
 static_assert(sizeof(AttendArgs) == 256, "AttendArgs: kernel argument layout");
@@ -197,21 +197,32 @@ __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h,
 }
 
 // One workgroup a split of kSplit slots, (kv head, tile of 16 query heads) and
-// sequence, its four wavefronts on alternate tiles of slots (32 of bf16, 16 of
-// fp32), each with its own running maximum, sum and output.
+// sequence, its four wavefronts on alternate tiles of 16 slots, each with its
+// own running maximum, sum and output.
 //
 // Both products run on the matrix cores with the slots as rows of the first
 // and as the inner axis of the second, the query heads as columns:
 //   S^T[slot][head] = K Q^T, O^T[dim][head] += V^T P^T.
 // A lane of S^T holds one head (lane % 16) and slots 4 (lane / 16) + 0 .. 3 of
-// each 16, and that is the order in which V's rows are loaded, so the scores
-// become the second product's operand without leaving their registers.  A
-// bf16 row of V is loaded with eight (DP = 64: four) adjacent dims a lane, 16
-// lanes a row, and pairs of rows are merged by byte permutes into operands of
-// one dim and eight slots; fp32 operands hold one slot and need none.
+// the tile, and that is the order in which V's rows are loaded, so the scores
+// become the second product's operand without leaving their registers.  K's
+// rows are read whole, 16 bytes a lane, and turned into operands through LDS.
+// A bf16 row of V is loaded with eight (DP = 64: four) adjacent dims a lane,
+// and pairs of rows are merged by byte permutes into operands of one dim and
+// four slots; fp32 operands hold one slot and need none.
 // fp32 queries and weights against a bf16 cache are split into three bf16
 // operands (exact), weights for a bf16 output into two (2^-17); everything
 // else is fp32.
+//
+// Bound by memory where the splits fill the chip: 64 sequences of 16384 keys
+// (4 kv heads of 128, bf16) at 5.7 TB/s, 512 of up to 1025 at 5.1, 64 of up to
+// 2176 in fp32 in 52 us (5.2).  Below that by what a workgroup does before its
+// first products and after its last (pages, queries, the four outputs joined):
+// 64 sequences of up to 1025 keys take 26.5 us, 21 without reading K or V, one
+// sequence of 16384 10.5, one of 300 7.5.  Splits of 256 slots because one
+// sequence must fill the chip; several splits a workgroup were no faster.  The
+// loads of the next tile stand before a tile's products and need no count of
+// what is in flight: there is always a tile's worth.
 template <typename C, typename IO, int DP, bool Paged, bool Once>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) == 2 ? (DP <= 64 ? 5 : DP <= 128 ? 4 : 2) : (DP <= 64 ? 5 : DP <= 128 ? 3 : 2)))) void kv_attend_split_kernel(AttendArgs a) {
     constexpr bool kHalf = sizeof(C) == 2;
@@ -553,7 +564,7 @@ __device__ __forceinline__ float2 join_ml(const float2 *ml, int ns) {
 }
 
 // The splits of (head, sequence) joined: a thread takes four dims of every
-// (1024 / DP)-th split.
+// (1024 / DP)-th split.  Latency: 2.5 to 4 us a launch for 2 to 64 splits.
 template <typename IO, int DP>
 __device__ __forceinline__ void join_splits(const AttendArgs &a, int64_t b, int h, int ns, f32x4_t *red) {
     const int tid = threadIdx.x, d = a.c.d;
@@ -592,12 +603,12 @@ __device__ __forceinline__ void join_splits(const AttendArgs &a, int64_t b, int 
 
 // Each slot's attention weight, summed over the query heads of its history
 // head, onto the history: by the scores that the splits left and the heads'
-// joined maxima and sums.  kWSlots slots a workgroup.
-constexpr int kWSlots = 512, kWHeads = 64;
+// joined maxima and sums.  NW slots a thread.
+constexpr int kWHeads = 64;
+template <int NW>
 __device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int hs, int j0, int n, float2 *ml) {
     const int tid = threadIdx.x;
     const int ns = (n + kSplit - 1) / kSplit, G = a.n_head / a.h_heads;
-    constexpr int NW = kWSlots / 256;
     float *const out = a.weight + (b * a.h_heads + hs) * a.h_slots;
     float w[NW], sum[NW];
 #pragma unroll
@@ -614,8 +625,9 @@ __device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int 
         float first[kAhead][NW];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
+            if (k < ng)
 #pragma unroll
-            for (int i = 0; i < NW; ++i) first[k][i] = a.score[(h0 + min(k, ng - 1)) * a.s_stride + min(j0 + 256 * i + tid, n - 1)];
+                for (int i = 0; i < NW; ++i) first[k][i] = a.score[(h0 + k) * a.s_stride + min(j0 + 256 * i + tid, n - 1)];
         __syncthreads();
         for (int i = tid >> 4; i < ng; i += 16) {
             const float2 t = join_ml<16>(a.ml + (h0 + i) * a.n_split, ns);
@@ -642,8 +654,11 @@ __device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int 
 }
 
 // What the splits left brought together: workgroups 0 .. joins - 1 of a
-// sequence take a head's output each, the others kWSlots slots of a history
-// head.
+// sequence take a head's output each, the others w_slots slots of a history
+// head: 512, so that few workgroups repeat the heads' maxima, or 256 where a
+// slot's weight takes the scores of many heads (24 sequences of up to 8191
+// slots: 32 heads 27.0 us with 512 and 25.5 with 256, 64 of up to 1025 with 4
+// heads 32.5 and 33.1).
 template <typename IO, int DP>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, int joins) {
     __shared__ f32x4_t red[256];
@@ -652,8 +667,12 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, int j
     if (x < joins) {
         if (n > kSplit) join_splits<IO, DP>(a, b, x, (n + kSplit - 1) / kSplit, red);  // else its only split wrote it
     } else {
-        const int hs = (x - joins) % a.h_heads, j0 = (x - joins) / a.h_heads * kWSlots;
-        if (j0 < n) add_weights(a, b, hs, j0, n, reinterpret_cast<float2 *>(red));
+        const int hs = (x - joins) % a.h_heads, j0 = (x - joins) / a.h_heads * a.w_slots;
+        if (j0 >= n) return;
+        if (a.w_slots == 256)
+            add_weights<1>(a, b, hs, j0, n, reinterpret_cast<float2 *>(red));
+        else
+            add_weights<2>(a, b, hs, j0, n, reinterpret_cast<float2 *>(red));
     }
 }
 
@@ -682,7 +701,7 @@ int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
     int st = check_launch("kv_attend_split_kernel");
     if (st) return st;
     const int joins = a.n_split > 1 ? a.n_head : 0;
-    const int64_t weights = a.weight ? static_cast<int64_t>((a.max_len + kWSlots - 1) / kWSlots) * a.h_heads : 0;
+    const int64_t weights = a.weight ? static_cast<int64_t>((a.max_len + a.w_slots - 1) / a.w_slots) * a.h_heads : 0;
     if (joins + weights > 0) {
         hipLaunchKernelGGL((kv_attend_join_kernel<IO, DP>), dim3(static_cast<unsigned>(joins + weights), seqs), dim3(256), 0, s, a, joins);
         st = check_launch("kv_attend_join_kernel");
@@ -762,6 +781,7 @@ int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history, c
         a.pos = history->pos;
         a.h_heads = history->heads;
         a.h_slots = history->slots;
+        a.w_slots = n_head / history->heads > 8 ? 256 : 512;
     }
     if (!seqs) return OURO_OK;
     if (!max_len) a.weight = nullptr;  // no slots to weigh
