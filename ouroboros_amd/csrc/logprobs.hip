@@ -17,6 +17,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kLogits = 32;                 // logits of a thread
 constexpr int kPartLogits = kThreads * kLogits;
+constexpr int kRowParts = 4;                // parts of a row that one workgroup takes whole, where rows are few
+constexpr unsigned kFewRows = 512;          // such workgroups that the chip holds at once
 constexpr int kSegs = kThreads / 16;        // segments of a part: 16 lanes each
 constexpr int kJoin = 1024;                 // threads that join a row's parts
 constexpr int kGroups = 256;                // groups of its segments
@@ -122,6 +124,21 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, int64_t row, int g, f
     if (a.rank) a.rank[row] = given ? ahead : -1;
 }
 
+// The sums of a wavefront's lanes joined, to each of them; their maximum.
+__device__ __forceinline__ float join_lanes(float m, float &l, float &s, int &ahead) {
+    float M = m;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, xor_shfl(M, off));
+    if (M != -INFINITY) merge(m, l, s, M, 0.f, 0.f);  // against the largest
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        l += xor_shfl(l, off);
+        s += xor_shfl(s, off);
+        ahead += xor_shfl(ahead, off);
+    }
+    return M;
+}
+
 // One workgroup a part of a row, its logits in registers: the wavefront's
 // maximum, then the sums against it, then the tokens ahead of the given one
 // and (Top) the largest key of each segment, that is of the vectors of 16
@@ -133,14 +150,14 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, int64_t row, int g, f
 // maximum is known before the first exponential and nothing is read twice; 16
 // bits hold twice as many in as many registers, but unpacked they take 183 and
 // the launch of bf16 rows 40 us.
-template <typename T, bool Top>
-__global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
+template <typename T, bool Top, int Parts>
+__global__ __launch_bounds__(Parts * kThreads) void logprobs_part_kernel(ScoreArgs a) {
     constexpr int VL = Row<T>::VL, kVec = Row<T>::kVec, kPart = Row<T>::kPart;
-    __shared__ float4 waves[kThreads / 64];
-    const int tid = threadIdx.x;
+    __shared__ float4 waves[Parts * kThreads / 64];
+    const int tid = threadIdx.x % kThreads;
     const int64_t row = blockIdx.y;
     const Row<T> x(a, row);
-    const int q0 = static_cast<int>(blockIdx.x) * kPart;
+    const int q0 = (static_cast<int>(blockIdx.x) * Parts + __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads)) * kPart;
     u32x4_t v[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
@@ -222,14 +239,26 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(ScoreArgs a) {
         l += xor_shfl(l, off);
         s += xor_shfl(s, off);
     }
-    if ((tid & 63) == 0) waves[tid >> 6] = make_float4(m, l, s, __int_as_float(ahead));
+    if ((tid & 63) == 0) waves[threadIdx.x >> 6] = make_float4(m, l, s, __int_as_float(ahead));
     __syncthreads();
-    if (tid) return;
+    // a part's wavefronts in order, by one lane
+    if (threadIdx.x >= (Parts > 1 ? 64 : 1)) return;
+    if (Parts == 1 || threadIdx.x < Parts) {
+        const int w0 = threadIdx.x * (kThreads / 64);
+        m = waves[w0].x, l = waves[w0].y, s = waves[w0].z, ahead = __float_as_int(waves[w0].w);
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) {
-        const float4 o = waves[w];
-        if (o.x != -INFINITY) merge(m, l, s, o.x, o.y, o.z);
-        ahead += __float_as_int(o.w);
+        for (int w = 1; w < kThreads / 64; ++w) {
+            const float4 o = waves[w0 + w];
+            if (o.x != -INFINITY) merge(m, l, s, o.x, o.y, o.z);
+            ahead += __float_as_int(o.w);
+        }
+    } else {
+        m = -INFINITY, l = s = 0.f, ahead = 0;
+    }
+    if constexpr (Parts > 1) {  // the lanes' sums as the other launch joins them
+        const float M = join_lanes(m, l, s, ahead);
+        if (threadIdx.x == 0) finish(a, row, g, xt, M, l, s, ahead);
+        return;
     }
     if (a.parts == 1 && !a.k)
         finish(a, row, g, xt, m, l, s, ahead);
@@ -286,16 +315,7 @@ __global__ __launch_bounds__(kJoin) void logprobs_join_kernel(ScoreArgs a) {
             if (o.x != -INFINITY) merge(m, l, s, o.x, o.y, o.z);
             ahead += __float_as_int(o.w);
         }
-        float M = m;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, xor_shfl(M, off));
-        if (M != -INFINITY) merge(m, l, s, M, 0.f, 0.f);  // against the row's maximum
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
-            l += xor_shfl(l, off);
-            s += xor_shfl(s, off);
-            ahead += xor_shfl(ahead, off);
-        }
+        const float M = join_lanes(m, l, s, ahead);
         if (lane == 0) {
             finish(a, row, g, xt, M, l, s, ahead);
             m_all = M;
@@ -396,6 +416,10 @@ __global__ __launch_bounds__(kJoin) void logprobs_join_kernel(ScoreArgs a) {
 
 template <typename T>
 int launch(const ScoreArgs &a, unsigned rows, hipStream_t s) {
+    // Few rows of few parts take one launch, of the same sums in the same order.
+    // (32003 bf16 logits: 1 row 5.5 us, 7.9 with two; 256 rows 8.9 and 11.7; 512
+    // 15.2 and 16.4; 1009 rows 25.8 and 22.8, the launch then runs in two rounds)
+    const bool whole = !a.k && a.parts > 1 && a.parts <= kRowParts && rows <= kFewRows;
     for (unsigned r = 0; r < rows; r += 65535) {  // grid y
         ScoreArgs b = a;
         const unsigned m = rows - r < 65535 ? rows - r : 65535;
@@ -405,12 +429,14 @@ int launch(const ScoreArgs &a, unsigned rows, hipStream_t s) {
         b.logprob = move(a.logprob), b.rank = move(a.rank), b.entropy = move(a.entropy), b.lse = move(a.lse);
         if (a.k) b.top_id = a.top_id + static_cast<size_t>(r) * a.k, b.top_logprob = a.top_logprob + static_cast<size_t>(r) * a.k;
         if (a.k)
-            hipLaunchKernelGGL((logprobs_part_kernel<T, true>), dim3(a.parts, m), dim3(kThreads), 0, s, b);
+            hipLaunchKernelGGL((logprobs_part_kernel<T, true, 1>), dim3(a.parts, m), dim3(kThreads), 0, s, b);
+        else if (whole)
+            hipLaunchKernelGGL((logprobs_part_kernel<T, false, kRowParts>), dim3(1, m), dim3(kRowParts * kThreads), 0, s, b);
         else
-            hipLaunchKernelGGL((logprobs_part_kernel<T, false>), dim3(a.parts, m), dim3(kThreads), 0, s, b);
+            hipLaunchKernelGGL((logprobs_part_kernel<T, false, 1>), dim3(a.parts, m), dim3(kThreads), 0, s, b);
         int st = check_launch("logprobs_part_kernel");
         if (st) return st;
-        if (a.k || a.parts > 1) {
+        if (a.k || (a.parts > 1 && !whole)) {
             hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3(m), dim3(a.k ? kJoin : 128), 0, s, b);
             if ((st = check_launch("logprobs_join_kernel"))) return st;
         }

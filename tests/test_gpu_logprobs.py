@@ -200,3 +200,33 @@ def test_refusals(gpu, code, more):
 
 def test_no_rows(gpu):
     ops.token_logprobs(DeviceBuffer((1,), np.float32), 0, 100)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [8178, 8186, 8191, 8193, 16390, 24577, 32754, 32762, 32767, 32769])
+def test_rows_of_few_parts(gpu, n, bf16):
+    """Without alternatives, around the lengths at which a row takes one, two .. five parts."""
+    rng = np.random.default_rng(n)
+    x = logits(n, 6, n)
+    x[0, rng.random(n) < 0.9] = -np.inf
+    x[1] = -np.inf
+    x[2, n - 1] = np.inf
+    x[3, rng.random(n) < 0.5] = np.nan
+    x[4] = np.finfo(np.float32).min
+    t = [n // 3, 0, n - 1, n - 2, 5, n // 2]
+    check(x, t, 0, bf16=bf16)
+    check(x, t, 0, bf16=bf16, offset=3, stride=n + 2)
+    check(x[5:], [n - 1], 0, bf16=bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [9000, 32000])
+def test_few_rows_and_many(gpu, n, bf16):
+    """A row's bits are those of a call of few rows, of many and with alternatives."""
+    x = logits(n, 8, n)
+    raw = f32_to_bf16_bits(x) if bf16 else x
+    t = np.arange(8) * 11
+    got = [ops.token_logprobs(np.tile(raw, (m, 1)), 8 * m, n, targets=np.tile(t, m).astype(np.int32), k=k) for m, k in ((1, 0), (64, 0), (65, 0), (1, 3))]
+    for other in got[1:]:
+        for name in ("logprob", "rank", "entropy", "lse"):
+            assert np.array_equal(other[name][-8:], got[0][name]), name
