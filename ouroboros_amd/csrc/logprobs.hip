@@ -145,7 +145,8 @@ __device__ __forceinline__ float join_lanes(float m, float &l, float &s, int &ah
 // lanes.  A row of one part is finished here.
 //
 // Bound by memory once the rows fill the chip: 512 rows of 248320 fp32 logits
-// in 90 us (5.6 TB/s), 64 in 16 (4.0), 1009 rows of 32003 bf16 in 19 (3.4).  A
+// in 90 us (5.6 TB/s), 64 in 16 (4.0), 1009 rows of 32003 bf16 in 19 (3.4; of
+// that 9 are the vector instructions, 12 a logit with its exponential).  A
 // part of 8192 logits leaves each thread its 32 in registers, so that the
 // maximum is known before the first exponential and nothing is read twice; 16
 // bits hold twice as many in as many registers, but unpacked they take 183 and
@@ -157,7 +158,8 @@ __global__ __launch_bounds__(Parts * kThreads) void logprobs_part_kernel(ScoreAr
     const int tid = threadIdx.x % kThreads;
     const int64_t row = blockIdx.y;
     const Row<T> x(a, row);
-    const int q0 = (static_cast<int>(blockIdx.x) * Parts + __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads)) * kPart;
+    const int group = Parts == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+    const int q0 = (static_cast<int>(blockIdx.x) * Parts + group) * kPart;
     u32x4_t v[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
