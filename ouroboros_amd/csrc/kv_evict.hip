@@ -61,8 +61,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs &a, int64_t b, int h, 
         const int64_t dst = kv_slot(a.c, b, m.x) * a.c.elem, src = kv_slot(a.c, b, m.y) * a.c.elem;
         if (src < 0 || dst < 0) continue;  // a hole
         const u32x4_t x = *reinterpret_cast<const u32x4_t *>(k + src), y = *reinterpret_cast<const u32x4_t *>(v + src);
-        *reinterpret_cast<u32x4_t *>(k + dst) = x;
-        *reinterpret_cast<u32x4_t *>(v + dst) = y;
+        // not kept by the caches, which whoever reads the row next is not behind
+        // (100 MB moved: 27.5 us, 33.1 with plain stores, 30.9 with loads past them too)
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t *>(k + dst));
+        __builtin_nontemporal_store(y, reinterpret_cast<u32x4_t *>(v + dst));
     }
 }
 
@@ -315,8 +317,8 @@ __global__ __launch_bounds__(kThreads) void kv_choose_kernel(EvictArgs a) {
 constexpr int kMoveThreads = 256;
 
 // One workgroup a (kv head, sequence) and share of its moves: bound by memory,
-// 100 MB read and written in 24 us (4.2 TB/s; a large copy reaches 4.9).  Four
-// rows in flight a lane instead of one took as long.
+// 100 MB read and written in 19 us, about a large copy's rate.  Four rows in
+// flight a lane instead of one took as long.
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(EvictArgs a) {
     const int lanes = a.vecs <= 16 ? 16 : a.vecs <= 32 ? 32 : 64;
     const int h = blockIdx.y, t = threadIdx.x;
@@ -326,8 +328,9 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(EvictArgs a) {
 }
 
 // Bytes of moved rows up to which the choosing workgroup moves them itself.  64
-// sequences and 4 heads: 256 moves of 512 bytes (128 KiB) 18.1 us by it, 21.6 by
-// a second launch, one move 7.8 and 11.1; 48 and 4, up to 512 moves: 38.7 and 32.9.
+// sequences and 4 heads: 256 moves of 512 bytes (128 KiB) 16.6 us by it, 19.9 by
+// a second launch, one move 7.9 and 11.3; with one sequence 9.7 and 10.6.  512
+// moves of 1 KiB take 19.0 by it and 11.8 with 4 sequences, 29.0 and 27.4 with 48.
 constexpr size_t kFew = 128 << 10;
 
 // Moves of a (sequence, head) at the most.
