@@ -122,7 +122,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 // x as a sum of N bf16 operands, each the rounding of what the ones before
 // leave (the differences are exact): 8 bits of the significand apiece, so three
-// hold a float whole and two hold it to 2^-17.
+// hold a float whole.
 template <int N, int M>
 __device__ __forceinline__ void split(const float (&x)[M], uint32_t (&w)[N][M / 2]) {
     float r[M];
@@ -210,9 +210,9 @@ __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h,
 // A bf16 row of V is loaded with eight (DP = 64: four) adjacent dims a lane,
 // and pairs of rows are merged by byte permutes into operands of one dim and
 // four slots; fp32 operands hold one slot and need none.
-// fp32 queries and weights against a bf16 cache are split into three bf16
-// operands (exact), weights for a bf16 output into two (2^-17); everything
-// else is fp32.
+// fp32 queries and the weights against a bf16 cache are split into three bf16
+// operands (exact), so that a bf16 output is rounded once, when it is stored;
+// everything else is fp32.
 //
 // Bound by memory where the splits fill the chip: 64 sequences of 16384 keys
 // (4 kv heads of 128, bf16) at 5.7 TB/s, 512 of up to 1025 at 5.1, 64 of up to
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
     constexpr int KC = kHalf ? 8 : 4;                     // dims of a lane's 16 bytes of K
     constexpr int NJ = DP / (4 * KC);                     // steps over the dims
     constexpr int NQ = kHalf && sizeof(IO) == 4 ? 3 : 1;  // operands of a query
-    constexpr int NP = sizeof(IO) == 4 ? 3 : 2;           // and of a weight (bf16 cache)
+    constexpr int NP = 3;                                 // and of a weight (bf16 cache)
     constexpr int CH = kHalf && DP > 64 ? 8 : 4;          // adjacent dims of V a lane
     constexpr int NB = DP / (16 * CH);
     constexpr int NR = TS / 4;                            // slots of a lane
