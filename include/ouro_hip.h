@@ -507,9 +507,11 @@ typedef struct ouro_kv_history {
  * per head on the host, qwen35.rs:1187-1210): for query head h of sequence b,
  * over its visible slots j < lens[b] (the page there, its mask byte not 0),
  *   s_j = scale q.k_j, out = softmax(s) v [* sigmoid(gate)], lse = ln sum e^s,
- * with kv head h / (n_head / n_head_kv).  Where no slot is visible out = 0
- * and lse = -inf.  What lies in slots that are not visible (NaN, infinities)
- * changes nothing.  The rows of a sequence do not depend on the batch it is
+ * with kv head h / (n_head / n_head_kv).  Where no slot is visible, or every
+ * visible one scores -inf, out = 0 and lse = -inf; a NaN among a head's visible
+ * scores makes its out, its lse and what it adds to the history of the slots
+ * that score above -inf NaN.  What lies in slots that are not visible (NaN,
+ * infinities) changes nothing, and their weights stay.  The rows of a sequence do not depend on the batch it is
  * in, and the same call gives the same bits.
  *   q, out [seqs][n_head][head_dim] of `dtype`, rows q_stride and out_stride
  *     elements apart; gate (or NULL) as q, q_stride apart too;

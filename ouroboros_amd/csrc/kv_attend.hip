@@ -6,6 +6,9 @@
 //   s_j = scale q.k_j,  m = max s_j,  l = sum e^(s_j - m),
 //   o = (1 / l) sum e^(s_j - m) v_j  [* sigmoid(gate)],  lse = m + ln l,
 // and o = 0, lse = -inf where no slot is visible.
+//
+// A running maximum passes over a NaN score, whose p = e^(s - m) makes the sum
+// NaN: the sum alone says whether anything was there (0: no score above -inf).
 #include "kv_cache.hpp"
 
 #include <atomic>
@@ -193,7 +196,7 @@ __device__ __forceinline__ void store_out(const AttendArgs &a, int64_t b, int h,
     store1(static_cast<IO *>(a.out), b * a.out_stride + i, o);
 }
 __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h, float m, float l) {
-    if (a.lse) a.lse[b * a.n_head + h] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    if (a.lse) a.lse[b * a.n_head + h] = (m + log2f(l)) * 0.6931471805599453f;  // -inf where l = 0
 }
 
 // One workgroup a split of kSplit slots, (kv head, tile of 16 query heads) and
@@ -537,7 +540,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
             const int64_t rec = (b * a.n_head + h0 + q) * a.n_split + split_at;
             if (dim == 0 && a.ml) a.ml[rec] = make_float2(M, L);
             if (whole) {
-                store_out<IO>(a, b, h0 + q, dim, M == -INFINITY ? 0.f : x / L);
+                store_out<IO>(a, b, h0 + q, dim, L == 0.f ? 0.f : x / L);
                 if (dim == 0) store_lse(a, b, h0 + q, M, L);
             } else {
                 a.part[rec * d + dim] = x;
@@ -553,11 +556,9 @@ __device__ __forceinline__ float2 join_ml(const float2 *ml, int ns) {
     float M = -INFINITY, L = 0.f;
     for (int s = threadIdx.x % N; s < ns; s += N) {
         const float2 x = ml[s];
-        const float mn = fmaxf(M, x.x);
-        if (mn != -INFINITY || x.x != x.x) {
-            L = L * __builtin_amdgcn_exp2f(M - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
-            M = mn;
-        }
+        const float mn = fmaxf(M, x.x), ref = mn == -INFINITY ? 0.f : mn;
+        L = L * __builtin_amdgcn_exp2f(M - ref) + x.y * __builtin_amdgcn_exp2f(x.x - ref);
+        M = mn;
     }
 #pragma unroll
     for (int off = N / 2; off >= 1; off >>= 1) {
@@ -603,7 +604,7 @@ __device__ __forceinline__ void join_splits(const AttendArgs &a, int64_t b, int 
     float o = 0.f;
 #pragma unroll
     for (int s = 0; s < NG; ++s) o += red[s * DL + tid / 4][tid % 4];
-    if (tid < d) store_out<IO>(a, b, h, tid, t.x == -INFINITY ? 0.f : o / t.y);
+    if (tid < d) store_out<IO>(a, b, h, tid, t.y == 0.f ? 0.f : o / t.y);
     if (tid == 0) store_lse(a, b, h, t.x, t.y);
 }
 
@@ -637,19 +638,21 @@ __device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int 
         __syncthreads();
         for (int i = tid >> 4; i < ng; i += 16) {
             const float2 t = join_ml<16>(a.ml + (h0 + i) * a.n_split, ns);
-            // nothing visible: every score is -inf, and 2^(-inf - 0) = 0
-            if (tid % 16 == 0) ml[i] = t.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(t.x, 1.0f / t.y);
+            if (tid % 16 == 0) ml[i] = make_float2(t.x == -INFINITY ? 0.f : t.x, 1.0f / t.y);  // no -inf - -inf
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int j = j0 + 256 * i + tid;
+            // a slot that is not visible has a score of -inf, and takes nothing
+            // even of a head whose sum is NaN (or 0: nothing visible)
+            auto add = [&](float s, float2 h) { sum[i] += __builtin_amdgcn_exp2f(s - h.x) * (s == -INFINITY ? 0.f : h.y); };
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-                if (k < ng) sum[i] += __builtin_amdgcn_exp2f(first[k][i] - ml[k].x) * ml[k].y;
+                if (k < ng) add(first[k][i], ml[k]);
             if (j < n)
 #pragma unroll 8
-                for (int k = kAhead; k < ng; ++k) sum[i] += __builtin_amdgcn_exp2f(a.score[(h0 + k) * a.s_stride + j] - ml[k].x) * ml[k].y;
+                for (int k = kAhead; k < ng; ++k) add(a.score[(h0 + k) * a.s_stride + j], ml[k]);
         }
     }
 #pragma unroll

@@ -1,0 +1,122 @@
+"""Attention over a paged cache (ouro_kv_attend) with a NaN where it counts: in
+a query or in a visible key.  The head is then NaN, and so are its lse and its
+part of the history; no slot that is not visible is touched by it.
+
+What is finite is held to the bars of test_gpu_kv_cache.py."""
+import numpy as np
+import pytest
+
+from ouroboros_amd.device import DeviceBuffer
+from ouroboros_amd.kvcache import History
+
+from test_gpu_kv_cache import U, Setup, dec, enc, name
+
+pytestmark = pytest.mark.gpu
+TYPES = [(True, False), (True, True), (False, False), (False, True)]  # (bf16 cache, bf16 rows)
+HKV, G, D, PAGE = 2, 3, 72, 16
+LENS = [(40,), (700, 33)]  # one split, and several
+
+
+class Call:
+    """Rows that a test changes before check(); slot 5 is masked, slots 16 .. 31 of sequence 0 are a hole."""
+
+    def __init__(self, lens, cache, io, seed=0):
+        self.io, self.cache, self.lens = io, cache, lens
+        self.t = Setup(seed + len(lens), lens, HKV, D, PAGE, cache, holes=[(0, 1, -1)] if lens[0] > PAGE else ())
+        self.q = self.t.rng.standard_normal((len(lens), HKV * G, D)).astype(np.float32)
+        self.mask = np.ones((len(lens), self.t.max_len), np.uint8)
+        self.mask[:, 5:6] = 0
+
+    def row(self, pool, b, slot):
+        return self.t.view(pool)[self.t.table[b, slot // PAGE], slot % PAGE]
+
+    def put(self, pool, b, slot, head, dim, x):
+        self.row(pool, b, slot)[head, dim] = enc(np.full(1, x, np.float32), self.cache)[0]
+
+    def check(self, scale=None):
+        t, B, H, L = self.t, len(self.lens), HKV * G, self.t.max_len
+        c = t.open()
+        q = enc(self.q, self.io)
+        w0 = t.rng.uniform(0, 4, (B, HKV, L)).astype(np.float32)
+        wb, pb = DeviceBuffer.from_host(w0), DeviceBuffer((B, HKV, L), np.int32, zero=True)
+        out = DeviceBuffer.from_host(enc(np.full((B, H, D), 77.0), self.io))
+        lse, lens = DeviceBuffer.from_host(np.full((B, H), 77.0, np.float32)), DeviceBuffer.from_host(t.lens)
+        c.attend(DeviceBuffer.from_host(q), out, lens, B, L, H, dtype=name(self.io), lse=lse, scale=scale,
+                 mask=DeviceBuffer.from_host(self.mask), history=History(wb, pb, HKV, L))
+        got, lse, w = dec(out.download()).astype(np.float64), lse.download(), wb.download()
+        for b in range(B):
+            j, k, v = t.rows(b)
+            live = self.mask[b, j] != 0
+            j, k, v = j[live], k[live], v[live]
+            hidden = np.setdiff1d(np.arange(L), j)
+            assert np.array_equal(w[b][:, hidden], w0[b][:, hidden])
+            want_w, bar_w = w0[b][:, j].astype(np.float64), U * w0[b][:, j]
+            for h in range(H):
+                with np.errstate(all="ignore"):
+                    qv, sc = dec(q[b, h]).astype(np.float64), D ** -0.5 if scale is None else scale
+                    s = sc * (k[:, h // G] * qv).sum(1)
+                    S = np.abs(sc * (np.abs(k[:, h // G]) * np.abs(qv))).sum(1)
+                    S = S[np.isfinite(S)].max(initial=0.0)
+                    if (s == -np.inf).all():
+                        assert (got[b, h] == 0).all() and lse[b, h] == -np.inf, (b, h)
+                        continue
+                    e = np.exp(s - s.max())
+                    p = e / e.sum()
+                    o = (p[:, None] * v[:, h // G]).sum(0)
+                    size = (p[:, None] * np.abs(v[:, h // G])).sum(0)
+                bar = 2 * 68 * U * S + 600 * U
+                if np.isnan(p).any():
+                    assert np.isnan(got[b, h]).all() and np.isnan(lse[b, h]), (b, h, got[b, h, 0], lse[b, h])
+                    # every slot whose score is not -inf takes the NaN
+                    want_w[h // G, s != -np.inf] = np.nan
+                    continue
+                w_lse = s.max() + np.log(e.sum())
+                assert abs(lse[b, h] - w_lse) <= 68 * U * S + 600 * U + 2 * U * abs(w_lse), (b, h)
+                fine = np.isfinite(o)
+                assert np.array_equal(got[b, h][~fine], o[~fine], equal_nan=True), (b, h)
+                room = bar * size[fine] + (2.0 ** -8 * np.abs(o[fine]) if self.io else 0)
+                assert (np.abs(got[b, h][fine] - o[fine]) <= room).all(), (b, h)
+                want_w[h // G] += p
+                bar_w[h // G] += (bar + 4 * U) * p + U * want_w[h // G]
+            nan = np.isnan(want_w)
+            assert np.array_equal(np.isnan(w[b][:, j]), nan)
+            assert (np.abs(w[b][:, j] - want_w)[~nan] <= bar_w[~nan]).all()
+        return got
+
+
+def each(f):
+    f = pytest.mark.parametrize("lens", LENS, ids=str)(f)
+    return pytest.mark.parametrize("cache,io", TYPES)(f)
+
+
+@each
+def test_nan_query(gpu, lens, cache, io):
+    """A head whose query holds a NaN is NaN, its neighbours are not."""
+    c = Call(lens, cache, io)
+    c.q[0, 1, 7] = np.nan
+    c.q[-1, 5] = np.nan
+    c.check()
+
+
+@each
+def test_nan_key(gpu, lens, cache, io):
+    """A visible key that holds a NaN makes its kv head NaN."""
+    c = Call(lens, cache, io)
+    c.put(c.t.k, 0, 9, 1, 70, np.nan)
+    c.check()
+    c = Call(lens, cache, io)
+    c.put(c.t.k, 0, lens[0] - 1, 0, 0, np.nan)  # the last split's last slot
+    c.check()
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+def test_lone_nan_key(gpu, cache, io):
+    """The only visible slot, and the only one of its split."""
+    c = Call((1,), cache, io)
+    c.put(c.t.k, 0, 0, 0, 3, np.nan)
+    c.check()
+    c = Call((600,), cache, io)
+    c.mask[0, 256:512] = 0
+    c.mask[0, 300] = 1
+    c.put(c.t.k, 0, 300, 1, 3, np.nan)
+    c.check()
