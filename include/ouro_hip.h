@@ -511,8 +511,8 @@ typedef struct ouro_kv_history {
  * visible one scores -inf, out = 0 and lse = -inf; a NaN among a head's visible
  * scores makes its out, its lse and what it adds to the history of the slots
  * that score above -inf NaN.  What lies in slots that are not visible (NaN,
- * infinities) changes nothing, and their weights stay.  The rows of a sequence do not depend on the batch it is
- * in, and the same call gives the same bits.
+ * infinities) changes nothing, and their weights stay.  The rows of a sequence
+ * do not depend on the batch it is in, and the same call gives the same bits.
  *   q, out [seqs][n_head][head_dim] of `dtype`, rows q_stride and out_stride
  *     elements apart; gate (or NULL) as q, q_stride apart too;
  *   k_new, v_new (or both NULL) [seqs][n_head_kv][head_dim] of `dtype`, rows

@@ -142,10 +142,24 @@ __device__ __forceinline__ void split(const float (&x)[M], uint32_t (&w)[N][M / 
             }
         }
 }
+// A query's: each operand cut off instead of rounded, so that the first is
+// infinite only where x is, and a finite x is finite whole; a NaN stays one.
 template <int N>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8_t (&s)[N]) {
+__device__ __forceinline__ void split_query(const float (&x)[8], bf16x8_t (&s)[N]) {
     uint32_t w[N][4];
-    split<N>(x, w);
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __builtin_canonicalizef(x[i]);  // a NaN with a top bit of its significand set
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[k][i] = __builtin_amdgcn_perm(__float_as_uint(r[2 * i + 1]), __float_as_uint(r[2 * i]), 0x07060302u);
+            if (k + 1 < N) {
+                r[2 * i] -= __uint_as_float(__float_as_uint(r[2 * i]) & 0xffff0000u);
+                r[2 * i + 1] -= __uint_as_float(__float_as_uint(r[2 * i + 1]) & 0xffff0000u);
+            }
+        }
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k] = __builtin_bit_cast(bf16x8_t, u32x4_t{w[k][0], w[k][1], w[k][2], w[k][3]});
 }
@@ -360,7 +374,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
         if (jr < nq && dim < d) load_row<KC>(static_cast<const IO *>(a.q) + b * a.q_stride + static_cast<int64_t>(h0 + jr) * d + dim, x);
         if constexpr (kHalf) {
             bf16x8_t s[NQ];
-            split8<NQ>(x, s);
+            split_query<NQ>(x, s);
 #pragma unroll
             for (int k = 0; k < NQ; ++k) reinterpret_cast<bf16x8_t *>(lds)[k * NJ * 64 + i] = s[k];
         } else {
@@ -442,6 +456,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
         f32x4_t sc = part[NQ - 1];  // the smallest first
 #pragma unroll
         for (int k = NQ - 2; k >= 0; --k) sc += part[k];
+        // Where a key or a query is infinite or NaN the first operands alone say
+        // what the score is: they have the queries' signs and zeros, and the
+        // others, of either sign or 0, would make an infinity NaN.
+        if constexpr (NQ > 1) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) sc[i] = fabsf(part[0][i]) < INFINITY ? sc[i] : part[0][i];
+        }
         sc *= sl2;
         if (now != 0xffffu) {
 #pragma unroll

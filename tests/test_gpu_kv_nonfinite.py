@@ -1,6 +1,8 @@
-"""Attention over a paged cache (ouro_kv_attend) with a NaN where it counts: in
-a query or in a visible key.  The head is then NaN, and so are its lse and its
-part of the history; no slot that is not visible is touched by it.
+"""Attention over a paged cache (ouro_kv_attend) with NaN and infinities where
+they count: in queries and in visible keys.  The formula in IEEE arithmetic
+holds: a NaN score, or one of +inf, makes its head NaN; a score of -inf weighs
+nothing.  Keys of a bf16 cache and of an fp32 cache alike, whatever the queries'
+type, and no slot that is not visible is touched by any of it.
 
 What is finite is held to the bars of test_gpu_kv_cache.py."""
 import numpy as np
@@ -119,4 +121,57 @@ def test_lone_nan_key(gpu, cache, io):
     c.mask[0, 256:512] = 0
     c.mask[0, 300] = 1
     c.put(c.t.k, 0, 300, 1, 3, np.nan)
+    c.check()
+
+
+@each
+def test_keys_of_minus_infinity(gpu, lens, cache, io):
+    """A visible key that scores -inf weighs nothing, for queries that bf16 holds and others."""
+    for whole in (False, True):
+        c = Call(lens, cache, io)
+        c.q[..., 11] = np.abs(c.q[..., 11]) + np.float32(0.1)
+        if whole:
+            c.q = dec(enc(c.q, True))
+        c.put(c.t.k, 0, 3, 0, 11, -np.inf)
+        c.put(c.t.k, 0, 35, 1, 11, -np.inf)
+        c.check()
+
+
+@each
+def test_keys_of_infinity(gpu, lens, cache, io):
+    """Queries of either sign: a head's score is -inf or +inf, whose softmax is NaN; 0 times infinity is NaN."""
+    c = Call(lens, cache, io)
+    c.put(c.t.k, 0, 3, 0, 11, np.inf)
+    c.q[0, 0, 11] = 0
+    c.q[0, 1, 11] = -0.7
+    c.q[0, 2, 11] = 0.7
+    c.check()
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+def test_all_scores_minus_infinity(gpu, cache, io):
+    """No score above -inf: as where no slot is visible."""
+    c = Call((40,), cache, io)
+    c.q[..., 11] = np.abs(c.q[..., 11]) + np.float32(0.1)
+    for j in range(40):
+        if j // PAGE != 1:
+            c.put(c.t.k, 0, j, 0, 11, -np.inf)
+    c.check()
+
+
+@pytest.mark.parametrize("cache", [True, False])
+def test_infinite_and_largest_queries(gpu, cache):
+    """An infinite query has scores of +inf and -inf; the type's largest one is a number like others."""
+    c = Call((300,), cache, False)
+    c.q[0, 0, 5] = np.inf
+    c.q[0, 4, 6] = -np.inf
+    c.check()
+    c = Call((300,), cache, False)
+    c.q[0, 1, 5] = np.finfo(np.float32).max
+    c.q[0, 3, 6] = -np.finfo(np.float32).max
+    for j in range(300):
+        if j // PAGE != 1:
+            for dim in (5, 6):
+                for head in range(HKV):
+                    c.put(c.t.k, 0, j, head, dim, c.t.rng.integers(-3, 4) * 2.0 ** -125)
     c.check()
