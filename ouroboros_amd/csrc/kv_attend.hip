@@ -55,6 +55,8 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short bf16x4_t __attribute__((ext_vector_type(4)));  // the builtin's type of four bf16
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
@@ -122,6 +124,13 @@ __device__ __forceinline__ void load_row(const T *p, float (&x)[N]) {
 // Two floats as bf16, rounded to nearest even, in one dword.
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+}
+// Two bf16 with infinities and NaN as the largest finite value of their sign:
+// by their bits, positive ones order as signed numbers and negative ones as
+// unsigned.
+__device__ __forceinline__ uint32_t finite_bf16(uint32_t w) {
+    const i16x2_t pos = __builtin_elementwise_min(__builtin_bit_cast(i16x2_t, w), i16x2_t(0x7f7f));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, pos), u16x2_t(0xff7f)));
 }
 // x as a sum of N bf16 operands, each the rounding of what the ones before
 // leave (the differences are exact): 8 bits of the significand apiece, so three
@@ -507,10 +516,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
                             w[e][i] = __builtin_amdgcn_perm(vf[2 * i + 1][nb][(e0 + e) >> 1], vf[2 * i][nb][(e0 + e) >> 1],
                                                             e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                    for (int k = 0; k < NP; ++k)
+                    for (int k = 0; k < NP; ++k) {
+                        // a value that is not finite counts by its weight's first
+                        // operand: the others, 0 or negative, would make an infinity NaN
+                        if (k == 1)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = u32x2_t{finite_bf16(w[e][0]), finite_bf16(w[e][1])};
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             o[nb][e0 + e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_t, w[e]), pf[k], o[nb][e0 + e], 0, 0, 0);
+                    }
                 }
         } else {
 #pragma unroll

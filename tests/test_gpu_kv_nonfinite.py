@@ -1,8 +1,9 @@
 """Attention over a paged cache (ouro_kv_attend) with NaN and infinities where
-they count: in queries and in visible keys.  The formula in IEEE arithmetic
+they count: in queries and in visible rows.  The formula in IEEE arithmetic
 holds: a NaN score, or one of +inf, makes its head NaN; a score of -inf weighs
-nothing.  Keys of a bf16 cache and of an fp32 cache alike, whatever the queries'
-type, and no slot that is not visible is touched by any of it.
+nothing; a value that is not finite makes its own dimension what the sum of
+p v is, and no other.  Rows of a bf16 cache and of an fp32 cache alike, whatever
+the queries' type, and no slot that is not visible is touched by any of it.
 
 What is finite is held to the bars of test_gpu_kv_cache.py."""
 import numpy as np
@@ -156,6 +157,25 @@ def test_all_scores_minus_infinity(gpu, cache, io):
     for j in range(40):
         if j // PAGE != 1:
             c.put(c.t.k, 0, j, 0, 11, -np.inf)
+    c.check()
+
+
+@each
+def test_infinite_and_nan_values(gpu, lens, cache, io):
+    """A value that is not finite decides its own dimension: inf, -inf, NaN, and inf beside -inf."""
+    c = Call(lens, cache, io)
+    for slot, dim, x in ((3, 0, np.inf), (35, 1, -np.inf), (36, 2, np.nan), (3, 71, np.inf), (37, 71, -np.inf), (38, 40, np.inf), (39, 40, np.inf)):
+        c.put(c.t.v, 0, slot, 1, dim, x)
+    got = c.check()
+    assert got[0, G, 0] == np.inf and got[0, G, 1] == -np.inf and np.isnan(got[0, G, [2, 71]]).all() and got[0, G, 40] == np.inf
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+def test_infinite_value_alone(gpu, cache, io):
+    """Weight 1 exactly: nothing is left for a weight's lower parts."""
+    c = Call((1,), cache, io)
+    c.put(c.t.v, 0, 0, 0, 3, -np.inf)
+    c.put(c.t.v, 0, 0, 1, 4, np.nan)
     c.check()
 
 
