@@ -549,6 +549,15 @@ int ouro_kv_attend(const ouro_kv_cache *cache, const ouro_kv_history *history,
  * `keep` that stays, rows of k and v (of all kv heads where the history has
  * one head) and history alike.  Sequences of at most `keep` slots stay as
  * they are.  Slots at or above the new length are left as they were.
+ * The choice goes by the history alone, so each slot below the length of a
+ * sequence that is cut must have its page.  Nothing is read or written through
+ * a hole, but what is said of the choice counts its slots like others: a row
+ * that should go to one is lost, and a slot that should be filled from one
+ * keeps the row it had.  Pages that were given up are taken out of the table
+ * first, the last page and its slots' history moved into their place: neither
+ * call minds the order of the slots.  A mask that attention was given is not
+ * moved: with one history head the caller's follows slot_from; where each head
+ * chooses for itself no mask of [seqs][slots] describes what is left.
  *   left (or NULL: the history itself) receives weight and pos of the slots
  *     kept; its slots >= min(keep, max_len);
  *   lens_out [seqs] = min(lens[b], keep), not the array lens;

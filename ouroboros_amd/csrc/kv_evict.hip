@@ -59,7 +59,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs &a, int64_t b, int h, 
     for (int i = first; i < n; i += step) {
         const int2 m = move[i];
         const int64_t dst = kv_slot(a.c, b, m.x) * a.c.elem, src = kv_slot(a.c, b, m.y) * a.c.elem;
-        if (src < 0 || dst < 0) continue;  // a hole
+        if (src < 0 || dst < 0) continue;  // a hole, which the caller promised not to have: no access through it
         const u32x4_t x = *reinterpret_cast<const u32x4_t *>(k + src), y = *reinterpret_cast<const u32x4_t *>(v + src);
         // not kept by the caches, which whoever reads the row next is not behind
         // (100 MB moved: 27.5 us, 33.1 with plain stores, 30.9 with loads past them too)

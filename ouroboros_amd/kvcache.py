@@ -68,7 +68,8 @@ class KVCache:
               out: History | None = None, slot_from=None, workspace=None, stream=None) -> None:
         """Cut every sequence to its `recent` newest positions and the heaviest
         other slots, `keep` in all; the history (or `out`) and lens_out describe
-        what is left."""
+        what is left.  Every slot in use of a sequence that is cut has its page
+        (the choice does not look at the page table), and masks are not moved."""
         call("ouro_kv_evict", self._ref, history._ref, _addr(lens), seqs, max_len, keep, recent,
              out._ref if out else None, _addr(lens_out), _addr(slot_from), _addr(workspace), stream)
 
