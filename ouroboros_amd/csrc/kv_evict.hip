@@ -17,13 +17,14 @@ struct EvictArgs {
     const float *weight;
     const int32_t *pos, *lens;
     float *weight_out;
-    int32_t *pos_out, *lens_out, *slot_from;  // slot_from [seqs][heads][keep]
+    int32_t *pos_out, *lens_out, *slot_from;  // slot_from [seqs][heads][n_from]
     int2 *move;                               // [seqs][heads][most]: a slot to fill, and the slot that fills it
     int32_t *moves;                           // [seqs][heads]
     int32_t heads, slots, slots_out, max_len, keep, recent, most, vecs;  // vecs: 16-byte vectors of a row
+    int32_t n_from, pad;  // n_from: keep, in the workspace no more than max_len
 };
 // passed by value to kernels: the host and device passes must lay it out alike
-static_assert(sizeof(EvictArgs) == 176, "EvictArgs: kernel argument layout");
+static_assert(sizeof(EvictArgs) == 184, "EvictArgs: kernel argument layout");
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -95,13 +96,13 @@ __global__ __launch_bounds__(kThreads) void kv_choose_kernel(EvictArgs a) {
     const int n = max(0, min(a.lens[b], a.max_len)), keep = a.keep;
     const float *weight = a.weight + row * a.slots;
     const int32_t *pos = a.pos + row * a.slots;
-    int32_t *from = a.slot_from + row * keep;
+    int32_t *from = a.slot_from + row * a.n_from;
     float *w_out = a.weight_out + row * a.slots_out;
     int32_t *pos_out = a.pos_out + row * a.slots_out;
     const bool apart = w_out != weight;
     if (hs == 0 && t == 0) a.lens_out[b] = min(n, keep);
     if (n <= keep) {
-        for (int j = t; j < keep; j += kThreads) from[j] = j < n ? j : -1;
+        for (int j = t; j < a.n_from; j += kThreads) from[j] = j < n ? j : -1;
         if (!Moves && t == 0) a.moves[row] = 0;
         if (apart)
             for (int j = t; j < n; j += kThreads) w_out[j] = weight[j], pos_out[j] = pos[j];
@@ -338,8 +339,10 @@ size_t most_moves(size_t max_len, size_t keep) {
     const size_t gone = max_len > keep ? max_len - keep : 0;
     return keep < gone ? keep : gone;
 }
-size_t evict_ws_bytes(size_t seqs, size_t heads, size_t max_len, size_t keep) {
-    return (seqs * heads * (most_moves(max_len, keep) * sizeof(int2) + (keep + 1) * sizeof(int32_t)) + 255) & ~size_t{255};
+// The workspace: the moves, their numbers, n_from entries a row of a slot_from
+// that the caller does not ask for.
+size_t evict_ws_bytes(size_t seqs, size_t heads, size_t max_len, size_t keep, size_t n_from) {
+    return (seqs * heads * (most_moves(max_len, keep) * sizeof(int2) + (n_from + 1) * sizeof(int32_t)) + 255) & ~size_t{255};
 }
 
 template <bool Moves>
@@ -365,7 +368,7 @@ using namespace ouro;
 extern "C" {
 
 size_t ouro_kv_evict_workspace_bytes(size_t seqs, size_t heads, size_t max_len, size_t keep) {
-    return evict_ws_bytes(seqs, heads, max_len, keep);
+    return evict_ws_bytes(seqs, heads, max_len, keep, keep);
 }
 
 int ouro_kv_evict(const ouro_kv_cache *cache, const ouro_kv_history *history, const int32_t *lens, size_t seqs,
@@ -390,8 +393,9 @@ int ouro_kv_evict(const ouro_kv_cache *cache, const ouro_kv_history *history, co
         (left->weight == history->weight && left->slots != history->slots))
         return fail(OURO_ERR_INVALID_ARG, "%s: the history left is neither the history nor apart from it", me);
     if (!seqs) return OURO_OK;
-    const size_t heads = history->heads, most = most_moves(max_len, keep), need = evict_ws_bytes(seqs, heads, max_len, keep);
-    if (!ws && !(ws = workspace(need, stream))) return OURO_ERR_HIP;
+    const size_t heads = history->heads, most = most_moves(max_len, keep);
+    const size_t n_from = slot_from ? keep : keep < max_len ? keep : max_len;  // a budget may be far above every length
+    if (!ws && !(ws = workspace(evict_ws_bytes(seqs, heads, max_len, keep, slot_from ? 0 : n_from), stream))) return OURO_ERR_HIP;
     a.weight = history->weight, a.pos = history->pos, a.lens = lens;
     a.weight_out = left->weight, a.pos_out = left->pos, a.lens_out = lens_out;
     a.move = static_cast<int2 *>(ws);
@@ -399,6 +403,7 @@ int ouro_kv_evict(const ouro_kv_cache *cache, const ouro_kv_history *history, co
     a.slot_from = slot_from ? slot_from : a.moves + seqs * heads;
     a.heads = static_cast<int>(heads), a.slots = history->slots, a.slots_out = left->slots;
     a.max_len = static_cast<int>(max_len), a.keep = static_cast<int>(keep), a.recent = static_cast<int>(recent);
+    a.n_from = static_cast<int>(n_from);
     a.most = static_cast<int>(most), a.vecs = a.c.d * a.c.elem / 16;
     hipStream_t s = as_stream(stream);
     if (most * (heads > 1 ? 1 : a.c.n_head_kv) * a.vecs * 32 <= kFew) {
