@@ -734,13 +734,15 @@ int launch_attend(const AttendArgs &a, unsigned seqs, hipStream_t s) {
     using Kernel = void (*)(AttendArgs);
     static const Kernel kernels[4] = {kv_attend_split_kernel<C, IO, DP, false, false>, kv_attend_split_kernel<C, IO, DP, false, true>,
                                       kv_attend_split_kernel<C, IO, DP, true, false>, kv_attend_split_kernel<C, IO, DP, true, true>};
-    if (lds + 1024 > 65536) {  // one opt-in per process and kernel for more than 64 KiB of LDS (idempotent)
-        static std::atomic<bool> done[4];
-        if (!done[which].load(std::memory_order_acquire)) {
+    if (lds + 1024 > 65536) {  // one opt-in per kernel and device for more than 64 KiB of LDS (idempotent)
+        static std::atomic<uint64_t> done[4];
+        const int dev = current_device();
+        const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t{1} << dev : 0;
+        if (!(done[which].load(std::memory_order_acquire) & bit)) {
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernels[which]),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
             if (e != hipSuccess) return fail(OURO_ERR_HIP, "ouro_kv_attend: LDS opt-in: %s", hipGetErrorString(e));
-            done[which].store(true, std::memory_order_release);
+            done[which].fetch_or(bit, std::memory_order_release);
         }
     }
     hipLaunchKernelGGL(kernels[which], grid, dim3(256), lds, s, a);
