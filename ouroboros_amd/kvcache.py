@@ -13,11 +13,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import KvCacheDesc, KvHistoryDesc, call, dtype_code
-from .device import DeviceBuffer
-
-
-def _addr(a):
-    return a.ptr if isinstance(a, DeviceBuffer) else a
+from .ops import _addr
 
 
 class History:
