@@ -66,6 +66,8 @@ constexpr int kQ = 16;       // query heads of a workgroup: the columns of its p
 // cache, which holds a smaller one from one call to the next where nothing else
 // comes between.  (64 sequences of up to 1025 keys, 134 MB: 37.4 -> 34.2 us; 24
 // of up to 8191 of half the width, 100 MB, called again and again: 24.9 -> 30.3)
+// Between these two the line is not measured closely: 63 sequences of 1025 keys,
+// just below it, take 39.7 us over three caches in turn, 64 above it 37.0.
 constexpr int64_t kKeptBytes = 128 << 20;
 constexpr int kJoin = 8;     // query heads that the wavefronts' outputs are joined for at a time
 
@@ -205,7 +207,8 @@ __device__ __forceinline__ T load_cache(const T *p) {
 }
 
 // x, as a value that is made where this stands: what is computed from it stays
-// in the loop instead of being kept in registers throughout it.
+// in the loop instead of being kept in registers throughout it.  The asm holds no
+// instruction, so that no wait state is owed around it.
 __device__ __forceinline__ int in_loop(int x) {
     asm volatile("" : "+v"(x));
     return x;
@@ -241,11 +244,12 @@ __device__ __forceinline__ void store_lse(const AttendArgs &a, int64_t b, int h,
 // everything else is fp32.
 //
 // Bound by memory where the splits fill the chip: 64 sequences of 16384 keys
-// (4 kv heads of 128, bf16) at 5.7 TB/s, 512 of up to 1025 at 5.1, 64 of up to
-// 2176 in fp32 in 52 us (5.2).  Below that by what a workgroup does before its
-// first products and after its last (pages, queries, the four outputs joined):
-// 64 sequences of up to 1025 keys take 26.5 us, 21 without reading K or V, one
-// sequence of 16384 10.5, one of 300 7.5.  Splits of 256 slots because one
+// (4 kv heads of 128, bf16) at 5.8 TB/s, 64 of up to 2176 in fp32 in 52.7 us
+// (5.1); a kernel that only reads 4 GiB reaches 7.  Below that by what a
+// workgroup does before its first products and after its last (pages, queries,
+// the four outputs joined): 64 sequences of up to 1025 keys take 26.9 us, of
+// which some 21 remain without reading K or V, one sequence of 16384 11.0, one of
+// 300 8.0.  Splits of 256 slots because one
 // sequence must fill the chip; several splits a workgroup were no faster.  The
 // loads of the next tile stand before a tile's products and need no count of
 // what is in flight: there is always a tile's worth.
@@ -257,7 +261,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(C) =
     constexpr int KC = kHalf ? 8 : 4;                     // dims of a lane's 16 bytes of K
     constexpr int NJ = DP / (4 * KC);                     // steps over the dims
     constexpr int NQ = kHalf && sizeof(IO) == 4 ? 3 : 1;  // operands of a query
-    constexpr int NP = 3;                                 // and of a weight (bf16 cache)
+    constexpr int NP = 3;                                 // and of a weight (bf16 cache); two, for bf16 rows, saved 0.15 us of 23.75
     constexpr int CH = kHalf && DP > 64 ? 8 : 4;          // adjacent dims of V a lane
     constexpr int NB = DP / (16 * CH);
     constexpr int NR = TS / 4;                            // slots of a lane
@@ -703,7 +707,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs &a, int64_t b, int 
 // head: 512, so that few workgroups repeat the heads' maxima, or 256 where a
 // slot's weight takes the scores of many heads (24 sequences of up to 8191
 // slots: 32 heads 27.0 us with 512 and 25.5 with 256, 64 of up to 1025 with 4
-// heads 32.5 and 33.1).
+// heads 32.5 and 33.1; between them, where the line is drawn, nothing is measured).
 template <typename IO, int DP>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, int joins) {
     __shared__ f32x4_t red[256];

@@ -73,18 +73,21 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBinBits = 11, kBins = 1 << kBinBits, kCopies = 4;  // bins of a count, and how many lanes' counts share one
 
 // The choice of one (head, sequence) by one workgroup of 16 wavefronts, each
-// with a run of slots in order, 64 R of them in registers (longer runs are read
-// again at each pass).  The runs' blocks of 64 start so that one starts at
-// slot `keep`: what a block's slots may become is the same for all of them.  The order of the last slot that stays is found from
-// counts in bins, from the largest order down, first of all orders, then of the
-// bin that holds it.  Moves: the workgroup copies the rows too.
+// with a run of slots in order, 64 R of them in registers (longer runs, past
+// 16384 places with the up to 63 before slot 0, are read again at each pass:
+// the whole call for 4 rows of 16384 slots cut to 2048 25 us, to 2000 40, 4 of
+// 16385 42, of 40000 67).  The runs' blocks of 64 start so that one starts at
+// slot `keep`: what a block's slots may become is the same for all of them.  The
+// order of the last slot that stays is found from counts in bins, from the
+// largest order down, first of all orders, then of the bin that holds it.
+// Moves: the workgroup copies the rows too.
 //
 // Bound by instructions and barriers: a pass over 16384 slots costs a workgroup
 // 256 cycles for each instruction a slot takes, a barrier about 400.  Four rows
-// of 16384 slots and 4 heads, a workgroup each: 17 us, of which the counts in
-// bins 4, the two passes over what stays 5, loads 2.  64 rows of 1025 slots, 4
-// heads: 7.8 us with the launch.  Counting thresholds with ballots, 12 rounds of
-// three, took 33 us where the bins take 19.
+// of 16384 slots, a workgroup each: 17.5 us, of which the counts in bins 4, the
+// two passes over what stays 5, loads 2.  64 rows of 1025 slots, 4 heads: 7.8 us
+// with the launch.  Counting thresholds with ballots, 12 rounds of three, took
+// 14 us more.
 template <int R, bool Moves>
 __global__ __launch_bounds__(kThreads) void kv_choose_kernel(EvictArgs a) {
     __shared__ int4 tmp[2][kWaves];

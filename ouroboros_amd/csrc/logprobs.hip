@@ -273,9 +273,15 @@ __global__ __launch_bounds__(Parts * kThreads) void logprobs_part_kernel(ScoreAr
 // A lower bound of the k-th largest key: the k-th largest of the groups' largest
 // (a group has every 256th segment).  Few segments reach it, and only their
 // logits are read again: those at or above the bound become candidates.  Where
-// ties or a skewed row make them more than kCap, the bound is raised by
-// bisection (keys are unique, so some bound leaves k to kCap of them).  The
-// candidates' places are their ranks among each other.
+// they are more than kCap, the bound is raised by bisection (keys are unique, so
+// some bound leaves k to kCap of them).  The candidates' places are their ranks
+// among each other.
+//
+// A row of fewer segments than k (16 a part of 8192 logits: up to 8192 logits
+// for k over 16, 24576 for k over 48) has no such bound: all its logits are
+// candidates, or what a bisection of them leaves, and their ranks cost their
+// number squared.  64 rows of 8000 logits take 14.4 us with k = 16 and 78 with 17
+// to 64, of 2000 14.4 and 90, of 24000 24.7 with 48 and 86 with 64.
 //
 // Bound by latency, a chain of loads and barriers: 6.5 us for one row of 248320
 // (31 parts) with 20 alternatives, 10 for 512 rows with 8.  1024 threads because
@@ -295,7 +301,7 @@ __global__ __launch_bounds__(kJoin) void logprobs_join_kernel(ScoreArgs a) {
     const Row<T> x(a, row);
     const int ns = a.parts * kSegs;
     const unsigned long long *seg = a.seg + row * ns;
-    // the groups' largest keys: thread t takes segments t, t + kJoin, ..: group t % 64
+    // the groups' largest keys: thread t takes segments t, t + kJoin, ..: group t % kGroups
     unsigned long long first = 0;  // the thread's first segment's key
     const int g = a.target ? a.target[row] : -1;
     float4 part = make_float4(-INFINITY, 0.f, 0.f, 0.f);
