@@ -17,8 +17,9 @@
  *     (k == 1): the lookup kernels' per-block partial sums;
  *   - ouro_matmul_q on a raw TL1 payload for k >= 2 columns: x as int8
  *     digit planes for the MFMA pass;
- *   - ouro_gdn_chunk_prefill, ouro_kv_attend, ouro_kv_evict and
- *     ouro_token_logprobs with a NULL workspace.
+ *   - ouro_gdn_chunk_prefill, ouro_kv_attend, ouro_kv_evict,
+ *     ouro_token_logprobs, ouro_kv8_attend and ouro_verify_drafts with a NULL
+ *     workspace.
  * A weight handle (ouro_weight_upload) or ouro_matvec_q_noalloc avoids them.
  *
  * Conventions
@@ -594,6 +595,163 @@ int ouro_token_logprobs(const void *logits, int dtype, size_t rows, size_t n,
                         float *logprob, int32_t *rank, float *entropy,
                         float *lse, int32_t *top_id, float *top_logprob,
                         void *workspace, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Head norms and rotary positions                                      */
+/* ------------------------------------------------------------------ */
+
+#define OURO_ROPE_ADJACENT 1u /* pairs (2i, 2i + 1); default (i, i + n_rot/2) as rope_partial_neox */
+
+/* Of every query and key head x [head_dim] of `rows` tokens, in one pass
+ * (rmsnorm_head and rope_partial_neox, qwen35.rs:96-106,1246-1248):
+ *   x <- x gain / sqrt(mean x^2 + eps)                  (gain NULL: x as it is)
+ *   (x_i, x_j) <- (x_i cos t - x_j sin t, x_j cos t + x_i sin t),
+ *     t = pos[axis[i] * rows + token] * freq[i], i = 0 .. n_rot/2 - 1
+ * over the first n_rot dims; the others are normed only.  The angle is taken in
+ * 64 bits, everything else in 32, and the result is rounded once.
+ *   q, q_out [rows][n_head][head_dim] of `dtype`, rows q_stride / q_out_stride
+ *     and heads q_head_stride elements apart (the output's heads without gap);
+ *     k, k_out with k_stride, k_out_stride in the same way (n_head_kv = 0: no
+ *     keys).  A stride of 0 stands for no gap.  An output may be its input
+ *     (the same address and strides); other overlaps are not allowed.
+ *   q_gain, k_gain f32 [head_dim]; freq f32 [n_rot/2], radians a position;
+ *   pos int32 [axes][rows], any position of 32 bits; axis (or NULL: all 0)
+ *     int32 [n_rot/2], each 0 .. axes - 1 (read as the nearest of them), for
+ *     positions in time, height and width.
+ * head_dim a multiple of 8, 8 .. 256; n_rot a multiple of 4, 0 .. head_dim;
+ * rows at most 2^24; rows start at multiples of 16 bytes.  Infinities and NaN go as the formulas
+ * take them, and reach no other head. */
+int ouro_qk_norm_rope(const void *q, size_t q_stride, size_t q_head_stride,
+                      const void *k, size_t k_stride, size_t k_head_stride,
+                      const float *q_gain, const float *k_gain,
+                      const int32_t *pos, size_t axes, const int32_t *axis,
+                      const float *freq, size_t n_rot, unsigned flags,
+                      void *q_out, size_t q_out_stride, void *k_out,
+                      size_t k_out_stride, int dtype, size_t rows,
+                      size_t n_head, size_t n_head_kv, size_t head_dim,
+                      float eps, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* A paged key-value cache of 8-bit codes                               */
+/* ------------------------------------------------------------------ */
+
+/* As ouro_kv_cache, with int8 codes: an element stands for code * scale, with
+ * one float scale for each block of block_tokens slots (0, block_tokens, .. of
+ * a page) and kv head,
+ *   k_scale[(page * (page_tokens / block_tokens) + block) * n_head_kv + head].
+ * k, v and the strides are multiples of 16 bytes (OURO_ERR_ALIGN), head_dim a
+ * multiple of 16, 16 .. 256, page_tokens a power of two, 16 .. 2^20, and
+ * block_tokens one, 16 .. 256 and at most page_tokens (OURO_ERR_SHAPE). */
+typedef struct ouro_kv8_cache {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    const int32_t *pages;                            /* [seqs][max_pages] */
+    int64_t page_stride, token_stride, head_stride;  /* bytes */
+    int32_t n_pages, max_pages, page_tokens, block_tokens, n_head_kv, head_dim;
+} ouro_kv8_cache;
+
+/* The newest rows of each sequence, for the calls below.  Sequence b has
+ * lens[b] slots in use, and rows cu[b] .. cu[b + 1] - 1 of the packed arrays are
+ * its newest: row i of its T is slot lens[b] - T + i.  cu [seqs + 1] (or NULL:
+ * max_new rows each, rows = seqs * max_new) and lens [seqs] are on the device;
+ * `rows` is the packed arrays' length (up to 2^23) and max_new bounds T.  What is out of
+ * range is not followed: cu is read as 0 .. rows, T as 0 .. max_new, lens as 0
+ * .. the slots of max_pages pages; a row before slot 0 has no slot.
+ *
+ * New keys and values into the cache, `dtype` rows [n_head_kv][head_dim],
+ * new_stride elements apart (0: no gap).  For each block and kv head that gets
+ * rows, and keys and values each,
+ *   scale = the smallest power of two with max |x| <= 127 scale over its new
+ *     rows; where slots before them are in the block, at least its old scale;
+ *   code = x / scale rounded to nearest even;
+ * and where the scale grew, the codes of the slots before are rounded to it.
+ * So a block's scale is the largest that its rows need, in whatever pieces they
+ * came, and a row's error is at most half a step when it is written and less
+ * than half of the present step more by later growth.  A NaN is held as 0, an
+ * infinity as +-127 steps of what finite values need (as 0 where all are 0), a
+ * block of zeros has scale 0.  Other slots keep their codes.  Two sequences must
+ * not write to one page in a call; rows of a hole are dropped. */
+int ouro_kv8_write(const ouro_kv8_cache *cache, const void *k_new,
+                   const void *v_new, size_t new_stride, int dtype,
+                   const int32_t *lens, const int32_t *cu, size_t seqs,
+                   size_t rows, size_t max_new, void *stream);
+/* Rows of the cache as code * scale (exact in either dtype with the scales of
+ * ouro_kv8_write, rounded to nearest even otherwise), 0 for a row without a
+ * slot or of a hole.  k_out or v_out may be NULL; rows past the last sequence
+ * are left as they were. */
+int ouro_kv8_read(const ouro_kv8_cache *cache, const int32_t *lens,
+                  const int32_t *cu, size_t seqs, size_t rows, size_t max_new,
+                  void *k_out, void *v_out, size_t out_stride, int dtype,
+                  void *stream);
+/* Attention of each sequence's newest rows (one new token, drafted ones, a
+ * piece of a prompt; already written) over its cache: for query head h of the
+ * row in slot r, over the slots
+ *   j <= r with r - j < window or j < sinks (window 0: every j <= r),
+ * whose page is there and whose mask byte is not 0,
+ *   s_j = scale q.k_j, out = softmax(s) v [* sigmoid(gate)], lse = ln sum e^s,
+ * with kv head h / (n_head / n_head_kv).  Where no slot is visible, out = 0 and
+ * lse = -inf; where a query holds an infinity or NaN, or a visible scale does,
+ * out and lse are NaN.  What lies in slots that are not visible changes
+ * nothing.  The same call gives the same bits, and a sequence's rows do not
+ * depend on the others in the call (max_new being the same).
+ *   q, out (rows q_stride, out_stride apart), gate, mask, lse as of
+ *     ouro_kv_attend, rows packed as above; mask [seqs] rows of max_len bytes;
+ *   max_len bounds lens, at most 2^30.
+ * A stride of 0 stands for rows without a gap.  `workspace`:
+ * ouro_kv8_attend_workspace_bytes() device bytes, 16-byte aligned; NULL takes
+ * the library's. */
+size_t ouro_kv8_attend_workspace_bytes(size_t seqs, size_t rows, size_t max_new,
+                                       size_t n_head, size_t n_head_kv,
+                                       size_t head_dim, size_t max_len);
+int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
+                    const int32_t *lens, const int32_t *cu, const uint8_t *mask,
+                    size_t mask_stride, const void *gate, void *out,
+                    size_t out_stride, float *lse, int dtype, size_t seqs,
+                    size_t rows, size_t max_new, size_t n_head, size_t max_len,
+                    size_t window, size_t sinks, float scale, void *workspace,
+                    void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Drafted tokens judged by the target's logits                         */
+/* ------------------------------------------------------------------ */
+
+/* Sequence b ran the tokens of rows cu[b] .. cu[b + 1] - 1 (as above, 1 ..
+ * max_new of them): its newest token, then drafted ones.  Row i's logits give
+ * p_i = softmax(logits / temperature[b]), which judges token i + 1, drawn from
+ * q_i = softmax(draft row i) (draft NULL: a drafter that named that token, q_i
+ * all on it).  Tokens are kept while u_accept[row i] q_i(t) < p_i(t); at the
+ * first that is not, the next token is drawn from max(p_i - q_i, 0), else from
+ * the last row's p: the lowest t whose cumulative sum over tokens 0 .. t
+ * exceeds u_next[b] of the whole.  So tokens come out distributed as the
+ * target's own.  Sums and comparisons are made in 64 bits.
+ * temperature[b] <= 0 (or NaN) takes the likeliest token (lowest index) for p;
+ * temperature NULL: 1.
+ *   logits, draft: rows of n, row_stride, draft_stride elements apart (0: n),
+ *     f32 or bf16 each; draft rows are what the drafter drew from, up to a
+ *     constant a row; row T - 1 of a sequence is not read;
+ *   tokens int32 [rows]; u_accept f32 [rows] in [0, 1), entry of the row that
+ *     judges; u_next f32 [seqs] in [0, 1);
+ *   accepted int32 [seqs]: drafted tokens kept; next int32 [seqs]: the token
+ *     that follows them;
+ *   lens_out (or NULL) = lens[b] - (T - 1 - accepted[b]): the slots still in use
+ *     after the refused tokens are taken back; may be lens.
+ * A NaN logit counts as -inf; +inf logits share the mass; a probability below
+ * 2^-1000 of the likeliest's counts as 0.  A token outside 0 ..
+ * n - 1 is refused (its q counts as 0).  Where p has no mass at all the token is
+ * refused and next = -1; where max(p - q, 0) has none, next is drawn from p.  A
+ * draft row without mass counts as q = 0.  A sequence without rows: accepted 0,
+ * next -1, lens_out = lens.  n < 2^24.  `workspace`:
+ * ouro_verify_drafts_workspace_bytes() device bytes, 16-byte aligned; NULL takes
+ * the library's. */
+size_t ouro_verify_drafts_workspace_bytes(size_t seqs, size_t rows, size_t n);
+int ouro_verify_drafts(const void *logits, int dtype, size_t row_stride,
+                       const void *draft, int draft_dtype, size_t draft_stride,
+                       const int32_t *tokens, const int32_t *cu, size_t seqs,
+                       size_t rows, size_t max_new, size_t n,
+                       const float *temperature, const float *u_accept,
+                       const float *u_next, const int32_t *lens,
+                       int32_t *accepted, int32_t *next, int32_t *lens_out,
+                       void *workspace, void *stream);
 
 #ifdef __cplusplus
 }

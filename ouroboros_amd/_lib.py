@@ -26,6 +26,7 @@ KIND_F32, KIND_F16, KIND_BF16, KIND_TQ1_0, KIND_TL1, KIND_I2_S, KIND_I2 = 0, 1, 
 KIND_Q8_0, KIND_Q3K, KIND_Q4K, KIND_Q5K, KIND_Q6K = 8, 11, 12, 13, 14
 DT_F32, DT_BF16 = 0, 1
 FWHT_INVERSE = 1
+ROPE_ADJACENT = 1
 GDN_L2NORM_QK, GDN_SCALE_Q, GDN_KHEAD_DIV, GDN_V_GROUPED = 1, 2, 4, 8
 
 
@@ -60,6 +61,13 @@ class KvCacheDesc(C.Structure):
 class KvHistoryDesc(C.Structure):
     """ouro_kv_history (include/ouro_hip.h)."""
     _fields_ = [("weight", C.c_void_p), ("pos", C.c_void_p), ("heads", C.c_int32), ("slots", C.c_int32)]
+
+
+class Kv8CacheDesc(C.Structure):
+    """ouro_kv8_cache (include/ouro_hip.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "pages")] + \
+        [(n, C.c_int64) for n in ("page_stride", "token_stride", "head_stride")] + \
+        [(n, C.c_int32) for n in ("n_pages", "max_pages", "page_tokens", "block_tokens", "n_head_kv", "head_dim")]
 
 
 # name -> (restype, argtypes); every function of include/ouro_hip.h.
@@ -117,6 +125,13 @@ SIGNATURES = {
     "ouro_kv_evict": (i32, [vp, vp, vp, sz, sz, sz, sz, vp, vp, vp, vp, vp]),
     "ouro_token_logprobs_workspace_bytes": (sz, [sz, sz, sz]),
     "ouro_token_logprobs": (i32, [vp, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "ouro_qk_norm_rope": (i32, [vp, sz, sz, vp, sz, sz, vp, vp, vp, sz, vp, vp, sz, u32, vp, sz, vp, sz, i32, sz, sz, sz, sz, f32, vp]),
+    "ouro_kv8_write": (i32, [vp, vp, vp, sz, i32, vp, vp, sz, sz, sz, vp]),
+    "ouro_kv8_read": (i32, [vp, vp, vp, sz, sz, sz, vp, vp, sz, i32, vp]),
+    "ouro_kv8_attend_workspace_bytes": (sz, [sz] * 7),
+    "ouro_kv8_attend": (i32, [vp, vp, sz, vp, vp, vp, sz, vp, vp, sz, vp, i32, sz, sz, sz, sz, sz, sz, sz, f32, vp, vp]),
+    "ouro_verify_drafts_workspace_bytes": (sz, [sz, sz, sz]),
+    "ouro_verify_drafts": (i32, [vp, i32, sz, vp, i32, sz, vp, vp, sz, sz, sz, sz, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "ouro_weight_upload": (i32, [i32, vp, sz, sz, sz, f32, sz, C.POINTER(vp)]),
     "ouro_weight_free": (i32, [vp]),
     "ouro_weight_payload": (vp, [vp]),

@@ -211,3 +211,38 @@ def token_logprobs(logits, rows: int, n: int, *, dtype="f32", row_stride: int = 
     if stream is not None:
         call("ouro_stream_synchronize", stream)
     return {name: b.download() for name, b in out.items()}
+
+
+def qk_norm_rope(q, k, q_out, k_out, pos, freq, *, rows: int, n_head: int, n_head_kv: int, head_dim: int, n_rot: int,
+                 dtype="f32", q_gain=None, k_gain=None, eps: float = 1e-6, axes: int = 1, axis=None,
+                 adjacent: bool = False, q_stride: int = 0, q_head_stride: int = 0, k_stride: int = 0,
+                 k_head_stride: int = 0, q_out_stride: int = 0, k_out_stride: int = 0, stream=None) -> None:
+    """RMS norm of every query and key head (where a gain is given) and the rotary
+    position of its first n_rot dims, in one pass (ouro_qk_norm_rope).
+
+    pos [axes][rows]; pair i turns by pos[axis[i]] * freq[i] radians.  Arguments
+    are device memory; k and k_out may be None with n_head_kv = 0."""
+    _lib.init()
+    call("ouro_qk_norm_rope", _addr(q), q_stride, q_head_stride, _addr(k), k_stride, k_head_stride, _addr(q_gain),
+         _addr(k_gain), _addr(pos), axes, _addr(axis), _addr(freq), n_rot, _lib.ROPE_ADJACENT if adjacent else 0,
+         _addr(q_out), q_out_stride, _addr(k_out), k_out_stride, _lib.dtype_code(dtype), rows, n_head, n_head_kv,
+         head_dim, eps, stream)
+
+
+def verify_drafts(logits, tokens, u_accept, u_next, accepted, next, *, seqs: int, rows: int, max_new: int, n: int,
+                  dtype="f32", row_stride: int = 0, cu=None, draft=None, draft_dtype="f32", draft_stride: int = 0,
+                  temperature=None, lens=None, lens_out=None, workspace=None, stream=None) -> None:
+    """Keep drafted tokens while u q(t) < p(t) and draw the token that follows
+    them, so that the answer is distributed as the target's own
+    (ouro_verify_drafts).  Arguments are device memory; rows are packed as
+    :class:`~ouroboros_amd.kvcache.KVCache8` takes them."""
+    _lib.init()
+    call("ouro_verify_drafts", _addr(logits), _lib.dtype_code(dtype), row_stride, _addr(draft),
+         _lib.dtype_code(draft_dtype), draft_stride, _addr(tokens), _addr(cu), seqs, rows, max_new, n,
+         _addr(temperature), _addr(u_accept), _addr(u_next), _addr(lens), _addr(accepted), _addr(next),
+         _addr(lens_out), _addr(workspace), stream)
+
+
+def verify_workspace_bytes(seqs: int, rows: int, n: int) -> int:
+    """Bytes of scratch that verify_drafts takes."""
+    return int(_lib.lib().ouro_verify_drafts_workspace_bytes(seqs, rows, n))
