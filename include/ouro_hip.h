@@ -690,10 +690,11 @@ int ouro_kv8_read(const ouro_kv8_cache *cache, const int32_t *lens,
  * whose page is there and whose mask byte is not 0,
  *   s_j = scale q.k_j, out = softmax(s) v [* sigmoid(gate)], lse = ln sum e^s,
  * with kv head h / (n_head / n_head_kv).  Where no slot is visible, out = 0 and
- * lse = -inf; where a query holds an infinity or NaN, or a visible scale does,
- * out and lse are NaN.  What lies in slots that are not visible changes
- * nothing.  The same call gives the same bits, and a sequence's rows do not
- * depend on the others in the call (max_new being the same).
+ * lse = -inf; where a query holds an infinity or NaN, out and lse are NaN, and so
+ * where a visible scale is negative or not finite (of V: out alone).  What lies
+ * in slots that are not visible changes nothing.  The same call gives the same
+ * bits, and a sequence's rows do not depend on the others in the call (max_new
+ * and max_len being the same).
  *   q, out (rows q_stride, out_stride apart), gate, mask, lse as of
  *     ouro_kv_attend, rows packed as above; mask [seqs] rows of max_len bytes;
  *   max_len bounds lens, at most 2^30.

@@ -29,11 +29,12 @@ HIPCC_FLAGS = [
     "-Wall",
 ]
 
-# Flags for one source file only.  kquant.hip, tl1_mfma.hip: MFMA results
-# in ordinary VGPRs (the accumulator-register form adds a copy per result
-# read; measured faster in both).
+# Flags for one source file only.  kquant.hip, tl1_mfma.hip, kv8_attend.hip: MFMA
+# results in ordinary VGPRs (the accumulator-register form adds a copy per result
+# read; measured faster in the first two, a wavefront more per SIMD in the third).
 FILE_FLAGS = {
     "kquant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kv8_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "tl1_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -7,10 +7,21 @@
 // and o = 0, lse = -inf where no slot is visible.
 #include "kv_cache.hpp"
 
+#include <atomic>
 #include <cmath>
 
 namespace ouro {
 namespace {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kTurn = 256;  // slots that a workgroup's four wavefronts take in turn: 2 tiles of 32 each
+constexpr int kJoin = 8;    // rows that the wavefronts' outputs are joined for at a time
 
 struct Attend8Args {
     Kv8View c;
@@ -19,10 +30,14 @@ struct Attend8Args {
     const uint8_t *mask;
     void *out;
     float *lse;
+    float *part;  // [rows][n_head][n_split][d]: the splits' outputs, not normalised
+    float2 *ml;   // [rows][n_head][n_split]: their maxima (of scores times log2 e) and sums
     int64_t q_stride, mask_stride, out_stride;
-    int32_t n_head, window, sinks;
+    int32_t n_head, window, sinks;  // window 0: every slot
     float scale;
+    int32_t n_split, turns;  // turns of a split
 };
+static_assert(sizeof(Attend8Args) == 224, "Attend8Args: kernel argument layout");
 
 template <typename T>
 __device__ __forceinline__ float load1(const T *p, int64_t i) {
@@ -38,60 +53,510 @@ __device__ __forceinline__ void store1(T *p, int64_t i, float x) {
     else
         p[i] = f32_to_bf16_bits(x);
 }
+// Sixteen adjacent values of a row.
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, float (&x)[16]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4_t v = reinterpret_cast<const f32x4_t *>(p)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const u32x4_t v = reinterpret_cast<const u32x4_t *>(p)[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[8 * i + e] = __uint_as_float(e & 1 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
+        }
+    }
+}
+// Maximum and sum over the four lanes l, l + 16, l + 32, l + 48.
+__device__ __forceinline__ float quad_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float lane_float(float v, int lane) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+// x, as a value that is made where this stands: what is read by it stays in the
+// loop.  The asm holds no instruction, so that no wait state is owed around it.
+__device__ __forceinline__ int in_loop(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
-// One wavefront a row and head, 64 slots at a time, a lane each.
+// A head's joined output (normalised), through the gate to its place.
 template <typename IO>
-__global__ __launch_bounds__(64) void kv8_attend_kernel(Attend8Args a) {
-    const SeqRows s = seq_rows(a.r, blockIdx.z);
-    const int i = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    if (i >= s.count) return;
-    const int64_t b = blockIdx.z, row = s.first + i;
-    const int d = a.c.d, at = s.n - s.count + i, kvh = h / (a.n_head / a.c.n_head_kv);
-    const IO *q = static_cast<const IO *>(a.q) + row * a.q_stride + static_cast<int64_t>(h) * d;
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-    for (int j0 = 0; j0 <= at; j0 += 64) {
-        const int j = j0 + lane;
-        bool seen = j <= at && (!a.window || at - j < a.window || j < a.sinks);
-        int32_t page = -1;
-        if (seen) {
-            page = a.c.pages[b * a.c.max_pages + (j >> a.c.page_shift)];
-            seen = page >= 0 && page < a.c.n_pages && (!a.mask || a.mask[b * a.mask_stride + j] != 0);
+__device__ __forceinline__ void store_out(const Attend8Args &a, int64_t row, int h, int dim, float o) {
+    const int64_t i = static_cast<int64_t>(h) * a.c.d + dim;
+    if (a.gate) o *= 1.0f / (1.0f + expf(-load1(static_cast<const IO *>(a.gate), row * a.q_stride + i)));
+    store1(static_cast<IO *>(a.out), row * a.out_stride + i, o);
+}
+__device__ __forceinline__ void store_lse(const Attend8Args &a, int64_t row, int h, float m, float l) {
+    if (a.lse) a.lse[row * a.n_head + h] = (m + log2f(l)) * 0.6931471805599453f;  // -inf where l = 0
+}
+// Whether a row in slot `at` can see any of slots j0 .. j1 - 1.
+__device__ __forceinline__ bool sees(const Attend8Args &a, int at, int j0, int j1) {
+    return j0 <= at && (!a.window || j1 + a.window > at + 1 || j0 < a.sinks);
+}
+
+// One workgroup takes 16 NT rows (token by token, each token's query heads of one
+// kv head) of a sequence and kv head against a split of its slots, its four
+// wavefronts on alternate tiles of 32 slots, each with its own running maxima,
+// sums and outputs.
+//
+// Both products run on the matrix cores with the slots as rows of the first and
+// as the inner axis of the second, the query rows as columns:
+//   S^T[slot][row] = K Q^T,  O^T[dim][row] += V^T P^T.
+// K's codes are the first product's operand as they lie in the cache: the query is
+// held in three signed digits of base 256 against a power of two of its row (2 U of
+// the row's largest magnitude, U = 2^-24), and the digits' products with the codes
+// are exact sums in 32-bit integers.  A lane then has one row and slots
+// 4 (lane / 16) + 0 .. 3 of two tiles of 16, and that is the order in which V's rows
+// are loaded, so the weights become the second operand without leaving their
+// registers.  V's codes become fp16 by a byte permute, which puts the offset code
+// of two slots into the low bytes of two fp16 as multiples of 2^-24, and one fused
+// multiply-add, which takes the offset off: exact.  A weight, times its slot's
+// scale of V against the largest so far, is held in two fp16 (2^-22 of it, or 2^-40
+// of the largest); sums, maxima and outputs are fp32.
+template <typename IO, int DP, int NT>
+__global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
+    constexpr int NJ = DP / 64;                   // steps of the first product over the dims
+    constexpr int CH = DP / 16;                   // adjacent dims of V a lane
+    constexpr int VW = CH / 4;                    // and their dwords
+    constexpr int LPR = NJ == 1 ? 4 : NJ == 2 ? 8 : 16;  // lanes that make a row's digits
+    constexpr int OS = DP + 4;                    // floats of an output row in LDS: rows start in different banks
+    constexpr int kRows = 16 * NT;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // digits [3][NT][NJ][64 lanes] of 16 bytes; later the outputs
+    __shared__ float row_scale[kRows];
+    __shared__ float sm[4][kRows], sl[4][kRows], sf[4];
+    typedef uint32_t vch_t __attribute__((ext_vector_type(VW)));
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int kvh = static_cast<int>(blockIdx.x) % a.c.n_head_kv;
+    const int64_t b = static_cast<int64_t>(blockIdx.x) / a.c.n_head_kv;
+    const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
+    const int split = blockIdx.z, first_slot = split * a.turns * kTurn;
+    // Lane l of wavefront w stands for slot 32 (w + 4 (l / 32)) + l % 32 of a turn:
+    // the wavefront's own tiles, whose pages, scales and visible slots stay in its
+    // registers.  A turn's page ids are read without waiting for the length.
+    const int mine = 32 * (wave + 4 * (lane >> 5)) + (lane & 31);
+    const int32_t *const pages = a.c.pages + b * a.c.max_pages;
+    auto page_at = [&](int j) { return j < a.r.max_len ? pages[j >> a.c.page_shift] : -1; };
+    int32_t id = page_at(first_slot + mine);
+    const SeqRows s = seq_rows(a.r, b);
+    const int R = s.count * G, row0 = static_cast<int>(blockIdx.y) * kRows;
+    if (row0 >= R) return;  // whole workgroup
+    const int before = s.n - s.count;  // slots ahead of the new rows
+    const int at_min = before + row0 / G, at_max = before + (min(row0 + kRows, R) - 1) / G;
+    const int split_end = min(first_slot + a.turns * kTurn, s.n);
+    const bool whole = s.n <= a.turns * kTurn;  // the sequence's only split
+    if (whole ? split > 0 : !sees(a, at_max, first_slot, split_end) && !sees(a, at_min, first_slot, split_end)) return;
+    const int end = min(split_end, at_max + 1);  // the slots taken are first_slot .. end - 1, of those that are seen
+
+    int32_t page = 0;   // held to 0 .. n_pages - 1: a hole's rows are read (of a page that is there), never used
+    float k_sc = 0.f, v_sc = 0.f;
+    uint64_t bits = 0;  // the turn's slots that some row sees
+    auto look = [&](int j) {  // of slot j, whose page id is `id`
+        bool seen = id >= 0 && id < a.c.n_pages && j < end && (!a.window || j > at_min - a.window || j < a.sinks);
+        if (seen && a.mask) seen = a.mask[b * a.mask_stride + j] != 0;
+        page = id >= 0 && id < a.c.n_pages ? id : 0;
+        bits = __ballot(seen);
+        // a tile of 16 slots lies in one block, whose scales all of its lanes read
+        const uint32_t tile = static_cast<uint32_t>(bits >> (lane & 48)) & 0xffffu;
+        k_sc = v_sc = 0.f;
+        if (tile) {
+            const int64_t i = kv8_scale(a.c, page, j & ((1 << a.c.page_shift) - 1), kvh);
+            const float x = a.c.k_scale[i], y = a.c.v_scale[i];
+            k_sc = x >= 0.f && x < INFINITY ? x : NAN;
+            v_sc = y >= 0.f && y < INFINITY ? y : NAN;
         }
-        const int t = j & ((1 << a.c.page_shift) - 1);
-        float sc = -INFINITY;
-        if (seen) {
-            const int8_t *k = a.c.k + kv8_row(a.c, page, t) + kvh * a.c.head_stride;
-            float x = 0.f;
-            for (int e = 0; e < d; ++e) x += load1(q, e) * static_cast<float>(k[e]);
-            sc = x * a.c.k_scale[kv8_scale(a.c, page, t, kvh)] * a.scale;
+    };
+    const int8_t *const kp = a.c.k + kvh * a.c.head_stride, *const vp = a.c.v + kvh * a.c.head_stride;
+    const uint32_t row_bytes = static_cast<uint32_t>(a.c.token_stride);
+    u32x4_t kf[2][NJ];  // K: slot r, dims 16 (4 j + g) .. + 15 of either tile
+    vch_t vf[2][4];     // V: slot 4 g + i, dims CH r .. + CH - 1
+    // 16 slots from a multiple of 16 stay in their page and block, so that every row
+    // that is read is a row of the pool.  Where a tile has nothing that is seen one
+    // line is read over and over, so that the loads in flight can be counted.
+    auto row_of = [&](int j, int k, int u) {
+        return static_cast<int64_t>(__builtin_amdgcn_readlane(page, 32 * k + 16 * u)) * a.c.page_stride +
+               static_cast<int64_t>((j + 16 * u) & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
+    };
+    auto load_k = [&](int j, int k, bool there) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int8_t *base = kp + (there ? row_of(j, k, u) : 0);
+            const uint32_t off = static_cast<uint32_t>(in_loop(r)) * (there ? row_bytes : 0u);
+#pragma unroll
+            for (int i = 0; i < NJ; ++i)
+                kf[u][i] = *reinterpret_cast<const u32x4_t *>(base + (off + static_cast<uint32_t>(min(16 * (4 * i + g), d - 16))));
         }
-        const uint64_t any = __ballot(seen);
-        float top = sc;
-        for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, xor_shfl(top, off));
-        const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, corr = expf(m - ref);
-        m = mn;
-        const float p = seen ? expf(sc - ref) : 0.f;
-        float sum = p;
-        for (int off = 32; off >= 1; off >>= 1) sum += xor_shfl(sum, off);
-        l = l * corr + sum;
-        for (int e = 0; e < 4; ++e) o[e] *= corr;
-        for (int u = 0; u < 64; ++u) {
-            if (!((any >> u) & 1)) continue;
-            const int pg = __shfl(page, u, 64), tu = (j0 + u) & ((1 << a.c.page_shift) - 1);
-            const float w = __shfl(p, u, 64) * a.c.v_scale[kv8_scale(a.c, pg, tu, kvh)];
-            const int8_t *v = a.c.v + kv8_row(a.c, pg, tu) + kvh * a.c.head_stride;
-            for (int e = 0; e < 4; ++e)
-                if (lane + 64 * e < d) o[e] += w * static_cast<float>(v[lane + 64 * e]);
+    };
+    auto load_v = [&](int j, int k, bool there) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int8_t *base = vp + (there ? row_of(j, k, u) : 0);
+            const uint32_t step = there ? row_bytes : 0u, off = 4 * static_cast<uint32_t>(in_loop(g)) * step;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                vf[u][i] = *reinterpret_cast<const vch_t *>(base + static_cast<uint64_t>(i) * step + (off + static_cast<uint32_t>(min(CH * r, d - CH))));
+        }
+    };
+    auto tile_bits = [&](int k) { return static_cast<uint32_t>(bits >> (32 * k)); };
+    look(first_slot + mine);
+    {
+        const int j = first_slot + 32 * wave;
+        load_k(j, 0, tile_bits(0) != 0);
+        load_v(j, 0, tile_bits(0) != 0);
+    }
+
+    // The rows' digits: lane group LPR a row, 16 dims a lane.  A negative scale
+    // goes into their sign, so that a row's largest score is that of its largest sum.
+    const bool negative = a.scale < 0.f;
+    for (int i = tid; i < kRows * LPR; i += 256) {
+        const int row = i / LPR, ch = i % LPR, rho = row0 + row;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
+        if (rho < R && 16 * ch < d)
+            load16(static_cast<const IO *>(a.q) + (s.first + rho / G) * a.q_stride + static_cast<int64_t>(kvh * G + rho % G) * d + 16 * ch, x);
+        uint32_t top = 0;  // magnitudes order as their bits do, NaN above infinity
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+        for (int off = LPR / 2; off >= 1; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, LPR)));
+        // the smallest power of two with max <= 127 65536 2^e (a row below 2^-94 takes 2^-117)
+        const int ex = max(static_cast<int>(top >> 23) - ((top & 0x7fffffu) <= 0x7e0000u ? 6 : 5), 26) - 127 - 16;
+        if (ch == 0) row_scale[row] = top >= 0x7f800000u ? NAN : ldexpf(fabsf(a.scale) * 1.4426950408889634f, ex);
+        if (ch < 4 * NJ) {
+            u32x4_t dg[3];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t p0 = 0, p1 = 0, p2 = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    int v = static_cast<int>(rintf(ldexpf(x[4 * w + e], -ex)));
+                    if (negative) v = -v;
+                    const int c0 = static_cast<int8_t>(v), v1 = (v - c0) >> 8, c1 = static_cast<int8_t>(v1), c2 = (v1 - c1) >> 8;
+                    p0 |= (static_cast<uint32_t>(c0) & 0xffu) << (8 * e);
+                    p1 |= (static_cast<uint32_t>(c1) & 0xffu) << (8 * e);
+                    p2 |= (static_cast<uint32_t>(c2) & 0xffu) << (8 * e);
+                }
+                dg[0][w] = p0, dg[1][w] = p1, dg[2][w] = p2;
+            }
+            const int to = ((row >> 4) * NJ + (ch >> 2)) * 64 + 16 * (ch & 3) + (row & 15);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) reinterpret_cast<u32x4_t *>(lds)[k * NT * NJ * 64 + to] = dg[k];
         }
     }
-    for (int e = 0; e < 4; ++e) {
-        const int dim = lane + 64 * e;
-        if (dim >= d) break;
-        float x = l == 0.f ? 0.f : o[e] / l;
-        if (a.gate) x *= 1.0f / (1.0f + expf(-load1(static_cast<const IO *>(a.gate), row * a.q_stride + static_cast<int64_t>(h) * d + dim)));
-        store1(static_cast<IO *>(a.out), row * a.out_stride + static_cast<int64_t>(h) * d + dim, x);
+    __syncthreads();
+
+    f32x4_t o[NT][CH];  // o[t][e][i]: dim CH (4 g + i) + e of row r of tile t
+    float m[NT], l[NT], qs[NT];
+    int at[NT];  // the row's own slot; -1 past the last row
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int rho = row0 + 16 * t + r;
+        at[t] = rho < R ? before + rho / G : -1;
+        m[t] = -INFINITY, l[t] = 0.f, qs[t] = row_scale[16 * t + r];
+#pragma unroll
+        for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    if (lane == 0 && a.lse) a.lse[row * a.n_head + h] = l == 0.f ? -INFINITY : m + logf(l);
+    float v_top = 0.f;  // the largest scale of V so far; outputs are in units of it (times 2^6)
+    const int turns = (end - first_slot + kTurn - 1) / kTurn;
+    for (int turn = 0; turn < turns; ++turn) {
+        const int t0 = first_slot + turn * kTurn;
+        if (turn + 1 < turns) id = page_at(t0 + kTurn + mine);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int j = t0 + 32 * (wave + 4 * k);
+            const uint32_t now = tile_bits(k);
+            const float ks[2] = {lane_float(k_sc, 32 * k), lane_float(k_sc, 32 * k + 16)};
+            const float vs[2] = {lane_float(v_sc, 32 * k), lane_float(v_sc, 32 * k + 16)};
+            const bool all = now == 0xffffffffu && j + 31 <= at_min && (!a.window || j > at_max - a.window || j + 31 < a.sinks);
+            u32x4_t ph[NT], pl[NT];  // the weights' two operands
+            float grown = 1.f;
+            if (now) {
+                const float top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
+                grown = top == v_top ? 1.f : v_top / top;
+                v_top = top;
+                const float f[2] = {v_top > 0.f ? vs[0] / v_top * 32768.f : vs[0], v_top > 0.f ? vs[1] / v_top * 32768.f : vs[1]};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float sum[2][4];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        i32x4_t hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+                        const u32x4_t *dg = reinterpret_cast<const u32x4_t *>(lds) + t * NJ * 64 + (NT > 1 ? in_loop(lane) : lane);
+#pragma unroll
+                        for (int i = 0; i < NJ; ++i)
+                            hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, kf[u][i]),
+                                                                       __builtin_bit_cast(i32x4_t, dg[2 * NT * NJ * 64 + i * 64]), hi, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < NJ; ++i)
+                            lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, kf[u][i]),
+                                                                       __builtin_bit_cast(i32x4_t, dg[i * 64]), lo, 0, 0, 0);
+                        hi = hi << 8;  // below 2^31: 256 dims of 127 128
+#pragma unroll
+                        for (int i = 0; i < NJ; ++i)
+                            hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, kf[u][i]),
+                                                                       __builtin_bit_cast(i32x4_t, dg[NT * NJ * 64 + i * 64]), hi, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sum[u][i] = __builtin_fmaf(static_cast<float>(hi[i]), 256.f, static_cast<float>(lo[i]));
+                    }
+                    const float kq[2] = {qs[t] * ks[0], qs[t] * ks[1]};
+                    bool vis[2][4];
+                    float top_s = -INFINITY;
+                    if (all) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            top_s = fmaxf(top_s, kq[u] * fmaxf(fmaxf(sum[u][0], sum[u][1]), fmaxf(sum[u][2], sum[u][3])));
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int jj = j + 16 * u + 4 * g + i;
+                                vis[u][i] = (now >> (16 * u + 4 * g + i) & 1) && jj <= at[t] && (!a.window || jj > at[t] - a.window || jj < a.sinks);
+                                if (vis[u][i]) top_s = fmaxf(top_s, kq[u] * sum[u][i]);
+                            }
+                    }
+                    const float mn = fmaxf(m[t], quad_max(top_s));
+                    const float ref = mn == -INFINITY ? 0.f : mn;  // no finite score yet: avoid inf - inf
+                    const float corr = __builtin_amdgcn_exp2f(m[t] - ref);
+                    m[t] = mn;
+                    float ps = 0.f;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sum[u][i], kq[u], -ref));
+                            if (!all && !vis[u][i]) p[i] = 0.f;
+                            ps += p[i];
+                            p[i] *= f[u];
+                            if (!all && !vis[u][i]) p[i] = 0.f;  // whatever the scale of a slot that is not seen
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const f16x2_t h = __builtin_convertvector(f32x2_t{p[2 * i], p[2 * i + 1]}, f16x2_t);
+                            const f16x2_t w = __builtin_convertvector(
+                                f32x2_t{p[2 * i] - static_cast<float>(h[0]), p[2 * i + 1] - static_cast<float>(h[1])}, f16x2_t);
+                            ph[t][2 * u + i] = __builtin_bit_cast(uint32_t, h);
+                            pl[t][2 * u + i] = __builtin_bit_cast(uint32_t, w);
+                        }
+                    }
+                    l[t] = l[t] * corr + quad_sum(ps);
+                    const float back = corr * grown;
+                    if (!__all(back == 1.0f)) {
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) o[t][e] *= back;
+                    }
+                }
+            }
+            // K's registers are free: the next tile's rows
+            if (k == 0) {
+                load_k(j + 128, 1, tile_bits(1) != 0);
+            } else {
+                look(t0 + kTurn + mine);  // past the last turn nothing is seen
+                load_k(j + 128, 0, tile_bits(0) != 0);
+            }
+            if (now) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vf[u][i] ^= vch_t(0x80808080u);  // code + 128
+#pragma unroll
+                for (int e = 0; e < CH; ++e) {
+                    u32x4_t w;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t two = __builtin_amdgcn_perm(vf[u][2 * i + 1][e / 4], vf[u][2 * i][e / 4],
+                                                                       0x0c040c00u + 0x00010001u * static_cast<uint32_t>(e % 4));
+                            // (c + 128) 2^-24 2^15 - 128 2^-9 = c 2^-9
+                            const f16x2_t c = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, two), f16x2_t{32768.f16, 32768.f16},
+                                                                        f16x2_t{-0.25f16, -0.25f16});
+                            w[2 * u + i] = __builtin_bit_cast(uint32_t, c);
+                        }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, ph[t]), o[t][e], 0, 0, 0);
+                        o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, pl[t]), o[t][e], 0, 0, 0);
+                    }
+                }
+            }
+            load_v(j + 128, 1 - k, tile_bits(1 - k) != 0);
+        }
+    }
+
+    // the four wavefronts' outputs joined, kJoin rows at a time
+    if (g == 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sm[wave][16 * t + r] = m[t], sl[wave][16 * t + r] = l[t];
+    if (lane == 0) sf[wave] = v_top * 0.015625f;
+    float *const ob = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int q0 = 16 * t + kJoin * half;
+            if (row0 + q0 >= R) continue;  // whole workgroup
+            __syncthreads();  // the digits, or the rows before, have been read
+            if (r / kJoin == half) {
+                float *row = ob + (wave * kJoin + r % kJoin) * OS + 4 * g;
+#pragma unroll
+                for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * e) = o[t][e];
+            }
+            __syncthreads();
+            for (int i = tid; i < kJoin * DP; i += 256) {
+                const int q = q0 + i / DP, dim = i % DP, rho = row0 + q;
+                if (dim >= d || rho >= R) continue;
+                const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
+                float L = 0.f, x = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
+                    L += f * sl[w][q];
+                    x += f * sf[w] * ob[(w * kJoin + q - q0) * OS + dim % CH * 16 + dim / CH];
+                }
+                const int64_t row = s.first + rho / G;
+                const int h = kvh * G + rho % G;
+                if (whole) {
+                    store_out<IO>(a, row, h, dim, L == 0.f ? 0.f : x / L);
+                    if (dim == 0) store_lse(a, row, h, M, L);
+                } else {
+                    const int64_t rec = (row * a.n_head + h) * a.n_split + split;
+                    if (dim == 0) a.ml[rec] = make_float2(M, L);
+                    a.part[rec * d + dim] = x;
+                }
+            }
+        }
+}
+
+// The splits of a row and head joined by NG groups of DP / 4 lanes, each with
+// every NG-th split and four dims a lane; 256 / (NG DP / 4) heads a workgroup.
+template <typename IO, int DP, int NG>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
+    constexpr int DL = DP / 4, PER = 256 / (NG * DL);
+    __shared__ f32x4_t red[256];
+    __shared__ float2 rml[256];
+    const int tid = threadIdx.x, who = tid / (NG * DL), grp = tid / DL % NG, dim = 4 * (tid % DL);
+    const int64_t b = blockIdx.z;
+    const SeqRows s = seq_rows(a.r, b);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * PER + who;  // row of the sequence, head
+    const int i = static_cast<int>(item / a.n_head), h = static_cast<int>(item % a.n_head);
+    const int slots = a.turns * kTurn;
+    if (s.n <= slots) return;  // its only split wrote it
+    const bool live = who < PER && i < s.count;
+    if (PER == 1 && !live) return;  // whole workgroup
+    const int at = s.n - s.count + i, d = a.c.d;
+    const int64_t row = s.first + i, rec = (row * a.n_head + h) * a.n_split;
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f;
+    if (live)
+        for (int sp = grp; sp * slots <= at; sp += NG) {
+            if (!sees(a, at, sp * slots, min((sp + 1) * slots, s.n))) continue;
+            const float2 ml = a.ml[rec + sp];
+            const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+            const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml.x - ref);
+            L = L * f + ml.y * w;
+            if (dim < d) x = x * f + w * *reinterpret_cast<const f32x4_t *>(a.part + (rec + sp) * d + dim);
+            M = mn;
+        }
+    if constexpr (NG > 1) {
+        red[tid] = x;
+        rml[tid] = make_float2(M, L);
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int k = 1; k < NG; ++k) {
+            const float2 ml = rml[tid + k * DL];
+            const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+            const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml.x - ref);
+            L = L * f + ml.y * w;
+            x = x * f + w * red[tid + k * DL];
+            M = mn;
+        }
+    }
+    if (!live || dim >= d) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, L == 0.f ? 0.f : x[e] / L);
+    if (dim == 0) store_lse(a, row, h, M, L);
+}
+
+template <typename IO, int DP, int NT>
+int launch_attend(const Attend8Args &a, size_t seqs, hipStream_t s) {
+    constexpr size_t digits = 3 * NT * (DP / 64) * 1024, outputs = 4 * kJoin * (DP + 4) * sizeof(float);
+    constexpr size_t lds = digits > outputs ? digits : outputs;
+    static_assert(lds + 4096 <= 65536, "more LDS than a launch gets unasked");
+    const int64_t rows = static_cast<int64_t>(a.r.max_new) * (a.n_head / a.c.n_head_kv);
+    const dim3 grid(static_cast<unsigned>(seqs * static_cast<size_t>(a.c.n_head_kv)), static_cast<unsigned>((rows + 16 * NT - 1) / (16 * NT)),
+                    static_cast<unsigned>(a.n_split));
+    hipLaunchKernelGGL((kv8_attend_kernel<IO, DP, NT>), grid, dim3(256), lds, s, a);
+    int st = check_launch("kv8_attend_kernel");
+    if (st || a.n_split == 1) return st;
+    const int64_t heads = static_cast<int64_t>(a.r.max_new) * a.n_head;
+    constexpr int DL = DP / 4, kMost = DL <= 64 ? 256 / DL : 1;
+    if (a.n_split > 4) {
+        hipLaunchKernelGGL((kv8_join_kernel<IO, DP, kMost>), dim3(static_cast<unsigned>(heads), 1, static_cast<unsigned>(seqs)), dim3(256), 0, s, a);
+    } else {
+        constexpr int PER = 256 / DL;
+        hipLaunchKernelGGL((kv8_join_kernel<IO, DP, 1>), dim3(static_cast<unsigned>((heads + PER - 1) / PER), 1, static_cast<unsigned>(seqs)),
+                           dim3(256), 0, s, a);
+    }
+    return check_launch("kv8_join_kernel");
+}
+
+// The dims of a lane of V must divide the head: 192 only for its multiples of 12.
+int padded(size_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 && d % 12 == 0 ? 192 : 256; }
+// Tiles of 16 rows of a workgroup.
+int tiles_of(int64_t rows, int dp) { return rows <= 16 ? 1 : rows <= 32 || dp > 128 ? 2 : 4; }
+// Turns of 256 slots of a split: one where a sequence's rows are few and the splits
+// must fill the chip, more where many rows do; at most 1024 splits.
+int turns_of(int64_t rows, int nt, size_t max_len) {
+    int turns = rows <= 16 ? 1 : rows <= 16 * nt ? 2 : 16;
+    while ((max_len + static_cast<size_t>(turns) * kTurn - 1) / (static_cast<size_t>(turns) * kTurn) > 1024) turns *= 2;
+    return turns;
+}
+struct Attend8Ws {
+    int n_split, turns, tiles;
+    size_t part, bytes;
+};
+Attend8Ws attend_ws(size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len) {
+    Attend8Ws w{};
+    // by the caller's max_new, whatever rows there are: a sequence alone goes the way that it goes with others
+    const int64_t of_one = n_head_kv ? static_cast<int64_t>((max_new < (1u << 24) ? max_new : 1u << 24) * (n_head / n_head_kv)) : 0;
+    w.tiles = tiles_of(of_one, padded(d));
+    w.turns = turns_of(of_one, w.tiles, max_len);
+    const size_t slots = static_cast<size_t>(w.turns) * kTurn;
+    w.n_split = max_len ? static_cast<int>((max_len + slots - 1) / slots) : 1;
+    if (w.n_split == 1) return w;
+    const size_t recs = rows * n_head * static_cast<size_t>(w.n_split);
+    w.part = (recs * sizeof(float2) + 255) & ~size_t{255};
+    w.bytes = w.part + recs * d * sizeof(float);
+    return w;
+}
+
+template <typename IO>
+int launch_attend(const Attend8Args &a, size_t seqs, int tiles, hipStream_t s) {
+    const int dp = padded(static_cast<size_t>(a.c.d));
+    if (dp == 64) return tiles == 1 ? launch_attend<IO, 64, 1>(a, seqs, s) : tiles == 2 ? launch_attend<IO, 64, 2>(a, seqs, s) : launch_attend<IO, 64, 4>(a, seqs, s);
+    if (dp == 128) return tiles == 1 ? launch_attend<IO, 128, 1>(a, seqs, s) : tiles == 2 ? launch_attend<IO, 128, 2>(a, seqs, s) : launch_attend<IO, 128, 4>(a, seqs, s);
+    if (dp == 192) return tiles == 1 ? launch_attend<IO, 192, 1>(a, seqs, s) : launch_attend<IO, 192, 2>(a, seqs, s);
+    return tiles == 1 ? launch_attend<IO, 256, 1>(a, seqs, s) : launch_attend<IO, 256, 2>(a, seqs, s);
 }
 
 }  // namespace
@@ -101,7 +566,9 @@ using namespace ouro;
 
 extern "C" {
 
-size_t ouro_kv8_attend_workspace_bytes(size_t, size_t, size_t, size_t, size_t, size_t, size_t) { return 0; }
+size_t ouro_kv8_attend_workspace_bytes(size_t, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t head_dim, size_t max_len) {
+    return attend_ws(rows, max_new, n_head, n_head_kv, head_dim, max_len).bytes;
+}
 
 int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride, const int32_t *lens, const int32_t *cu,
                     const uint8_t *mask, size_t mask_stride, const void *gate, void *out, size_t out_stride, float *lse, int dtype,
@@ -130,19 +597,23 @@ int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(gate)) & 15 ||
         q_stride % unit || out_stride % unit)
         return fail(OURO_ERR_ALIGN, "%s: rows must start at multiples of 16 bytes", me);
-    if (!seqs || !(max_new = static_cast<size_t>(a.r.max_new))) return OURO_OK;
+    if (!seqs || !a.r.max_new) return OURO_OK;
     auto most = [](size_t x) { return static_cast<int32_t>(x < (1u << 30) ? x : 1u << 30); };
     a.q = q, a.gate = gate, a.mask = mask, a.out = out, a.lse = lse;
     a.q_stride = static_cast<int64_t>(q_stride), a.out_stride = static_cast<int64_t>(out_stride);
     a.mask_stride = static_cast<int64_t>(mask_stride);
     a.n_head = static_cast<int>(n_head), a.window = most(window), a.sinks = most(sinks), a.scale = scale;
-    (void)ws;
-    const dim3 grid(static_cast<unsigned>(max_new), static_cast<unsigned>(n_head), static_cast<unsigned>(seqs));
-    if (dtype == OURO_DT_F32)
-        hipLaunchKernelGGL(kv8_attend_kernel<float>, grid, dim3(64), 0, as_stream(stream), a);
-    else
-        hipLaunchKernelGGL(kv8_attend_kernel<uint16_t>, grid, dim3(64), 0, as_stream(stream), a);
-    return check_launch("kv8_attend_kernel");
+    const Attend8Ws w = attend_ws(rows, max_new, n_head, hkv, d, max_len);
+    a.n_split = w.n_split, a.turns = w.turns;
+    const size_t most_new = static_cast<size_t>(a.r.max_new);
+    if (seqs * hkv >= (1u << 24) || most_new * (n_head / hkv) > (1u << 20) || most_new * n_head >= (1u << 24))
+        return fail(OURO_ERR_SHAPE, "%s: %zu rows of one sequence of %zu heads, %zu sequences", me, most_new, n_head, seqs);
+    if (w.bytes) {
+        if (!ws && !(ws = workspace(w.bytes, stream))) return OURO_ERR_HIP;
+        a.ml = static_cast<float2 *>(ws);
+        a.part = reinterpret_cast<float *>(static_cast<unsigned char *>(ws) + w.part);
+    }
+    return dtype == OURO_DT_F32 ? launch_attend<float>(a, seqs, w.tiles, as_stream(stream)) : launch_attend<uint16_t>(a, seqs, w.tiles, as_stream(stream));
 }
 
 }  // extern "C"
