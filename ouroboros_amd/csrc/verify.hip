@@ -19,18 +19,31 @@
 namespace ouro {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kLogits = 32;  // logits of a thread
-constexpr int kPartLogits = kThreads * kLogits;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kSegLogits = 2048;  // logits of a segment: 32 a lane of a wavefront
 constexpr double kLog2e = 1.4426950408889634;
 
-// Sum of e^((x - m) / T) and the argmax (key) of a part of a row.
-struct Part {
+// Maximum, its lowest index and the sum of e^((x - m) / T) of a segment of a row.
+struct Seg {
     double sum;
     float m;
     uint32_t at;
 };
-static_assert(sizeof(Part) == 16, "Part: workspace layout");
+static_assert(sizeof(Seg) == 16, "Seg: workspace layout");
+
+// A row's, brought together.
+struct Sums {
+    double z;
+    float m;
+    uint32_t at;
+};
+// What a sequence came to: its deciding row (relative), whether that refused its
+// token, the row's sums of p and q, the token (-1: none in the vocabulary).
+struct Verdict {
+    Sums p, q;
+    int32_t row, refused, token, pad;
+};
+static_assert(sizeof(Verdict) == 48, "Verdict: workspace layout");
 
 struct VerifyArgs {
     NewRows r;
@@ -39,52 +52,82 @@ struct VerifyArgs {
     const int32_t *tokens, *lens;
     const float *temperature, *u_accept, *u_next;
     int32_t *accepted, *next, *lens_out;
-    Part *part;        // [2][rows][parts]
-    double *left;      // [seqs][parts]: sums of max(p - q, 0)
-    int32_t n, parts;
+    Seg *seg;          // [2][rows][segs]
+    double *left;      // [seqs][segs]: sums of max(p - q, 0)
+    Verdict *verdict;  // [seqs], NULL where the last launch judges the rows itself
+    int32_t n, segs;
 };
-static_assert(sizeof(VerifyArgs) == 152, "VerifyArgs: kernel argument layout");
+static_assert(sizeof(VerifyArgs) == 160, "VerifyArgs: kernel argument layout");
 
-// 2^y for y <= 0: y = k + f, |f| <= 1/2, 2^f by its Taylor series, whose first
-// term left out is (f ln 2)^12 / 12! <= 7e-15.  Below 2^-1000 it is 0, so that a
-// product of what is not 0 never is.
+// 2^y: y = k + f, |f| <= 1/2, and the polynomial of degree 8 that equals 2^f at
+// the nine Chebyshev points of [-1/2, 1/2], within 1.1e-12 of it between them
+// and 1 at 0.  Below 2^-1074, and for NaN, it is 0.
 __device__ __forceinline__ double exp2_64(double y) {
-    if (!(y > -1000.0)) return 0.0;
-    const double k = rint(y), z = (y - k) * 0.6931471805599453;
-    double s = 1.0 / 39916800;
-    s = fma(s, z, 1.0 / 3628800);
-    s = fma(s, z, 1.0 / 362880);
-    s = fma(s, z, 1.0 / 40320);
-    s = fma(s, z, 1.0 / 5040);
-    s = fma(s, z, 1.0 / 720);
-    s = fma(s, z, 1.0 / 120);
-    s = fma(s, z, 1.0 / 24);
-    s = fma(s, z, 1.0 / 6);
-    s = fma(s, z, 0.5);
-    s = fma(s, z, 1.0);
-    s = fma(s, z, 1.0);
+    y = fmax(y, -2000.0);
+    const double k = rint(y), f = y - k;
+    double s = 0x1.63d136366db24p-20;
+    s = fma(s, f, 0x1.00dc4a532fb8ep-16);
+    s = fma(s, f, 0x1.4308ac85aa947p-13);
+    s = fma(s, f, 0x1.5d8745a728441p-10);
+    s = fma(s, f, 0x1.3b2ab7181b755p-7);
+    s = fma(s, f, 0x1.c6b08dd6fd234p-5);
+    s = fma(s, f, 0x1.ebfbdff823cedp-3);
+    s = fma(s, f, 0x1.62e42fef84cf0p-1);
+    s = fma(s, f, 1.0);
     return __builtin_amdgcn_ldexp(s, static_cast<int>(k));
 }
-// e^((x - m) / T), c = log2 e / T, x <= m: 1 where x = m, infinite or not.
+// e^((x - m) / T), c = log2 e / T, x <= m: 1 where x = m, infinite or not, and 0
+// below 2^-1000, so that a product of what is not 0 never is.
 __device__ __forceinline__ double weight(float x, float m, double c) {
-    return x == m ? 1.0 : exp2_64((static_cast<double>(x) - static_cast<double>(m)) * c);
+    if (x == m) return 1.0;
+    const double y = (static_cast<double>(x) - static_cast<double>(m)) * c;
+    return y > -1000.0 ? exp2_64(y) : 0.0;
 }
-__device__ __forceinline__ double shfl_xor64(double v, int mask) {
+// Lane `lane`'s value, the same lane for all.
+__device__ __forceinline__ double lane64(double v, int lane) {
     const uint64_t u = __double_as_longlong(v);
-    const uint32_t lo = __shfl_xor(static_cast<uint32_t>(u), mask, 64), hi = __shfl_xor(static_cast<uint32_t>(u >> 32), mask, 64);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(u), lane), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(u >> 32), lane);
     return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += shfl_xor64(v, off);
-    return v;
+// v plus that of the lane that a data-parallel move names, 0 where it names none.
+template <int Ctrl, int Rows>
+__device__ __forceinline__ double plus_dpp(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u), Ctrl, Rows, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u >> 32), Ctrl, Rows, 0xf, false);
+    return v + __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+// Inclusive sums over a wavefront's lanes: over each row of 16 lanes by moves of 1,
+// 2, 4 and 8, then the last lane of rows 0 and 2 to rows 1 and 3, and lane 31 to
+// both of them.  (Lane exchanges through LDS instead: 0.5 us a sum.)
+__device__ __forceinline__ double wave_scan(double v) {
+    v = plus_dpp<0x111, 0xf>(v);
+    v = plus_dpp<0x112, 0xf>(v);
+    v = plus_dpp<0x114, 0xf>(v);
+    v = plus_dpp<0x118, 0xf>(v);
+    v = plus_dpp<0x142, 0xa>(v);
+    return plus_dpp<0x143, 0xc>(v);
+}
+__device__ __forceinline__ double wave_sum(double v) { return lane64(wave_scan(v), 63); }
+// Over the 64 lanes: within rows of 16 by moves, across them by swaps.
+template <typename F>
+__device__ __forceinline__ uint32_t wave_join(uint32_t v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false));
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return f(b[0], b[1]);
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, xor_shfl(v, off));
-    return v;
+    return __uint_as_float(wave_join(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
 }
-// Draws by likeliest token where the temperature is not above 0.
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+    return wave_join(v, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+// The likeliest token is taken where the temperature is not above 0.
 __device__ __forceinline__ float heat(const VerifyArgs &a, int64_t b) { return a.temperature ? a.temperature[b] : 1.f; }
 
 template <typename T>
@@ -92,158 +135,170 @@ __device__ __forceinline__ LogitRow<T> row_at(const VerifyArgs &a, int which, in
     return LogitRow<T>(static_cast<const T *>(a.x[which]) + row * a.stride[which], a.n);
 }
 
-// A part of a row: its maximum, the lowest index of it, the sum against it.
+// A segment by one wavefront: its maximum and, as the row is drawn from or not,
+// the sum against it or the maximum's lowest index.
 template <typename T>
-__device__ __forceinline__ void part_of(const VerifyArgs &a, int which, int64_t row, double c, Part *out) {
-    constexpr int VL = LogitRow<T>::VL, kVec = kLogits / VL;
-    __shared__ float top[kThreads / 64];
-    __shared__ double sums[kThreads / 64];
-    __shared__ uint32_t first[kThreads / 64];
-    const int tid = threadIdx.x, wave = tid >> 6;
+__device__ __forceinline__ void segment(const VerifyArgs &a, int which, int64_t row, int seg, float t, Seg *out) {
+    constexpr int VL = LogitRow<T>::VL, kVec = 32 / VL;
+    const int lane = threadIdx.x & 63;
     const LogitRow<T> x = row_at<T>(a, which, row);
-    const int q0 = static_cast<int>(blockIdx.x) * (kPartLogits / VL) + tid;
+    const int q0 = seg * (kSegLogits / VL) + lane;
     u32x4_t v[kVec];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] = x.load(q0 + k * kThreads);
+    for (int k = 0; k < kVec; ++k) v[k] = x.load(q0 + 64 * k);
     float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
 #pragma unroll
         for (int e = 0; e < VL; ++e) m = fmaxf(m, x.raw(v[k], e));  // passes over a NaN
     m = wave_max(m);
-    if ((tid & 63) == 0) top[wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, top[w]);
     double sum = 0.0;
     uint32_t at = 0xffffffffu;
-    if (m > -INFINITY) {
+    if (!(t > 0.f) && m > -INFINITY) {
 #pragma unroll
         for (int k = 0; k < kVec; ++k)
 #pragma unroll
-            for (int e = 0; e < VL; ++e) {
-                const float f = x.at(v[k], e);
-                if (c > 0.0) sum += weight(f, m, c);
-                if (f == m) at = min(at, static_cast<uint32_t>(x.first(q0 + k * kThreads) + e));
-            }
-    }
-    sum = wave_sum(sum);
+            for (int e = 0; e < VL; ++e)
+                if (x.raw(v[k], e) == m) at = min(at, static_cast<uint32_t>(x.first(q0 + 64 * k) + e));
+        at = wave_min(at);
+    } else if (m == INFINITY) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) at = min(at, static_cast<uint32_t>(xor_shfl(static_cast<int>(at), off)));
-    if ((tid & 63) == 0) sums[wave] = sum, first[wave] = at;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) sum += sums[w], at = min(at, first[w]);
-        *out = Part{sum, m, at};
+        for (int k = 0; k < kVec; ++k)
+#pragma unroll
+            for (int e = 0; e < VL; ++e) sum += x.raw(v[k], e) == m ? 1.0 : 0.0;
+        sum = wave_sum(sum);
+    } else if (m > -INFINITY) {
+        const double c = kLog2e / static_cast<double>(t), mc = -static_cast<double>(m) * c;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+#pragma unroll
+            for (int e = 0; e < VL; ++e) sum += exp2_64(fma(static_cast<double>(x.raw(v[k], e)), c, mc));
+        sum = wave_sum(sum);
     }
+    if (lane == 0) *out = Seg{sum, m, at};
 }
 
+// A wavefront a segment, of the target's rows and then of the drafter's.  No
+// barrier and no LDS: what a wavefront waits for is its 8 KiB of logits.
 template <typename T, typename D>
-__global__ __launch_bounds__(kThreads) void verify_part_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kThreads) void verify_segments_kernel(VerifyArgs a) {
     const int which = static_cast<int>(blockIdx.y) / a.r.max_new, i = static_cast<int>(blockIdx.y) % a.r.max_new;
+    const int seg = static_cast<int>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const SeqRows s = seq_rows(a.r, blockIdx.z);
-    if (i >= s.count - which) return;  // the last row has no token to judge
+    if (i >= s.count - which || seg >= a.segs) return;  // the last row has no token to judge
     const float t = heat(a, blockIdx.z);
-    const bool draws = t > 0.f;
-    if (which && !draws) return;
+    if (which && !(t > 0.f)) return;
     const int64_t row = s.first + i;
-    Part *out = a.part + (static_cast<int64_t>(which) * a.r.rows + row) * a.parts + blockIdx.x;
+    Seg *out = a.seg + (static_cast<int64_t>(which) * a.r.rows + row) * a.segs + seg;
     if (which)
-        part_of<D>(a, 1, row, kLog2e, out);
+        segment<D>(a, 1, row, seg, 1.f, out);
     else
-        part_of<T>(a, 0, row, draws ? kLog2e / static_cast<double>(t) : 0.0, out);
+        segment<T>(a, 0, row, seg, t, out);
 }
 
-// A row's maximum, sum and argmax by one wavefront, to each of its lanes.
-struct Sums {
-    double z;
-    float m;
-    uint32_t at;
-};
-__device__ __forceinline__ Sums join_parts(const VerifyArgs &a, int which, int64_t row, double c) {
-    const Part *p = a.part + (static_cast<int64_t>(which) * a.r.rows + row) * a.parts;
+// A row's segments brought together by one wavefront, to each of its lanes.
+__device__ __forceinline__ Sums join_segments(const VerifyArgs &a, int which, int64_t row, bool draws, double c) {
+    const Seg *p = a.seg + (static_cast<int64_t>(which) * a.r.rows + row) * a.segs;
     const int lane = threadIdx.x & 63;
+    constexpr int kHeld = 2;  // of a lane, that are read once
+    Seg held[kHeld];
     Sums s{0.0, -INFINITY, 0xffffffffu};
-    for (int i = lane; i < a.parts; i += 64) s.m = fmaxf(s.m, p[i].m);
-    s.m = wave_max(s.m);
-    for (int i = lane; i < a.parts; i += 64) {
-        const Part x = p[i];
-        if (x.m == -INFINITY) continue;
-        s.z += x.sum * weight(x.m, s.m, c);
-        if (x.m == s.m) s.at = min(s.at, x.at);
-    }
-    s.z = wave_sum(s.z);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) s.at = min(s.at, static_cast<uint32_t>(xor_shfl(static_cast<int>(s.at), off)));
+    for (int i = 0; i < kHeld; ++i) {
+        held[i] = Seg{0.0, -INFINITY, 0xffffffffu};
+        if (lane + 64 * i < a.segs) held[i] = p[lane + 64 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) s.m = fmaxf(s.m, held[i].m);
+    for (int i = lane + 64 * kHeld; i < a.segs; i += 64) s.m = fmaxf(s.m, p[i].m);
+    s.m = wave_max(s.m);
+    auto add = [&](const Seg &x) {
+        if (x.m == -INFINITY) return;
+        if (draws) s.z += x.sum * weight(x.m, s.m, c);
+        if (x.m == s.m) s.at = min(s.at, x.at);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) add(held[i]);
+    for (int i = lane + 64 * kHeld; i < a.segs; i += 64) add(p[i]);
+    if (draws)
+        s.z = wave_sum(s.z);
+    else
+        s.at = wave_min(s.at);
     return s;
 }
-
-// What a sequence came to: its deciding row (relative), whether that refused a
-// token, its sums of p and q, the token refused (-1: none in the vocabulary).
-struct Verdict {
-    Sums p, q;
-    int32_t row, refused, token, pad;
-};
 
 // The rows of a sequence judged, a wavefront each, up to the first that refuses.
 template <typename T, typename D>
 __device__ __forceinline__ Verdict decide(const VerifyArgs &a, const SeqRows &s, float t, Verdict *lds) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool draws = t > 0.f;
     const double c = draws ? kLog2e / static_cast<double>(t) : 0.0;
-    for (int i0 = 0; i0 < s.count; i0 += kThreads / 64) {
+    for (int i0 = 0; i0 < s.count; i0 += kWaves) {
         const int i = i0 + wave;
         if (i < s.count) {
             const int64_t row = s.first + i;
+            const bool judges = i + 1 < s.count;
+            const int next = judges ? a.tokens[row + 1] : -1;
+            const bool in = next >= 0 && next < a.n;
+            float x = -INFINITY, y = -INFINITY, u = 0.f;
+            if (in && draws) {  // on their way while the segments are joined
+                u = a.u_accept[row];
+                x = logit(row_at<T>(a, 0, row).x, next);
+                if (a.x[1]) y = logit(row_at<D>(a, 1, row).x, next);
+            }
             Verdict v{};
             v.row = i;
-            v.p = join_parts(a, 0, row, c);
-            v.token = -1;
-            if (i + 1 < s.count) {
-                const int next = a.tokens[row + 1];
-                const bool in = next >= 0 && next < a.n;
-                bool keep;
+            v.p = join_segments(a, 0, row, draws, c);
+            if (judges && draws && a.x[1]) v.q = join_segments(a, 1, row, true, kLog2e);
+            v.token = in ? next : -1;
+            if (judges) {
+                bool keep = in && v.p.m > -INFINITY;
                 if (!draws) {
-                    keep = in && v.p.m > -INFINITY && static_cast<uint32_t>(next) == v.p.at;
-                } else {
-                    double p = 0.0, q = 1.0;
-                    if (in && v.p.m > -INFINITY) p = weight(logit(row_at<T>(a, 0, row).x, next), v.p.m, c) / v.p.z;
-                    if (a.x[1]) {
-                        v.q = join_parts(a, 1, row, kLog2e);
-                        q = in && v.q.m > -INFINITY ? weight(logit(row_at<D>(a, 1, row).x, next), v.q.m, kLog2e) / v.q.z : 0.0;
-                    }
-                    keep = in && static_cast<double>(a.u_accept[row]) * q < p;
+                    keep = keep && static_cast<uint32_t>(next) == v.p.at;
+                } else if (keep) {
+                    const double q = !a.x[1] ? 1.0 : v.q.m > -INFINITY ? weight(y, v.q.m, kLog2e) / v.q.z : 0.0;
+                    keep = static_cast<double>(u) * q < weight(x, v.p.m, c) / v.p.z;
                 }
                 v.refused = !keep;
-                v.token = in ? next : -1;
             }
             if ((threadIdx.x & 63) == 0) lds[wave] = v;
         }
         __syncthreads();
-        for (int w = 0; w < kThreads / 64; ++w)
+        for (int w = 0; w < kWaves; ++w)
             if (i0 + w < s.count && (lds[w].refused || i0 + w + 1 == s.count)) return lds[w];
         __syncthreads();
     }
     return Verdict{};  // no rows: not reached
 }
 
-// What a token is drawn by, of a part of the deciding row: max(p - q, 0) where a
-// token was refused, p where none was or where nothing is left of it.
+// A distribution's values, e^((x - m) / T) / z.
+struct Share {
+    double c, mc, z;  // log2 e / T, -m c, 1 / z
+    float top;        // +inf where m is: the mass is that of the +inf logits, else NaN
+    __device__ __forceinline__ Share() {}
+    __device__ __forceinline__ Share(const Sums &s, double scale) : c(scale), mc(-static_cast<double>(s.m) * scale), z(1.0 / s.z), top(s.m == INFINITY ? INFINITY : NAN) {}
+    // Of a logit as it lies there: 0 for NaN and -inf.
+    __device__ __forceinline__ double of(float x) const {
+#pragma clang fp contract(off)
+        if (top == INFINITY) return x == top ? z : 0.0;
+        return exp2_64(__builtin_fma(static_cast<double>(x), c, mc)) * z;
+    }
+};
+
+// What a token is drawn by: max(p - q, 0) where one was refused, p where none was
+// or where nothing is left of it.
 template <typename T, typename D>
 struct Left {
-    static constexpr int VL = LogitRow<T>::VL, kVec = kLogits / VL;
+    static constexpr int VL = LogitRow<T>::VL;
     LogitRow<T> x;
     LogitRow<D> y;
-    double c, pz, qz;
-    float pm, qm;
+    Share p, q;
     int token;  // that a drafter without draft rows named, -1: none
     bool minus;
     __device__ __forceinline__ Left(const VerifyArgs &a, const SeqRows &s, const Verdict &v, float t, bool residual)
-        : x(row_at<T>(a, 0, s.first + v.row)), y(row_at<D>(a, a.x[1] ? 1 : 0, s.first + v.row)) {
-        c = kLog2e / static_cast<double>(t);
-        pm = v.p.m, pz = 1.0 / v.p.z;
-        qm = v.q.m, qz = 1.0 / v.q.z;
+        : x(row_at<T>(a, 0, s.first + v.row)), y(row_at<D>(a, a.x[1] ? 1 : 0, s.first + v.row)), p(v.p, kLog2e / static_cast<double>(t)) {
         minus = residual && a.x[1] && v.q.m > -INFINITY;
+        if (minus) q = Share(v.q, kLog2e);
         token = residual && !a.x[1] ? v.token : -1;
     }
     // The draft's values at the places of vector q of x.
@@ -251,7 +306,7 @@ struct Left {
         if (LogitRow<D>::VL == VL && x.shift == y.shift) {
             const u32x4_t v = y.load(q);
 #pragma unroll
-            for (int e = 0; e < VL; ++e) g[e] = y.at(v, e);
+            for (int e = 0; e < VL; ++e) g[e] = y.raw(v, e);
         } else {
 #pragma unroll
             for (int e = 0; e < VL; ++e) {
@@ -260,200 +315,199 @@ struct Left {
             }
         }
     }
-    // Of the elements of vector q; places outside the row have none.  The products
+    // Of the elements of vector at; places outside the row hold -inf.  Both products
     // are rounded before they are subtracted, so that equal p and q leave nothing.
-    __device__ __forceinline__ void weights(int q, double (&r)[VL]) const {
+    __device__ __forceinline__ void weights(int at, double (&r)[VL]) const {
 #pragma clang fp contract(off)
-        const u32x4_t v = x.load(q);
+        const u32x4_t v = x.load(at);
         float g[VL];
-        if (minus) beside(q, g);
+        if (minus) beside(at, g);
 #pragma unroll
         for (int e = 0; e < VL; ++e) {
-            const int i = x.first(q) + e;
-            r[e] = i >= 0 && i < x.n && i != token ? weight(x.at(v, e), pm, c) * pz : 0.0;
-            if (minus) r[e] = fmax(r[e] - weight(g[e], qm, kLog2e) * qz, 0.0);
+            r[e] = p.of(x.raw(v, e));
+            if (minus) r[e] = fmax(r[e] - q.of(g[e]), 0.0);
+            if (token >= 0 && x.first(at) + e == token) r[e] = 0.0;
         }
     }
-    // A thread's sums of a part, by vectors: those of all threads' k-th follow
-    // each other, then the k + 1-st.
-    __device__ __forceinline__ void sums(int part, double (&s)[kVec]) const {
+    // A lane's sum of vectors q, q + 64, ..
+    template <int N>
+    __device__ __forceinline__ double sum(int q) const {
+        double s = 0.0;
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) {
+        for (int k = 0; k < N; ++k) {
             double r[VL];
-            weights(part * (kPartLogits / VL) + k * kThreads + static_cast<int>(threadIdx.x), r);
-            s[k] = 0.0;
+            weights(q + 64 * k, r);
 #pragma unroll
-            for (int e = 0; e < VL; ++e) s[k] += r[e];
+            for (int e = 0; e < VL; ++e) s += r[e];
         }
+        return s;
     }
 };
 
-// A part's sum, to every thread; lds: a double of each wavefront.
-template <typename L>
-__device__ __forceinline__ double part_sum(const L &left, int part, double *lds) {
-    double s[L::kVec], sum = 0.0;
-    left.sums(part, s);
-#pragma unroll
-    for (int k = 0; k < L::kVec; ++k) sum += s[k];
-    sum = wave_sum(sum);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+__device__ __forceinline__ void say(const VerifyArgs &a, int64_t b, const SeqRows &s, int kept) {
+    a.accepted[b] = kept;
+    if (a.lens_out) a.lens_out[b] = a.lens[b] - (s.count ? s.count - 1 - kept : 0);
 }
 
-// Sums of max(p - q, 0) over the parts of a sequence's refusing row.
+// Every workgroup of a sequence judges its rows (all wait for the same few
+// kilobytes); where a token was refused each wavefront then sums max(p - q, 0)
+// over a segment of that row.  64 sequences of up to four drafted tokens over
+// 248320 logits, some 90 MB of refusing rows: 33 us; the judging in a launch of
+// its own 8 + 25 us and one launch more, two segments a wavefront 43.
 template <typename T, typename D>
 __global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a) {
-    __shared__ Verdict lds[kThreads / 64];
-    __shared__ double waves[kThreads / 64];
-    const SeqRows s = seq_rows(a.r, blockIdx.y);
-    const float t = heat(a, blockIdx.y);
-    if (s.count == 0 || !(t > 0.f)) return;
+    constexpr int VL = Left<T, D>::VL;
+    __shared__ Verdict lds[kWaves];
+    const int64_t b = blockIdx.y;
+    const SeqRows s = seq_rows(a.r, b);
+    const float t = heat(a, b);
+    if (s.count == 0) return;  // whole workgroup
     const Verdict v = decide<T, D>(a, s, t, lds);
-    if (!v.refused || v.p.m == -INFINITY) return;
-    const Left<T, D> left(a, s, v, t, true);
-    const double sum = part_sum(left, blockIdx.x, waves);
-    if (threadIdx.x == 0) a.left[static_cast<int64_t>(blockIdx.y) * a.parts + blockIdx.x] = sum;
-}
-
-// Inclusive sums over a wavefront's lanes.
-__device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint64_t u = __double_as_longlong(v);
-        const uint32_t lo = __shfl_up(static_cast<uint32_t>(u), off, 64), hi = __shfl_up(static_cast<uint32_t>(u >> 32), off, 64);
-        if (lane >= off) v += __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        a.verdict[b] = v;
+        say(a, b, s, v.row);
     }
-    return v;
+    const int seg = static_cast<int>(blockIdx.x) * kWaves + static_cast<int>(threadIdx.x >> 6);
+    if (!v.refused || !(t > 0.f) || v.p.m == -INFINITY || seg >= a.segs) return;
+    const Left<T, D> left(a, s, v, t, true);
+    const double sum = wave_sum(left.template sum<32 / VL>(seg * (kSegLogits / VL) + (threadIdx.x & 63)));
+    if ((threadIdx.x & 63) == 0) a.left[b * a.segs + seg] = sum;
 }
 
-// The next token of a sequence: the part in which the cumulative sum passes
-// u' of the whole, in it the wavefront's vectors, the lane, the element.  Sums that
+// The next token of a sequence: the segment in which the cumulative sum passes u'
+// of the whole, in it the wavefront's quarter, the lane, the element.  Sums that
 // are made in two orders differ by roundings: where none passes, the last with
 // any weight is taken, so that a token of weight 0 never is.
-constexpr int kMaxParts = ((1 << 24) + 7 + kPartLogits - 1) / kPartLogits;
 template <typename T, typename D>
 __global__ __launch_bounds__(kThreads) void verify_next_kernel(VerifyArgs a) {
     using L = Left<T, D>;
-    constexpr int kWaves = kThreads / 64, kSegs = L::kVec * kWaves;
+    constexpr int VL = L::VL, kQuarter = kSegLogits / kWaves / VL, kVec = kQuarter / 64;
     __shared__ Verdict lds[kWaves];
-    __shared__ double mass[kMaxParts], waves[kWaves], seg[kSegs];
-    __shared__ int chosen;
-    __shared__ double before;
+    __shared__ double part[kWaves * kVec];
     const int64_t b = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const SeqRows s = seq_rows(a.r, b);
     const float t = heat(a, b);
     Verdict v{};
-    if (s.count) v = decide<T, D>(a, s, t, lds);
-    if (tid == 0) {
-        a.accepted[b] = v.row;
-        if (a.lens_out) a.lens_out[b] = a.lens[b] - (s.count ? s.count - 1 - v.row : 0);
-    }
+    if (s.count) v = a.verdict ? a.verdict[b] : decide<T, D>(a, s, t, lds);
+    if (tid == 0 && (!a.verdict || !s.count)) say(a, b, s, v.row);
     if (!s.count || v.p.m == -INFINITY || !(t > 0.f)) {
         if (tid == 0) a.next[b] = !s.count || v.p.m == -INFINITY ? -1 : static_cast<int32_t>(v.p.at);
         return;
     }
-    const Part *const parts = a.part + (s.first + v.row) * static_cast<int64_t>(a.parts);
+    const Seg *const segs = a.seg + (s.first + v.row) * static_cast<int64_t>(a.segs);
     for (int residual = v.refused ? 1 : 0; residual >= 0; --residual) {
         const L left(a, s, v, t, residual != 0);
-        // the parts' weights: p's from the first pass, less a token that was named
-        for (int i = tid; i < a.parts; i += kThreads)
-            mass[i] = left.minus ? a.left[b * a.parts + i] : parts[i].m == -INFINITY ? 0.0 : parts[i].sum * weight(parts[i].m, v.p.m, left.c) * left.pz;
+        // the segment of a token that was named, without it
+        int named = -1;
+        double rest = 0.0;
         if (left.token >= 0) {
-            const int i = (left.token + left.x.shift) / kPartLogits;
-            const double m = part_sum(left, i, waves);
-            if (tid == 0) mass[i] = m;
-        }
-        __syncthreads();
-        if (wave == 0) {
-            double total = 0.0;
-            for (int i = lane; i < a.parts; i += 64) total += mass[i];
-            total = wave_sum(total);
-            const double want = static_cast<double>(a.u_next[b]) * total;
-            double cum = 0.0, at = 0.0;
-            int last = -1;
-            for (int i0 = 0; i0 < a.parts; i0 += 64) {
-                const double m = i0 + lane < a.parts ? mass[i0 + lane] : 0.0, end = cum + wave_scan(m);
-                const uint64_t has = __ballot(m > 0.0), past = __ballot(m > 0.0 && end > want);
-                if (has | past) {
-                    const int i = past ? __ffsll(static_cast<long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(has));
-                    last = i0 + i;
-                    at = __shfl(end, i, 64) - __shfl(m, i, 64);
-                    if (past) break;
-                }
-                cum = __shfl(end, 63, 64);
-            }
-            if (lane == 0) chosen = last, before = want - at;
-        }
-        __syncthreads();
-        const int part = chosen;
-        double want = before;
-        if (part < 0) {  // nothing left of p: drawn from p itself
+            named = (left.token + left.x.shift) / kSegLogits;
+            const double sum = wave_sum(left.template sum<kVec>(named * (kSegLogits / VL) + wave * kQuarter + lane));
+            if (lane == 0) part[wave] = sum;
             __syncthreads();
-            continue;
+            for (int w = 0; w < kWaves; ++w) rest += part[w];
+            __syncthreads();
         }
-        double sum[L::kVec];
-        left.sums(part, sum);
+        // the segments' weights: p's from the first pass
+        auto mass = [&](int i) {
+            if (i >= a.segs) return 0.0;
+            if (left.minus) return a.left[b * a.segs + i];
+            if (i == named) return rest;
+            const Seg x = segs[i];
+            return x.m == -INFINITY ? 0.0 : x.sum * weight(x.m, v.p.m, left.p.c) * left.p.z;
+        };
+        double total = 0.0, want, cum = 0.0, at = 0.0;
+        for (int i = lane; i < a.segs; i += 64) total += mass(i);
+        want = static_cast<double>(a.u_next[b]) * wave_sum(total);
+        int seg = -1;
+        for (int i0 = 0; i0 < a.segs; i0 += 64) {
+            const double m = mass(i0 + lane), end = cum + wave_scan(m);
+            const uint64_t has = __ballot(m > 0.0), past = __ballot(m > 0.0 && end > want);
+            if (has) {
+                const int i = past ? __ffsll(static_cast<long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(has));
+                seg = i0 + i;
+                at = lane64(end, i) - lane64(m, i);
+                if (past) break;
+            }
+            cum = lane64(end, 63);
+        }
+        if (seg < 0) continue;  // nothing left of p: drawn from p itself
+        want -= at;
+        const int q0 = seg * (kSegLogits / VL) + wave * kQuarter + lane;
+        double r[kVec][VL], mine[kVec];
 #pragma unroll
-        for (int k = 0; k < L::kVec; ++k) {
-            const double w = wave_sum(sum[k]);
-            if (lane == 0) seg[k * kWaves + wave] = w;
+        for (int k = 0; k < kVec; ++k) {
+            left.weights(q0 + 64 * k, r[k]);
+            mine[k] = 0.0;
+#pragma unroll
+            for (int e = 0; e < VL; ++e) mine[k] += r[k][e];
+            const double w = wave_sum(mine[k]);
+            if (lane == 0) part[wave * kVec + k] = w;
         }
         __syncthreads();
-        int at = -1;
+        int from = -1;
         bool passed = false;
-        double cum = 0.0, start = 0.0;
-        for (int i = 0; i < kSegs && !passed; ++i) {
-            if (seg[i] > 0.0) at = i, start = cum, passed = cum + seg[i] > want;
-            cum += seg[i];
+        cum = 0.0;
+        double start = 0.0;
+        for (int i = 0; i < kWaves * kVec && !passed; ++i) {
+            if (part[i] > 0.0) from = i, start = cum, passed = cum + part[i] > want;
+            cum += part[i];
         }
-        if (at % kWaves == wave) {
-            const int q = part * (kPartLogits / L::VL) + at / kWaves * kThreads + tid;
-            double r[L::VL], mine = 0.0;
-            left.weights(q, r);
 #pragma unroll
-            for (int e = 0; e < L::VL; ++e) mine += r[e];
-            const double end = start + wave_scan(mine);
-            const uint64_t has = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && end > want);
-            const int from = past ? __ffsll(static_cast<long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(has));
-            if (lane == from) {
-                double c2 = end - mine;
-                int token = -1;
-                bool done = false;
+        for (int k = 0; k < kVec; ++k)
+            if (from == wave * kVec + k) {
+                const double end = start + wave_scan(mine[k]);
+                const uint64_t has = __ballot(mine[k] > 0.0), past = __ballot(mine[k] > 0.0 && end > want);
+                const int who = past ? __ffsll(static_cast<long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(has));
+                if (lane == who) {
+                    double c2 = end - mine[k];
+                    int token = -1;
+                    bool done = false;
 #pragma unroll
-                for (int e = 0; e < L::VL; ++e) {
-                    c2 += r[e];
-                    if (!done && r[e] > 0.0) token = left.x.first(q) + e, done = c2 > want;
+                    for (int e = 0; e < VL; ++e) {
+                        c2 += r[k][e];
+                        if (!done && r[k][e] > 0.0) token = left.x.first(q0 + 64 * k) + e, done = c2 > want;
+                    }
+                    a.next[b] = token;
                 }
-                a.next[b] = token;
             }
-        }
         return;
     }
 }
 
 template <typename T, typename D>
-int launch_verify(const VerifyArgs &a, unsigned seqs, hipStream_t s) {
+int launch_verify(VerifyArgs a, unsigned seqs, hipStream_t s) {
+    const unsigned groups = static_cast<unsigned>((a.segs + kWaves - 1) / kWaves);
     int st = OURO_OK;
     if (a.r.max_new) {
-        hipLaunchKernelGGL((verify_part_kernel<T, D>), dim3(a.parts, (a.x[1] ? 2 : 1) * a.r.max_new, seqs), dim3(kThreads), 0, s, a);
-        if ((st = check_launch("verify_part_kernel"))) return st;
+        hipLaunchKernelGGL((verify_segments_kernel<T, D>), dim3(groups, (a.x[1] ? 2 : 1) * a.r.max_new, seqs), dim3(kThreads), 0, s, a);
+        if ((st = check_launch("verify_segments_kernel"))) return st;
     }
     if (a.x[1] && a.r.max_new > 1) {
-        hipLaunchKernelGGL((verify_left_kernel<T, D>), dim3(a.parts, seqs), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((verify_left_kernel<T, D>), dim3(groups, seqs), dim3(kThreads), 0, s, a);
         if ((st = check_launch("verify_left_kernel"))) return st;
+    } else {
+        a.verdict = nullptr;
     }
     hipLaunchKernelGGL((verify_next_kernel<T, D>), dim3(seqs), dim3(kThreads), 0, s, a);
     return check_launch("verify_next_kernel");
 }
 
-// A part's logits begin at a multiple of 16 bytes, before the row's first where
+// A row's segments begin at a multiple of 16 bytes, before its first logit where
 // that is not one: up to 7 places more than the row has.
-size_t parts_of(size_t n) { return (n + 7 + kPartLogits - 1) / kPartLogits; }
-size_t up(size_t x) { return (x + 255) & ~size_t{255}; }
+size_t segs_of(size_t n) { return (n + 7 + kSegLogits - 1) / kSegLogits; }
+struct VerifyWs {
+    size_t left, verdict, bytes;
+};
+VerifyWs verify_ws(size_t seqs, size_t rows, size_t n) {
+    auto up = [](size_t x) { return (x + 255) & ~size_t{255}; };
+    VerifyWs w{};
+    w.left = up(2 * rows * segs_of(n) * sizeof(Seg));
+    w.verdict = w.left + up(seqs * segs_of(n) * sizeof(double));
+    w.bytes = w.verdict + up(seqs * sizeof(Verdict));
+    return w;
+}
 
 }  // namespace
 }  // namespace ouro
@@ -462,10 +516,7 @@ using namespace ouro;
 
 extern "C" {
 
-size_t ouro_verify_drafts_workspace_bytes(size_t seqs, size_t rows, size_t n) {
-    const size_t parts = parts_of(n);
-    return up(2 * rows * parts * sizeof(Part)) + up(seqs * parts * sizeof(double));
-}
+size_t ouro_verify_drafts_workspace_bytes(size_t seqs, size_t rows, size_t n) { return verify_ws(seqs, rows, n).bytes; }
 
 int ouro_verify_drafts(const void *logits, int dtype, size_t row_stride, const void *draft, int draft_dtype, size_t draft_stride,
                        const int32_t *tokens, const int32_t *cu, size_t seqs, size_t rows, size_t max_new, size_t n,
@@ -495,11 +546,13 @@ int ouro_verify_drafts(const void *logits, int dtype, size_t row_stride, const v
     a.stride[0] = static_cast<int64_t>(row_stride), a.stride[1] = static_cast<int64_t>(draft_stride);
     a.tokens = tokens, a.lens = lens, a.temperature = temperature, a.u_accept = u_accept, a.u_next = u_next;
     a.accepted = accepted, a.next = next, a.lens_out = lens_out;
-    a.n = static_cast<int>(n), a.parts = static_cast<int>(parts_of(n));
-    const size_t need = ouro_verify_drafts_workspace_bytes(seqs, rows, n);
-    if (need && !ws && !(ws = workspace(need, stream))) return OURO_ERR_HIP;
-    a.part = static_cast<Part *>(ws);
-    a.left = reinterpret_cast<double *>(static_cast<unsigned char *>(ws) + up(2 * rows * static_cast<size_t>(a.parts) * sizeof(Part)));
+    a.n = static_cast<int>(n), a.segs = static_cast<int>(segs_of(n));
+    const VerifyWs w = verify_ws(seqs, rows, n);
+    if (!ws && !(ws = workspace(w.bytes, stream))) return OURO_ERR_HIP;
+    unsigned char *const p = static_cast<unsigned char *>(ws);
+    a.seg = reinterpret_cast<Seg *>(p);
+    a.left = reinterpret_cast<double *>(p + w.left);
+    a.verdict = reinterpret_cast<Verdict *>(p + w.verdict);
     const unsigned B = static_cast<unsigned>(seqs);
     hipStream_t s = as_stream(stream);
     if (half) return dhalf ? launch_verify<uint16_t, uint16_t>(a, B, s) : launch_verify<uint16_t, float>(a, B, s);

@@ -6,7 +6,7 @@ from pathlib import Path
 
 import pytest
 
-from ouroboros_amd import ops
+from ouroboros_amd import kvcache, ops
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -23,9 +23,20 @@ def test_calls_before_init_are_refused():
     assert r.returncode == 0 and "ok" in r.stdout, r.stderr
 
 
-@pytest.mark.parametrize("seqs,rows,n", [(1, 1, 1), (1, 5, 32003), (64, 320, 248320), (0, 0, 10), (3, 7, 8185), (3, 7, 8186)])
+@pytest.mark.parametrize("seqs,rows,n", [(1, 1, 1), (1, 5, 32003), (64, 320, 248320), (0, 0, 10), (3, 7, 2041), (3, 7, 2042)])
 def test_verify_workspace(seqs, rows, n):
-    parts = (n + 7 + 8191) // 8192  # the last of which may hold none where a row starts at a multiple of 16 bytes
-    need = 2 * rows * parts * 16 + seqs * parts * 8  # a maximum, its place and a sum of each part, of target and draft; what is left
+    segs = (n + 7 + 2047) // 2048  # the last of which may hold none where a row starts at a multiple of 16 bytes
+    # a maximum, its place and a sum of each segment, of target and draft; what is left; what the sequence came to
+    need = 2 * rows * segs * 16 + seqs * (segs * 8 + 48)
     got = ops.verify_workspace_bytes(seqs, rows, n)
     assert need <= got <= need + 4096
+
+
+@pytest.mark.parametrize("seqs,rows,max_new,heads,kv,d,max_len", [
+    (1, 1, 1, 16, 4, 128, 1), (64, 64, 1, 16, 4, 128, 2176), (48, 200, 6, 32, 2, 64, 8191), (2, 2048, 1024, 16, 4, 128, 16384), (1, 0, 0, 4, 1, 64, 100)])
+def test_attend_workspace(seqs, rows, max_new, heads, kv, d, max_len):
+    got = kvcache.attend8_workspace_bytes(seqs, rows, max_new, heads, kv, d, max_len)
+    # outputs, maxima and sums of the splits, each of a whole number of 256 slots; none where one holds all
+    most = -(-max_len // 256)
+    assert got <= rows * heads * most * (d + 2) * 4 + 256
+    assert got == 0 if max_len <= 256 or not rows else got >= rows * heads * 2 * (d + 2) * 4
