@@ -171,12 +171,16 @@ def lib() -> C.CDLL:
     return _LIB
 
 
-def call(name: str, *args) -> None:
-    """Call a status-returning entry point; raise OuroError on failure."""
-    st = getattr(lib(), name)(*args)
+def check(name: str, st: int) -> None:
+    """Raise OuroError where an entry point's status is not OURO_OK."""
     if st != OURO_OK:
         msg = lib().ouro_last_error()
         raise OuroError(name, st, msg.decode() if msg else "")
+
+
+def call(name: str, *args) -> None:
+    """Call a status-returning entry point; raise OuroError on failure."""
+    check(name, getattr(lib(), name)(*args))
 
 
 _INIT_DEVICE: int | None = None

@@ -14,7 +14,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 128;   // pairs of a head
-constexpr int kMaxTokens = 4;   // tokens of a workgroup
+constexpr int kMaxTokens = 8;   // tokens of a workgroup
+constexpr int64_t kManyRows = 2048;  // from here a workgroup takes several tokens, below a part of one's heads
 
 struct RopeArgs {
     const void *in[2];  // queries, keys
@@ -22,15 +23,15 @@ struct RopeArgs {
     const float *gain[2];
     const int32_t *pos, *axis;
     const float *freq;
-    int64_t in_stride[2], head_stride[2], out_stride[2];
+    int64_t in_stride[2], head_stride[2], out_stride[2], out_head[2];
     int64_t rows;
     int32_t heads, q_heads;  // query and key heads together, and the queries'
     int32_t d, half, axes, adjacent;
-    float eps;
-    int32_t tokens;  // of a workgroup
+    float eps, inv_d;
+    int32_t token_shift, pad;  // tokens of a workgroup
 };
 // passed by value to kernels: the host and device passes must lay it out alike
-static_assert(sizeof(RopeArgs) == 160, "RopeArgs: kernel argument layout");
+static_assert(sizeof(RopeArgs) == 184, "RopeArgs: kernel argument layout");
 
 // cos and sin of pos * freq.  In quarter turns u = pos freq 2/pi: its nearest
 // integer says which of cos, sin, -cos, -sin, and of what is left, within 1/2,
@@ -96,13 +97,17 @@ __device__ __forceinline__ void store(T *p, const float (&x)[E]) {
 // its own, so that nothing but the sum of squares crosses lanes: for pairs
 // (i, i + half) piece p of either half, for adjacent pairs pieces 2p and 2p + 1;
 // past n_rot two pieces in a row.  The angles of a token are the same for all of
-// its heads and are made once, by as many threads as it has pairs.
+// its heads: they are made once, by as many threads as it has pairs, and a group
+// of G lanes stays with one token and keeps its angles and gains in registers.
 template <typename T, int E, int G>
 __global__ __launch_bounds__(kThreads) void qk_rope_kernel(RopeArgs a) {
     __shared__ __attribute__((aligned(16))) float cs[kMaxTokens][kMaxHalf], sn[kMaxTokens][kMaxHalf];
     const int tid = threadIdx.x, p = tid % G;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens;
-    const int tokens = static_cast<int>(min(static_cast<int64_t>(a.tokens), a.rows - t0));
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) << a.token_shift;
+    const int tokens = static_cast<int>(min(int64_t{1} << a.token_shift, a.rows - t0));
+    const int groups = (kThreads / G) >> a.token_shift;  // of a token
+    const int t = tid / G / groups, step = groups * static_cast<int>(gridDim.y);
+    int h = tid / G % groups + groups * static_cast<int>(blockIdx.y);
     const int rot = a.half / E;  // pieces of a half
     int i0, i1;
     if (p < rot) {
@@ -113,75 +118,89 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(RopeArgs a) {
         i1 = i0 + E;
     }
     const bool in0 = i0 < a.d, in1 = i1 < a.d;
-    const int tasks = tokens * a.heads;
-    float x[E], y[E];
-    auto fetch = [&](int task) {
-        const int h = task % a.heads, key = h >= a.q_heads;
-        const T *row = static_cast<const T *>(a.in[key]) + (t0 + task / a.heads) * a.in_stride[key] +
-                       static_cast<int64_t>(key ? h - a.q_heads : h) * a.head_stride[key];
+    const int heads = t < tokens ? a.heads : 0;
+    float x[E], y[E], u[E], v[E];
+    auto fetch = [&](int head, float (&f)[E], float (&s)[E]) {
+        const int key = head >= a.q_heads;
+        const T *row = static_cast<const T *>(a.in[key]) + (t0 + t) * a.in_stride[key] +
+                       static_cast<int64_t>(key ? head - a.q_heads : head) * a.head_stride[key];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = y[e] = 0.f;
-        if (in0) load<E>(row + i0, x);
-        if (in1) load<E>(row + i1, y);
+        for (int e = 0; e < E; ++e) f[e] = s[e] = 0.f;
+        if (in0) load<E>(row + i0, f);
+        if (in1) load<E>(row + i1, s);
     };
-    int task = tid / G;
-    if (task < tasks) fetch(task);  // on its way while the angles are made
+    if (h < heads) fetch(h, x, y);  // on its way while the angles are made
     for (int i = tid; i < tokens * a.half; i += kThreads) {
-        const int t = i / a.half, j = i % a.half;
+        const int at = i / a.half, j = i % a.half;
         const int axis = a.axis ? max(0, min(a.axis[j], a.axes - 1)) : 0;
-        const float2 r = cos_sin(a.pos[axis * a.rows + t0 + t], a.freq[j]);
-        cs[t][j] = r.x;
-        sn[t][j] = r.y;
+        const float2 r = cos_sin(a.pos[axis * a.rows + t0 + at], a.freq[j]);
+        cs[at][j] = r.x;
+        sn[at][j] = r.y;
     }
     __syncthreads();
-    for (; task < tasks; task += kThreads / G) {
-        const int t = task / a.heads, h = task % a.heads, key = h >= a.q_heads;
-        const float *gain = a.gain[key];
-        if (gain) {
+    float c[E], s[E], g0[E], g1[E];
+    if (p < rot)
+#pragma unroll
+        for (int e = 0; e < E; ++e) c[e] = cs[t][p * E + e], s[e] = sn[t][p * E + e];
+    int have = -1;  // whose gains are held
+    for (; h < heads; h += step) {
+        const int key = h >= a.q_heads;
+        if (h + step < heads) fetch(h + step, u, v);
+        if (a.gain[key]) {
+            if (have != key) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    g0[e] = in0 ? a.gain[key][i0 + e] : 0.f;
+                    g1[e] = in1 ? a.gain[key][i1 + e] : 0.f;
+                }
+                have = key;
+            }
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) ss += x[e] * x[e] + y[e] * y[e];
 #pragma unroll
             for (int off = G / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, G);
-            const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.d) + a.eps);
+            const float inv = rsqrtf(ss * a.inv_d + a.eps);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (in0) x[e] = x[e] * inv * gain[i0 + e];
-                if (in1) y[e] = y[e] * inv * gain[i1 + e];
-            }
+            for (int e = 0; e < E; ++e) x[e] = x[e] * inv * g0[e], y[e] = y[e] * inv * g1[e];
         }
         if (p < rot) {
-            float c[E], s[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) c[e] = cs[t][p * E + e], s[e] = sn[t][p * E + e];
             if (a.adjacent) {
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {
-                    const float u = x[e], v = x[e + 1], w = y[e], z = y[e + 1];
-                    x[e] = u * c[e / 2] - v * s[e / 2], x[e + 1] = v * c[e / 2] + u * s[e / 2];
-                    y[e] = w * c[(E + e) / 2] - z * s[(E + e) / 2], y[e + 1] = z * c[(E + e) / 2] + w * s[(E + e) / 2];
+                    const float x0 = x[e], x1 = x[e + 1], y0 = y[e], y1 = y[e + 1];
+                    x[e] = x0 * c[e / 2] - x1 * s[e / 2], x[e + 1] = x1 * c[e / 2] + x0 * s[e / 2];
+                    y[e] = y0 * c[(E + e) / 2] - y1 * s[(E + e) / 2], y[e + 1] = y1 * c[(E + e) / 2] + y0 * s[(E + e) / 2];
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float u = x[e], v = y[e];
-                    x[e] = u * c[e] - v * s[e];
-                    y[e] = v * c[e] + u * s[e];
+                    const float x0 = x[e], y0 = y[e];
+                    x[e] = x0 * c[e] - y0 * s[e];
+                    y[e] = y0 * c[e] + x0 * s[e];
                 }
             }
         }
         T *row = static_cast<T *>(a.out[key]) + (t0 + t) * a.out_stride[key] +
-                 static_cast<int64_t>(key ? h - a.q_heads : h) * (a.in[key] == a.out[key] ? a.head_stride[key] : a.d);
+                 static_cast<int64_t>(key ? h - a.q_heads : h) * a.out_head[key];
         if (in0) store<E>(row + i0, x);
         if (in1) store<E>(row + i1, y);
-        if (task + kThreads / G < tasks) fetch(task + kThreads / G);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = u[e], y[e] = v[e];
     }
 }
 
 template <typename T, int E, int G>
 int launch(const RopeArgs &a, hipStream_t s) {
-    const int64_t blocks = (a.rows + a.tokens - 1) / a.tokens;
-    hipLaunchKernelGGL((qk_rope_kernel<T, E, G>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, a);
+    RopeArgs b = a;
+    unsigned parts = 1;
+    if (a.rows >= kManyRows) {
+        while (b.token_shift < 3 && (kThreads / G) >> b.token_shift > 4) ++b.token_shift;
+    } else {
+        parts = static_cast<unsigned>((a.heads + kThreads / G - 1) / (kThreads / G));
+    }
+    const int64_t tokens = int64_t{1} << b.token_shift;
+    hipLaunchKernelGGL((qk_rope_kernel<T, E, G>), dim3(static_cast<unsigned>((a.rows + tokens - 1) / tokens), parts), dim3(kThreads), 0, s, b);
     return check_launch("qk_rope_kernel");
 }
 // Pieces of 16 bytes where a half is whole pieces, else of the largest power of
@@ -243,7 +262,7 @@ extern "C" int ouro_qk_norm_rope(const void *q, size_t q_stride, size_t q_head_s
         if (in[i] > (size_t{1} << 40) || out[i] > (size_t{1} << 40)) return fail(OURO_ERR_SHAPE, "%s: a stride past 2^40", me);
         a.in[i] = src[i], a.out[i] = dst[i];
         a.in_stride[i] = static_cast<int64_t>(in[i]), a.head_stride[i] = static_cast<int64_t>(head[i]);
-        a.out_stride[i] = static_cast<int64_t>(out[i]);
+        a.out_stride[i] = static_cast<int64_t>(out[i]), a.out_head[i] = static_cast<int64_t>(dst[i] == src[i] ? head[i] : d);
     }
     if (!rows) return OURO_OK;
     a.gain[0] = q_gain, a.gain[1] = k_gain;
@@ -251,7 +270,6 @@ extern "C" int ouro_qk_norm_rope(const void *q, size_t q_stride, size_t q_head_s
     a.rows = static_cast<int64_t>(rows);
     a.q_heads = static_cast<int>(n_head), a.heads = static_cast<int>(n_head + n_head_kv);
     a.d = static_cast<int>(d), a.half = static_cast<int>(n_rot / 2), a.axes = static_cast<int>(axes);
-    a.adjacent = flags & OURO_ROPE_ADJACENT ? 1 : 0, a.eps = eps;
-    a.tokens = rows >= 2048 ? kMaxTokens : 1;
+    a.adjacent = flags & OURO_ROPE_ADJACENT ? 1 : 0, a.eps = eps, a.inv_d = 1.0f / static_cast<float>(d);
     return dtype == OURO_DT_F32 ? launch<float>(a, as_stream(stream)) : launch<uint16_t>(a, as_stream(stream));
 }

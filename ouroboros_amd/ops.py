@@ -223,10 +223,13 @@ def qk_norm_rope(q, k, q_out, k_out, pos, freq, *, rows: int, n_head: int, n_hea
     pos [axes][rows]; pair i turns by pos[axis[i]] * freq[i] radians.  Arguments
     are device memory; k and k_out may be None with n_head_kv = 0."""
     _lib.init()
-    call("ouro_qk_norm_rope", _addr(q), q_stride, q_head_stride, _addr(k), k_stride, k_head_stride, _addr(q_gain),
-         _addr(k_gain), _addr(pos), axes, _addr(axis), _addr(freq), n_rot, _lib.ROPE_ADJACENT if adjacent else 0,
-         _addr(q_out), q_out_stride, _addr(k_out), k_out_stride, _lib.dtype_code(dtype), rows, n_head, n_head_kv,
-         head_dim, eps, stream)
+    # the function itself, not by name through call(): this call is bound by its time on the host
+    st = _lib.lib().ouro_qk_norm_rope(
+        _addr(q), q_stride, q_head_stride, _addr(k), k_stride, k_head_stride, _addr(q_gain), _addr(k_gain), _addr(pos),
+        axes, _addr(axis), _addr(freq), n_rot, adjacent and _lib.ROPE_ADJACENT, _addr(q_out), q_out_stride, _addr(k_out),
+        k_out_stride, _lib.dtype_code(dtype), rows, n_head, n_head_kv, head_dim, eps, stream)
+    if st:
+        _lib.check("ouro_qk_norm_rope", st)
 
 
 def verify_drafts(logits, tokens, u_accept, u_next, accepted, next, *, seqs: int, rows: int, max_new: int, n: int,
