@@ -207,7 +207,9 @@ struct ReadArgs {
 };
 static_assert(sizeof(ReadArgs) == 144, "ReadArgs: kernel argument layout");
 
-// A thread makes 16 bytes of the output: four or eight codes of a row and head.
+// A thread makes 16 bytes of the output, four or eight codes of a row and head, of
+// kReadRows rows, whose loads are on their way together.
+constexpr int kReadRows = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a, int per_row) {
     constexpr int E = 16 / sizeof(T);
@@ -215,39 +217,52 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a, int per_row) 
     const int which = blockIdx.y;
     if (!a.dst[which]) return;
     const int d = a.c.d, pieces = d / E * a.c.n_head_kv;  // of a row
-    const int rows = 256 / per_row, row = static_cast<int>(blockIdx.x) * rows + static_cast<int>(threadIdx.x) / per_row;
-    if (row >= s.count || static_cast<int>(threadIdx.x) >= rows * per_row) return;
-    const int slot = s.n - s.count + row;
-    int32_t page = -1;
-    if (slot >= 0) page = a.c.pages[static_cast<int64_t>(blockIdx.z) * a.c.max_pages + (slot >> a.c.page_shift)];
-    const bool there = page >= 0 && page < a.c.n_pages;
-    const int t = slot & ((1 << a.c.page_shift) - 1);
+    const int at_once = 256 / per_row, row0 = static_cast<int>(blockIdx.x) * at_once * kReadRows + static_cast<int>(threadIdx.x) / per_row;
+    if (static_cast<int>(threadIdx.x) >= at_once * per_row) return;
+    int32_t page[kReadRows];
+    int t[kReadRows];
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+        const int row = row0 + k * at_once, slot = s.n - s.count + row;
+        page[k] = -1;
+        if (row < s.count && slot >= 0) page[k] = a.c.pages[static_cast<int64_t>(blockIdx.z) * a.c.max_pages + (slot >> a.c.page_shift)];
+        t[k] = slot & ((1 << a.c.page_shift) - 1);
+    }
     for (int i = static_cast<int>(threadIdx.x) % per_row; i < pieces; i += per_row) {
         const int head = i / (d / E), dim = i % (d / E) * E;
-        float x[E];
+        const int8_t *const pool = (which ? a.c.v : a.c.k) + head * a.c.head_stride + dim;
+        uint32_t w[kReadRows][E / 4];
+        float f[kReadRows];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = 0.f;
-        if (there) {
-            const int8_t *p = (which ? a.c.v : a.c.k) + kv8_row(a.c, page, t) + head * a.c.head_stride + dim;
-            const float f = (which ? a.c.v_scale : a.c.k_scale)[kv8_scale(a.c, page, t, head)];
-            uint32_t w[E / 4];
+        for (int k = 0; k < kReadRows; ++k) {
+            f[k] = 0.f;
+            w[k][0] = w[k][E / 4 - 1] = 0;
+            if (page[k] < 0 || page[k] >= a.c.n_pages) continue;
+            const int8_t *p = pool + kv8_row(a.c, page[k], t[k]);
+            f[k] = (which ? a.c.v_scale : a.c.k_scale)[kv8_scale(a.c, page[k], t[k], head)];
             if constexpr (E == 4) {
-                w[0] = *reinterpret_cast<const uint32_t *>(p);
+                w[k][0] = *reinterpret_cast<const uint32_t *>(p);
             } else {
                 const u32x2_t v = *reinterpret_cast<const u32x2_t *>(p);
-                w[0] = v[0], w[1] = v[1];
+                w[k][0] = v[0], w[k][1] = v[1];
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w[e / 4] >> (8 * (e & 3)))) * f;
         }
-        T *out = static_cast<T *>(a.dst[which]) + (s.first + row) * a.stride + static_cast<int64_t>(head) * d + dim;
-        if constexpr (E == 4) {
-            *reinterpret_cast<f32x4_t *>(out) = f32x4_t{x[0], x[1], x[2], x[3]};
-        } else {
-            u32x4_t w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16_bits(x[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(x[2 * e + 1])) << 16;
-            *reinterpret_cast<u32x4_t *>(out) = w;
+        for (int k = 0; k < kReadRows; ++k) {
+            const int row = row0 + k * at_once;
+            if (row >= s.count) break;
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w[k][e / 4] >> (8 * (e & 3)))) * f[k];
+            T *out = static_cast<T *>(a.dst[which]) + (s.first + row) * a.stride + static_cast<int64_t>(head) * d + dim;
+            if constexpr (E == 4) {
+                *reinterpret_cast<f32x4_t *>(out) = f32x4_t{x[0], x[1], x[2], x[3]};
+            } else {
+                u32x4_t v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = f32_to_bf16_bits(x[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(x[2 * e + 1])) << 16;
+                *reinterpret_cast<u32x4_t *>(out) = v;
+            }
         }
     }
 }
@@ -306,7 +321,7 @@ int ouro_kv8_read(const ouro_kv8_cache *cache, const int32_t *lens, const int32_
     a.stride = static_cast<int64_t>(out_stride);
     const int pieces = cache->head_dim / (dtype == OURO_DT_F32 ? 4 : 8) * cache->n_head_kv;
     const int per_row = pieces < 256 ? pieces : 256;
-    const size_t at_once = 256 / static_cast<size_t>(per_row);
+    const size_t at_once = static_cast<size_t>(256 / per_row * kReadRows);
     const dim3 grid(static_cast<unsigned>((max_new + at_once - 1) / at_once), 2, static_cast<unsigned>(seqs));
     hipStream_t s = as_stream(stream);
     if (dtype == OURO_DT_F32)
