@@ -9,6 +9,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace ouro {
 namespace {
@@ -33,7 +34,7 @@ struct Attend8Args {
     float *part;  // [rows][n_head][n_split][d]: the splits' outputs, not normalised
     float2 *ml;   // [rows][n_head][n_split]: their maxima (of scores times log2 e) and sums
     int64_t q_stride, mask_stride, out_stride;
-    int32_t n_head, window, sinks;  // window 0: every slot
+    int32_t n_head, window, sinks;  // window 2^30: every slot
     float scale;
     int32_t n_split, turns;  // turns of a split
 };
@@ -88,6 +89,13 @@ __device__ __forceinline__ float quad_sum(float v) {
 __device__ __forceinline__ float lane_float(float v, int lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
+// Two codes of a byte pair each (code + 128 in the low bytes) as fp16 times 2^-9:
+// (c + 128) 2^-24 2^15 - 128 2^-9 = c 2^-9, exact.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
+    const f16x2_t c = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, two), f16x2_t{32768.f16, 32768.f16}, f16x2_t{-0.25f16, -0.25f16});
+    return __builtin_bit_cast(uint32_t, c);
+}
+
 // x, as a value that is made where this stands: what is read by it stays in the
 // loop.  The asm holds no instruction, so that no wait state is owed around it.
 __device__ __forceinline__ int in_loop(int x) {
@@ -107,7 +115,7 @@ __device__ __forceinline__ void store_lse(const Attend8Args &a, int64_t row, int
 }
 // Whether a row in slot `at` can see any of slots j0 .. j1 - 1.
 __device__ __forceinline__ bool sees(const Attend8Args &a, int at, int j0, int j1) {
-    return j0 <= at && (!a.window || j1 + a.window > at + 1 || j0 < a.sinks);
+    return j0 <= at && (at + 1 - a.window < j1 || j0 < a.sinks);
 }
 
 // One workgroup takes 16 NT rows (token by token, each token's query heads of one
@@ -149,11 +157,18 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
     const int split = blockIdx.z, first_slot = split * a.turns * kTurn;
     // Lane l of wavefront w stands for slot 32 (w + 4 (l / 32)) + l % 32 of a turn:
     // the wavefront's own tiles, whose pages, scales and visible slots stay in its
-    // registers.  A turn's page ids are read without waiting for the length.
+    // registers.  A turn's page ids and mask are read without waiting for the length.
     const int mine = 32 * (wave + 4 * (lane >> 5)) + (lane & 31);
     const int32_t *const pages = a.c.pages + b * a.c.max_pages;
-    auto page_at = [&](int j) { return j < a.r.max_len ? pages[j >> a.c.page_shift] : -1; };
-    int32_t id = page_at(first_slot + mine);
+    int32_t id = -1;   // of the turn that is looked at next
+    uint32_t kept = 1;  // and its mask byte
+    auto fetch = [&](int j) {
+        id = -1;
+        if (j >= a.r.max_len) return;
+        id = pages[j >> a.c.page_shift];
+        if (a.mask) kept = a.mask[b * a.mask_stride + j];
+    };
+    fetch(first_slot + mine);
     const SeqRows s = seq_rows(a.r, b);
     const int R = s.count * G, row0 = static_cast<int>(blockIdx.y) * kRows;
     if (row0 >= R) return;  // whole workgroup
@@ -164,22 +179,31 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
     if (whole ? split > 0 : !sees(a, at_max, first_slot, split_end) && !sees(a, at_min, first_slot, split_end)) return;
     const int end = min(split_end, at_max + 1);  // the slots taken are first_slot .. end - 1, of those that are seen
 
+    // The rows' queries are on their way while the cache is looked at: 16 dims a lane,
+    // LPR lanes a row.
+    constexpr int NI = (kRows * LPR + 255) / 256;
+    float x[NI][16];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+        const int i = 256 * k + tid, rho = row0 + i / LPR, ch = i % LPR;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[k][e] = 0.f;
+        if (i < kRows * LPR && rho < R && 16 * ch < d)
+            load16(static_cast<const IO *>(a.q) + (s.first + rho / G) * a.q_stride + static_cast<int64_t>(kvh * G + rho % G) * d + 16 * ch, x[k]);
+    }
     int32_t page = 0;   // held to 0 .. n_pages - 1: a hole's rows are read (of a page that is there), never used
-    float k_sc = 0.f, v_sc = 0.f;
+    float k_raw = 0.f, v_raw = 0.f;
     uint64_t bits = 0;  // the turn's slots that some row sees
-    auto look = [&](int j) {  // of slot j, whose page id is `id`
-        bool seen = id >= 0 && id < a.c.n_pages && j < end && (!a.window || j > at_min - a.window || j < a.sinks);
-        if (seen && a.mask) seen = a.mask[b * a.mask_stride + j] != 0;
-        page = id >= 0 && id < a.c.n_pages ? id : 0;
-        bits = __ballot(seen);
+    auto look = [&](int j) {  // at slot j, which was fetched
+        const bool there = id >= 0 && id < a.c.n_pages;
+        page = there ? id : 0;
+        bits = __ballot(there && kept != 0 && j < end && (j > at_min - a.window || j < a.sinks));
         // a tile of 16 slots lies in one block, whose scales all of its lanes read
-        const uint32_t tile = static_cast<uint32_t>(bits >> (lane & 48)) & 0xffffu;
-        k_sc = v_sc = 0.f;
-        if (tile) {
+        k_raw = v_raw = 0.f;
+        if (static_cast<uint32_t>(bits >> (lane & 48)) & 0xffffu) {
             const int64_t i = kv8_scale(a.c, page, j & ((1 << a.c.page_shift) - 1), kvh);
-            const float x = a.c.k_scale[i], y = a.c.v_scale[i];
-            k_sc = x >= 0.f && x < INFINITY ? x : NAN;
-            v_sc = y >= 0.f && y < INFINITY ? y : NAN;
+            k_raw = a.c.k_scale[i];
+            v_raw = a.c.v_scale[i];
         }
     };
     const int8_t *const kp = a.c.k + kvh * a.c.head_stride, *const vp = a.c.v + kvh * a.c.head_stride;
@@ -221,19 +245,16 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
         load_v(j, 0, tile_bits(0) != 0);
     }
 
-    // The rows' digits: lane group LPR a row, 16 dims a lane.  A negative scale
-    // goes into their sign, so that a row's largest score is that of its largest sum.
+    // The rows' digits.  A negative scale goes into their sign, so that a row's
+    // largest score is that of its largest sum.
     const bool negative = a.scale < 0.f;
-    for (int i = tid; i < kRows * LPR; i += 256) {
-        const int row = i / LPR, ch = i % LPR, rho = row0 + row;
-        float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        if (rho < R && 16 * ch < d)
-            load16(static_cast<const IO *>(a.q) + (s.first + rho / G) * a.q_stride + static_cast<int64_t>(kvh * G + rho % G) * d + 16 * ch, x);
+    for (int k = 0; k < NI; ++k) {
+        const int i = 256 * k + tid, row = i / LPR, ch = i % LPR;
+        if (i >= kRows * LPR) break;
         uint32_t top = 0;  // magnitudes order as their bits do, NaN above infinity
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
 #pragma unroll
         for (int off = LPR / 2; off >= 1; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, LPR)));
         // the smallest power of two with max <= 127 65536 2^e (a row below 2^-94 takes 2^-117)
@@ -246,7 +267,7 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
                 uint32_t p0 = 0, p1 = 0, p2 = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    int v = static_cast<int>(rintf(ldexpf(x[4 * w + e], -ex)));
+                    int v = static_cast<int>(rintf(ldexpf(x[k][4 * w + e], -ex)));
                     if (negative) v = -v;
                     const int c0 = static_cast<int8_t>(v), v1 = (v - c0) >> 8, c1 = static_cast<int8_t>(v1), c2 = (v1 - c1) >> 8;
                     p0 |= (static_cast<uint32_t>(c0) & 0xffu) << (8 * e);
@@ -257,7 +278,7 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
             }
             const int to = ((row >> 4) * NJ + (ch >> 2)) * 64 + 16 * (ch & 3) + (row & 15);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) reinterpret_cast<u32x4_t *>(lds)[k * NT * NJ * 64 + to] = dg[k];
+            for (int n = 0; n < 3; ++n) reinterpret_cast<u32x4_t *>(lds)[n * NT * NJ * 64 + to] = dg[n];
         }
     }
     __syncthreads();
@@ -273,25 +294,32 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
 #pragma unroll
         for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    float v_top = 0.f;  // the largest scale of V so far; outputs are in units of it (times 2^6)
+    float v_top = 0.f, v_inv = 1.f;  // the largest scale of V so far and its reciprocal; outputs are in units of it (times 2^6)
     const int turns = (end - first_slot + kTurn - 1) / kTurn;
     for (int turn = 0; turn < turns; ++turn) {
         const int t0 = first_slot + turn * kTurn;
-        if (turn + 1 < turns) id = page_at(t0 + kTurn + mine);
+        const float k_sc = k_raw >= 0.f && k_raw < INFINITY ? k_raw : NAN, v_sc = v_raw >= 0.f && v_raw < INFINITY ? v_raw : NAN;
+        fetch(turn + 1 < turns ? t0 + kTurn + mine : a.r.max_len);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int j = t0 + 32 * (wave + 4 * k);
             const uint32_t now = tile_bits(k);
             const float ks[2] = {lane_float(k_sc, 32 * k), lane_float(k_sc, 32 * k + 16)};
             const float vs[2] = {lane_float(v_sc, 32 * k), lane_float(v_sc, 32 * k + 16)};
-            const bool all = now == 0xffffffffu && j + 31 <= at_min && (!a.window || j > at_max - a.window || j + 31 < a.sinks);
+            const bool all = now == 0xffffffffu && j + 31 <= at_min && (j > at_max - a.window || j + 31 < a.sinks);
             u32x4_t ph[NT], pl[NT];  // the weights' two operands
-            float grown = 1.f;
-            if (now) {
+            // A tile's scores, running maxima and weights.  Masked: some row does not
+            // see some slot.
+            auto weigh = [&](auto masked) {
+                constexpr bool Masked = decltype(masked)::value;
                 const float top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
-                grown = top == v_top ? 1.f : v_top / top;
-                v_top = top;
-                const float f[2] = {v_top > 0.f ? vs[0] / v_top * 32768.f : vs[0], v_top > 0.f ? vs[1] / v_top * 32768.f : vs[1]};
+                float grown = 1.f;
+                if (top != v_top) {
+                    grown = v_top / top;
+                    v_top = top;
+                    v_inv = 1.0f / top;
+                }
+                const float f[2] = {vs[0] * v_inv * 32768.f, vs[1] * v_inv * 32768.f};
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     float sum[2][4];
@@ -316,37 +344,45 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
                         for (int i = 0; i < 4; ++i) sum[u][i] = __builtin_fmaf(static_cast<float>(hi[i]), 256.f, static_cast<float>(lo[i]));
                     }
                     const float kq[2] = {qs[t] * ks[0], qs[t] * ks[1]};
-                    bool vis[2][4];
+                    uint32_t vis = 0;  // bit 4 u + i: slot 16 u + i after the lane's first, j + 4 g, is seen
                     float top_s = -INFINITY;
-                    if (all) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            top_s = fmaxf(top_s, kq[u] * fmaxf(fmaxf(sum[u][0], sum[u][1]), fmaxf(sum[u][2], sum[u][3])));
-                    } else {
+                    if constexpr (Masked) {
+                        // it is up to `last`, but for what lies between `sinks` and the window
+                        const int last = at[t] - j - 4 * g, low = last - a.window, sinks = a.sinks - j - 4 * g;
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const int jj = j + 16 * u + 4 * g + i;
-                                vis[u][i] = (now >> (16 * u + 4 * g + i) & 1) && jj <= at[t] && (!a.window || jj > at[t] - a.window || jj < a.sinks);
-                                if (vis[u][i]) top_s = fmaxf(top_s, kq[u] * sum[u][i]);
+                                const int slot = 16 * u + i;
+                                const uint32_t in = static_cast<uint32_t>(slot <= last) & (static_cast<uint32_t>(slot > low) | static_cast<uint32_t>(slot < sinks));
+                                vis |= (in & (now >> (slot + 4 * g))) << (4 * u + i);
+                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? kq[u] * sum[u][i] : -INFINITY);
                             }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            top_s = fmaxf(top_s, kq[u] * fmaxf(fmaxf(sum[u][0], sum[u][1]), fmaxf(sum[u][2], sum[u][3])));
                     }
-                    const float mn = fmaxf(m[t], quad_max(top_s));
-                    const float ref = mn == -INFINITY ? 0.f : mn;  // no finite score yet: avoid inf - inf
-                    const float corr = __builtin_amdgcn_exp2f(m[t] - ref);
-                    m[t] = mn;
-                    float ps = 0.f;
+                    // the reference moves only where some row of the tile has a larger score
+                    if (__any(top_s > m[t]) || grown != 1.f) {
+                        const float mn = fmaxf(m[t], quad_max(top_s));
+                        const float back = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));  // no inf - inf
+                        m[t] = mn;
+                        l[t] *= back;
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) o[t][e] *= back * grown;
+                    }
+                    const float ref = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         float p[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sum[u][i], kq[u], -ref));
-                            if (!all && !vis[u][i]) p[i] = 0.f;
-                            ps += p[i];
+                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;
+                            l[t] += p[i];
                             p[i] *= f[u];
-                            if (!all && !vis[u][i]) p[i] = 0.f;  // whatever the scale of a slot that is not seen
+                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;  // whatever the scale of a slot that is not seen
                         }
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
@@ -357,14 +393,12 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
                             pl[t][2 * u + i] = __builtin_bit_cast(uint32_t, w);
                         }
                     }
-                    l[t] = l[t] * corr + quad_sum(ps);
-                    const float back = corr * grown;
-                    if (!__all(back == 1.0f)) {
-#pragma unroll
-                        for (int e = 0; e < CH; ++e) o[t][e] *= back;
-                    }
                 }
-            }
+            };
+            if (all)
+                weigh(std::false_type{});
+            else if (now)
+                weigh(std::true_type{});
             // K's registers are free: the next tile's rows
             if (k == 0) {
                 load_k(j + 128, 1, tile_bits(1) != 0);
@@ -384,12 +418,8 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const uint32_t two = __builtin_amdgcn_perm(vf[u][2 * i + 1][e / 4], vf[u][2 * i][e / 4],
-                                                                       0x0c040c00u + 0x00010001u * static_cast<uint32_t>(e % 4));
-                            // (c + 128) 2^-24 2^15 - 128 2^-9 = c 2^-9
-                            const f16x2_t c = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, two), f16x2_t{32768.f16, 32768.f16},
-                                                                        f16x2_t{-0.25f16, -0.25f16});
-                            w[2 * u + i] = __builtin_bit_cast(uint32_t, c);
+                            w[2 * u + i] = codes_f16(__builtin_amdgcn_perm(vf[u][2 * i + 1][e / 4], vf[u][2 * i][e / 4],
+                                                                           0x0c040c00u + 0x00010001u * static_cast<uint32_t>(e % 4)));
                         }
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
@@ -403,9 +433,11 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
     }
 
     // the four wavefronts' outputs joined, kJoin rows at a time
-    if (g == 0)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sm[wave][16 * t + r] = m[t], sl[wave][16 * t + r] = l[t];
+    for (int t = 0; t < NT; ++t) {
+        const float sum = quad_sum(l[t]);
+        if (g == 0) sm[wave][16 * t + r] = m[t], sl[wave][16 * t + r] = sum;
+    }
     if (lane == 0) sf[wave] = v_top * 0.015625f;
     float *const ob = reinterpret_cast<float *>(lds);
 #pragma unroll
@@ -446,8 +478,350 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
         }
 }
 
+// The same for many rows of a sequence and kv head: 64 RT of them a workgroup, 16 RT
+// a wavefront, which takes them through all slots of the split, so that nothing is
+// joined but splits.  64 slots at a time of K and V are turned to fp16 operands
+// once for all of them and go through LDS, a buffer being filled while the other
+// is read; wavefronts 0 and 1 make V's operands, 2 and 3 K's.  A query is one fp16
+// operand against a power of two of its row (bf16 fits it whole) or, in fp32, two
+// (2^-22 of a value), and the scores are summed in fp32: the codes' exact products
+// of three digits cost a third more matrix instructions and four conversions a
+// score.
+template <typename IO, int DP, int RT>
+__global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
+    constexpr int NC = DP / 32;                // steps of the first product over the dims
+    constexpr int CH = DP / 16, VW = CH / 4;   // adjacent dims of V a lane, and their dwords
+    constexpr int NQ = sizeof(IO) == 4 ? 2 : 1;
+    constexpr int kStage = 64;
+    constexpr int kK = 4 * NC * 64, kV = 2 * CH * 64;  // operands of 16 bytes a buffer
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // two buffers of K's [4][NC][64] and V's [2][CH][64]
+    typedef uint32_t vch_t __attribute__((ext_vector_type(VW)));
+    u32x4_t *const buf = reinterpret_cast<u32x4_t *>(lds);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int kvh = static_cast<int>(blockIdx.x) % a.c.n_head_kv;
+    const int64_t b = static_cast<int64_t>(blockIdx.x) / a.c.n_head_kv;
+    const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
+    const SeqRows s = seq_rows(a.r, b);
+    const int R = s.count * G, group0 = static_cast<int>(blockIdx.y) * 64 * RT;
+    if (group0 >= R) return;  // whole workgroup
+    const int before = s.n - s.count;  // slots ahead of the new rows
+    const int slots = a.turns * kTurn, split = blockIdx.z, split_first = split * slots, split_end = min(split_first + slots, s.n);
+    const int at_min = before + group0 / G, at_max = before + (min(group0 + 64 * RT, R) - 1) / G;
+    const bool whole = s.n <= slots;  // the sequence's only split
+    if (whole ? split > 0 : !sees(a, at_max, split_first, split_end) && !sees(a, at_min, split_first, split_end)) return;
+    const int end = min(split_end, at_max + 1);
+    // what lies behind every row's window is not walked through, but where the first slots are seen
+    const int first = split_first < a.sinks ? split_first : max(split_first, (at_min + 1 - a.window) & ~(kStage - 1));
+    const int stages = end > first ? (end - first + kStage - 1) / kStage : 0;
+    const int row0 = group0 + 16 * RT * wave;  // the wavefront's
+    const int mine_min = before + min(row0, R - 1) / G, mine_max = before + (min(row0 + 16 * RT, R) - 1) / G;
+
+    // Lane l stands for slot l of a stage; every wavefront looks at all of them.
+    const int32_t *const pages = a.c.pages + b * a.c.max_pages;
+    int32_t id = -1;
+    uint32_t kept = 1;
+    auto fetch = [&](int stage) {
+        const int j = first + kStage * stage + lane;
+        id = -1;
+        if (stage >= stages || j >= a.r.max_len) return;
+        id = pages[j >> a.c.page_shift];
+        if (a.mask) kept = a.mask[b * a.mask_stride + j];
+    };
+    int32_t page = 0;
+    float k_raw = 0.f, v_raw = 0.f;
+    uint64_t bits = 0;
+    auto look = [&](int stage) {
+        const int j = first + kStage * stage + lane;
+        const bool there = id >= 0 && id < a.c.n_pages;
+        page = there ? id : 0;  // a hole's rows are read (of a page that is there), never used
+        bits = __ballot(there && kept != 0 && j < end && (j > at_min - a.window || j < a.sinks));
+        k_raw = v_raw = 0.f;
+        if (static_cast<uint32_t>(bits >> (lane & 48)) & 0xffffu) {
+            const int64_t i = kv8_scale(a.c, page, j & ((1 << a.c.page_shift) - 1), kvh);
+            k_raw = a.c.k_scale[i];
+            v_raw = a.c.v_scale[i];
+        }
+    };
+    // The wavefront's part of a stage: 32 slots, from 32 (wave % 2).  16 slots from a
+    // multiple of 16 stay in their page; where none of 16 is seen, one line is read.
+    const int8_t *const kp = a.c.k + kvh * a.c.head_stride, *const vp = a.c.v + kvh * a.c.head_stride;
+    u32x4_t raw[2 * (DP / 64) > 4 * VW / 2 ? 2 * (DP / 64) : 4 * VW / 2];  // 2 DP / 64 pieces of K, or 8 of VW dwords of V
+    constexpr int NJ = DP / 64;
+    const int part = 32 * (wave & 1);
+    auto load = [&](int stage) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bool there = static_cast<uint32_t>(bits >> (part + 16 * u)) & 0xffffu;
+            const int j = first + kStage * stage + part + 16 * u;
+            const int64_t row = there ? static_cast<int64_t>(__builtin_amdgcn_readlane(page, part + 16 * u)) * a.c.page_stride +
+                                            static_cast<int64_t>(j & ((1 << a.c.page_shift) - 1)) * a.c.token_stride
+                                      : 0;
+            const uint32_t step = there ? static_cast<uint32_t>(a.c.token_stride) : 0u;
+            if (wave >= 2) {
+#pragma unroll
+                for (int i = 0; i < NJ; ++i)
+                    raw[u * NJ + i] = *reinterpret_cast<const u32x4_t *>(kp + row + (static_cast<uint32_t>(r) * step + static_cast<uint32_t>(min(16 * (4 * i + g), d - 16))));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const vch_t v = *reinterpret_cast<const vch_t *>(vp + row + (static_cast<uint64_t>(4 * g + i) * step + static_cast<uint32_t>(min(CH * r, d - CH))));
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) raw[(VW * (4 * u + i) + w) / 4][(VW * (4 * u + i) + w) % 4] = v[w];
+                }
+            }
+        }
+    };
+    auto stage_out = [&](int into) {
+        u32x4_t *const to = buf + into * (kK + kV);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(raw) / 16); ++i) raw[i] ^= u32x4_t(0x80808080u);  // code + 128
+        if (wave >= 2) {
+            // 16 dims of a slot: eight each of operands 2 j and 2 j + 1
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < NJ; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        u32x4_t w;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t four = raw[u * NJ + i][2 * h + x / 2];
+                            w[x] = codes_f16(__builtin_amdgcn_perm(four, four, x & 1 ? 0x0c030c02u : 0x0c010c00u));
+                        }
+                        to[((part / 16 + u) * NC + 2 * i + h) * 64 + lane] = w;
+                    }
+        } else {
+            // eight slots of CH dims: an operand of each dim
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+                u32x4_t w;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int n0 = VW * (2 * x) + e / 4, n1 = VW * (2 * x + 1) + e / 4;
+                    w[x] = codes_f16(__builtin_amdgcn_perm(raw[n1 / 4][n1 % 4], raw[n0 / 4][n0 % 4], 0x0c040c00u + 0x00010001u * static_cast<uint32_t>(e % 4)));
+                }
+                to[kK + (part / 32 * CH + e) * 64 + lane] = w;
+            }
+        }
+    };
+
+    fetch(0);
+    // The wavefront's queries as operands: dims 64 j + 16 g + 8 h .. + 7 of row r in
+    // operand 2 j + h, against a power of two at or above the row's largest half.
+    u32x4_t qf[RT][NQ][NC];
+    float qs[RT];
+    int at[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int rho = row0 + 16 * t + r;
+        at[t] = rho < R ? before + rho / G : -1;
+        float x[NJ][16];
+        uint32_t top = 0;  // magnitudes order as their bits do, NaN above infinity
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) {
+            const int dim = 64 * i + 16 * g;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[i][e] = 0.f;
+            if (rho < R && dim < d) load16(static_cast<const IO *>(a.q) + (s.first + rho / G) * a.q_stride + static_cast<int64_t>(kvh * G + rho % G) * d + dim, x[i]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+        }
+        top = max(top, static_cast<uint32_t>(xor_shfl(static_cast<int>(top), 16)));
+        top = max(top, static_cast<uint32_t>(xor_shfl(static_cast<int>(top), 32)));
+        const int ex = max(static_cast<int>(top >> 23), 27) - 127 - 14;  // max < 2^15 2^ex (a row below 2^-100 takes 2^-114)
+        // the codes are multiples of 2^-9; a negative scale goes into the operands' sign
+        qs[t] = top >= 0x7f800000u ? NAN : ldexpf(fabsf(a.scale) * 1.4426950408889634f * 512.f, ex);
+#pragma unroll
+        for (int i = 0; i < NJ; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float x0 = ldexpf(a.scale < 0.f ? -x[i][8 * h + 2 * w] : x[i][8 * h + 2 * w], -ex);
+                    const float x1 = ldexpf(a.scale < 0.f ? -x[i][8 * h + 2 * w + 1] : x[i][8 * h + 2 * w + 1], -ex);
+                    const f16x2_t hi = __builtin_convertvector(f32x2_t{x0, x1}, f16x2_t);
+                    qf[t][0][2 * i + h][w] = __builtin_bit_cast(uint32_t, hi);
+                    if constexpr (NQ == 2)
+                        qf[t][1][2 * i + h][w] = __builtin_bit_cast(
+                            uint32_t, __builtin_convertvector(f32x2_t{x0 - static_cast<float>(hi[0]), x1 - static_cast<float>(hi[1])}, f16x2_t));
+                }
+    }
+    f32x4_t o[RT][CH];  // o[t][e][i]: dim CH (4 g + i) + e of row r of tile t
+    float m[RT], l[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        m[t] = -INFINITY, l[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    float v_top = 0.f, v_inv = 1.f;
+    look(0);
+    load(0);
+    fetch(1);
+    stage_out(0);
+    uint64_t seen = bits;
+    float k_sc = k_raw, v_sc = v_raw;
+    __syncthreads();
+    for (int stage = 0; stage < stages; ++stage) {
+        k_sc = k_sc >= 0.f && k_sc < INFINITY ? k_sc : NAN, v_sc = v_sc >= 0.f && v_sc < INFINITY ? v_sc : NAN;
+        look(stage + 1);  // past the last nothing is seen
+        load(stage + 1);
+        fetch(stage + 2);
+        const u32x4_t *const from = buf + (stage & 1) * (kK + kV);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int j = first + kStage * stage + 32 * half;
+            uint32_t now = static_cast<uint32_t>(seen >> (32 * half));
+            if (j > mine_max || (j + 31 <= mine_min - a.window && j >= a.sinks) || row0 >= R) now = 0;
+            const bool all = now == 0xffffffffu && j + 31 <= mine_min && (j > mine_max - a.window || j + 31 < a.sinks);
+            const float ks[2] = {lane_float(k_sc, 32 * half), lane_float(k_sc, 32 * half + 16)};
+            const float vs[2] = {lane_float(v_sc, 32 * half), lane_float(v_sc, 32 * half + 16)};
+            u32x4_t ph[RT], pl[RT];
+            auto weigh = [&](auto masked) {
+                constexpr bool Masked = decltype(masked)::value;
+                const float top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
+                float grown = 1.f;
+                if (top != v_top) {
+                    grown = v_top / top;
+                    v_top = top;
+                    v_inv = 1.0f / top;
+                }
+                const float f[2] = {vs[0] * v_inv * 32768.f, vs[1] * v_inv * 32768.f};
+                f32x4_t sum[RT][2];
+#pragma unroll
+                for (int t = 0; t < RT; ++t) sum[t][0] = sum[t][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = NQ - 1; n >= 0; --n)  // the smaller operand first
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        u32x4_t k[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) k[u] = from[((2 * half + u) * NC + c) * 64 + lane];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int t = 0; t < RT; ++t)
+                                sum[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k[u]), __builtin_bit_cast(f16x8_t, qf[t][n][c]), sum[t][u], 0, 0, 0);
+                    }
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const float kq[2] = {qs[t] * ks[0], qs[t] * ks[1]};
+                    uint32_t vis = 0;
+                    float top_s = -INFINITY;
+                    if constexpr (Masked) {
+                        const int last = at[t] - j - 4 * g, low = last - a.window, sinks = a.sinks - j - 4 * g;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int slot = 16 * u + i;
+                                const uint32_t in = static_cast<uint32_t>(slot <= last) & (static_cast<uint32_t>(slot > low) | static_cast<uint32_t>(slot < sinks));
+                                vis |= (in & (now >> (slot + 4 * g))) << (4 * u + i);
+                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? kq[u] * sum[t][u][i] : -INFINITY);
+                            }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            top_s = fmaxf(top_s, kq[u] * fmaxf(fmaxf(sum[t][u][0], sum[t][u][1]), fmaxf(sum[t][u][2], sum[t][u][3])));
+                    }
+                    if (__any(top_s > m[t]) || grown != 1.f) {
+                        const float mn = fmaxf(m[t], quad_max(top_s));
+                        const float back = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));  // no inf - inf
+                        m[t] = mn;
+                        l[t] *= back;
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) o[t][e] *= back * grown;
+                    }
+                    const float ref = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sum[t][u][i], kq[u], -ref));
+                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;
+                            l[t] += p[i];
+                            p[i] *= f[u];
+                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;  // whatever the scale of a slot that is not seen
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const f16x2_t h = __builtin_convertvector(f32x2_t{p[2 * i], p[2 * i + 1]}, f16x2_t);
+                            const f16x2_t w = __builtin_convertvector(
+                                f32x2_t{__builtin_fmaf(static_cast<float>(h[0]), -1.f, p[2 * i]), __builtin_fmaf(static_cast<float>(h[1]), -1.f, p[2 * i + 1])}, f16x2_t);
+                            ph[t][2 * u + i] = __builtin_bit_cast(uint32_t, h);
+                            pl[t][2 * u + i] = __builtin_bit_cast(uint32_t, w);
+                        }
+                    }
+                }
+            };
+            if (all)
+                weigh(std::false_type{});
+            else if (now)
+                weigh(std::true_type{});
+            if (now) {
+                // four dims at a time: no product waits for the one before it
+#pragma unroll
+                for (int e0 = 0; e0 < CH; e0 += 4) {
+                    u32x4_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = from[kK + (half * CH + e0 + e) * 64 + lane];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int t = 0; t < RT; ++t)
+                                o[t][e0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[e]), __builtin_bit_cast(f16x8_t, n ? pl[t] : ph[t]), o[t][e0 + e], 0, 0, 0);
+                }
+            }
+        }
+        if (stage + 1 < stages) stage_out((stage + 1) & 1);  // last read a stage ago, before the barrier
+        seen = bits;
+        k_sc = k_raw, v_sc = v_raw;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float L = quad_sum(l[t]);
+        const int rho = row0 + 16 * t + r;
+        if (rho >= R) continue;
+        const int64_t row = s.first + rho / G;
+        const int h = kvh * G + rho % G;
+        const float unit = v_top * 0.015625f;  // outputs are in units of V's largest scale, times 2^6
+        const int64_t rec = (row * a.n_head + h) * a.n_split + split;
+        if (g == 0) {
+            if (whole)
+                store_lse(a, row, h, m[t], L);
+            else
+                a.ml[rec] = make_float2(m[t], L);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int dim = CH * (4 * g + i);
+            if (dim >= d) continue;
+#pragma unroll
+            for (int e = 0; e < CH; e += 4) {
+                f32x4_t x;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = o[t][e + k][i] * unit;
+                if (whole) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) store_out<IO>(a, row, h, dim + e + k, L == 0.f ? 0.f : x[k] / L);
+                } else {
+                    *reinterpret_cast<f32x4_t *>(a.part + rec * d + dim + e) = x;
+                }
+            }
+        }
+    }
+}
+
 // The splits of a row and head joined by NG groups of DP / 4 lanes, each with
-// every NG-th split and four dims a lane; 256 / (NG DP / 4) heads a workgroup.
+// every NG-th split and four dims a lane, kAhead splits on their way at a time;
+// 256 / (NG DP / 4) heads a workgroup.
+constexpr int kAhead = 4;
 template <typename IO, int DP, int NG>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
     constexpr int DL = DP / 4, PER = 256 / (NG * DL);
@@ -467,14 +841,27 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
     f32x4_t x = {0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
     if (live)
-        for (int sp = grp; sp * slots <= at; sp += NG) {
-            if (!sees(a, at, sp * slots, min((sp + 1) * slots, s.n))) continue;
-            const float2 ml = a.ml[rec + sp];
-            const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-            const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml.x - ref);
-            L = L * f + ml.y * w;
-            if (dim < d) x = x * f + w * *reinterpret_cast<const f32x4_t *>(a.part + (rec + sp) * d + dim);
-            M = mn;
+        for (int s0 = grp; s0 * slots <= at; s0 += kAhead * NG) {
+            float2 ml[kAhead];
+            f32x4_t part[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int sp = s0 + k * NG;
+                ml[k] = make_float2(-INFINITY, 0.f);
+                part[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (sp * slots <= at && sees(a, at, sp * slots, min((sp + 1) * slots, s.n))) {
+                    ml[k] = a.ml[rec + sp];
+                    if (dim < d) part[k] = *reinterpret_cast<const f32x4_t *>(a.part + (rec + sp) * d + dim);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const float mn = fmaxf(M, ml[k].x), ref = mn == -INFINITY ? 0.f : mn;
+                const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml[k].x - ref);
+                L = L * f + ml[k].y * w;
+                x = x * f + w * part[k];
+                M = mn;
+            }
         }
     if constexpr (NG > 1) {
         red[tid] = x;
@@ -497,6 +884,22 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
     if (dim == 0) store_lse(a, row, h, M, L);
 }
 
+// The join after a kernel of the splits.
+template <typename IO, int DP>
+int launch_join(const Attend8Args &a, size_t seqs, hipStream_t s);
+
+template <typename IO, int DP, int RT>
+int launch_rows(const Attend8Args &a, size_t seqs, hipStream_t s) {
+    constexpr size_t lds = 2 * (4 * (DP / 32) + 2 * (DP / 16)) * 1024;
+    static_assert(lds <= 65536, "more LDS than a launch gets unasked");
+    const int64_t rows = static_cast<int64_t>(a.r.max_new) * (a.n_head / a.c.n_head_kv);
+    const dim3 grid(static_cast<unsigned>(seqs * static_cast<size_t>(a.c.n_head_kv)), static_cast<unsigned>((rows + 64 * RT - 1) / (64 * RT)),
+                    static_cast<unsigned>(a.n_split));
+    hipLaunchKernelGGL((kv8_rows_kernel<IO, DP, RT>), grid, dim3(256), lds, s, a);
+    const int st = check_launch("kv8_rows_kernel");
+    return st ? st : launch_join<IO, DP>(a, seqs, s);
+}
+
 template <typename IO, int DP, int NT>
 int launch_attend(const Attend8Args &a, size_t seqs, hipStream_t s) {
     constexpr size_t digits = 3 * NT * (DP / 64) * 1024, outputs = 4 * kJoin * (DP + 4) * sizeof(float);
@@ -506,42 +909,74 @@ int launch_attend(const Attend8Args &a, size_t seqs, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(seqs * static_cast<size_t>(a.c.n_head_kv)), static_cast<unsigned>((rows + 16 * NT - 1) / (16 * NT)),
                     static_cast<unsigned>(a.n_split));
     hipLaunchKernelGGL((kv8_attend_kernel<IO, DP, NT>), grid, dim3(256), lds, s, a);
-    int st = check_launch("kv8_attend_kernel");
-    if (st || a.n_split == 1) return st;
+    const int st = check_launch("kv8_attend_kernel");
+    return st ? st : launch_join<IO, DP>(a, seqs, s);
+}
+
+template <typename IO, int DP>
+int launch_join(const Attend8Args &a, size_t seqs, hipStream_t s) {
+    if (a.n_split == 1) return OURO_OK;
     const int64_t heads = static_cast<int64_t>(a.r.max_new) * a.n_head;
-    constexpr int DL = DP / 4, kMost = DL <= 64 ? 256 / DL : 1;
-    if (a.n_split > 4) {
-        hipLaunchKernelGGL((kv8_join_kernel<IO, DP, kMost>), dim3(static_cast<unsigned>(heads), 1, static_cast<unsigned>(seqs)), dim3(256), 0, s, a);
-    } else {
-        constexpr int PER = 256 / DL;
-        hipLaunchKernelGGL((kv8_join_kernel<IO, DP, 1>), dim3(static_cast<unsigned>((heads + PER - 1) / PER), 1, static_cast<unsigned>(seqs)),
+    // groups that can have work: a group takes kAhead splits at a time
+    constexpr int DL = DP / 4, kMost = 256 / DL, kSome = kMost < 4 ? kMost : 4;
+    auto go = [&](auto groups) {
+        constexpr int NG = decltype(groups)::value, PER = 256 / (NG * DL);
+        hipLaunchKernelGGL((kv8_join_kernel<IO, DP, NG>), dim3(static_cast<unsigned>((heads + PER - 1) / PER), 1, static_cast<unsigned>(seqs)),
                            dim3(256), 0, s, a);
-    }
+    };
+    if (a.n_split <= kAhead)
+        go(std::integral_constant<int, 1>{});
+    else if (a.n_split <= 4 * kAhead)
+        go(std::integral_constant<int, kSome>{});
+    else
+        go(std::integral_constant<int, kMost>{});
     return check_launch("kv8_join_kernel");
 }
 
 // The dims of a lane of V must divide the head: 192 only for its multiples of 12.
 int padded(size_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 && d % 12 == 0 ? 192 : 256; }
-// Tiles of 16 rows of a workgroup.
-int tiles_of(int64_t rows, int dp) { return rows <= 16 ? 1 : rows <= 32 || dp > 128 ? 2 : 4; }
-// Turns of 256 slots of a split: one where a sequence's rows are few and the splits
-// must fill the chip, more where many rows do; at most 1024 splits.
-int turns_of(int64_t rows, int nt, size_t max_len) {
-    int turns = rows <= 16 ? 1 : rows <= 16 * nt ? 2 : 16;
-    while ((max_len + static_cast<size_t>(turns) * kTurn - 1) / (static_cast<size_t>(turns) * kTurn) > 1024) turns *= 2;
-    return turns;
+
+// How a call goes, by the most rows that a sequence has of a kv head (new tokens
+// times query heads of it): never by how many sequences there are, so that a
+// sequence's bits do not depend on the batch it is in.
+struct Way {
+    int tiles;  // of 16 rows of a workgroup, or 0: kv8_rows_kernel
+    int turns;  // of 256 slots of a split
+};
+Way way_of(int64_t rows, int n_head_kv, int dp, int io_bytes, size_t max_len) {
+    Way w;
+    if (rows <= 16) {
+        // two turns: 64 sequences of 1024 slots 19 us (one turn 22, four 17), one of 16384
+        // 14.3 (13.0, 18.6); wider heads four: 32 of 4096 and 256 dims 51 us (two turns 61)
+        w = {1, dp <= 128 ? 2 : 4};
+    } else if (rows <= 256 || dp > 128) {
+        // 64 sequences of 2048 slots and 20 rows 38 us (one tile at best 43), 48 of 4096
+        // and 96 rows 58 (kv8_rows_kernel 56), 4 of 4096 and 256 rows 42 (45)
+        w = {2, dp <= 128 ? 4 : 8};
+    } else {
+        // splits until some 512 workgroups of a sequence's have work, of four to eight
+        // turns: one sequence of 16384 slots and 1024 rows 99 us with four (eight 119), one
+        // prompt of 4096 with 16384 rows 217 with eight (sixteen 250)
+        const int64_t groups = (rows + (io_bytes == 2 ? 127 : 63)) / (io_bytes == 2 ? 128 : 64) * n_head_kv;
+        const int64_t splits = groups < 512 ? 512 / groups : 1, all = static_cast<int64_t>((max_len + kTurn - 1) / kTurn);
+        const int64_t turns = (all + splits - 1) / splits;
+        w = {0, static_cast<int>(turns < 4 ? 4 : turns > 8 ? 8 : turns)};
+    }
+    // at most 1024 splits
+    while ((max_len + static_cast<size_t>(w.turns) * kTurn - 1) / (static_cast<size_t>(w.turns) * kTurn) > 1024) w.turns *= 2;
+    return w;
 }
 struct Attend8Ws {
-    int n_split, turns, tiles;
+    Way way;
+    int n_split;
     size_t part, bytes;
 };
-Attend8Ws attend_ws(size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len) {
+Attend8Ws attend_ws(size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len, int io_bytes) {
     Attend8Ws w{};
     // by the caller's max_new, whatever rows there are: a sequence alone goes the way that it goes with others
     const int64_t of_one = n_head_kv ? static_cast<int64_t>((max_new < (1u << 24) ? max_new : 1u << 24) * (n_head / n_head_kv)) : 0;
-    w.tiles = tiles_of(of_one, padded(d));
-    w.turns = turns_of(of_one, w.tiles, max_len);
-    const size_t slots = static_cast<size_t>(w.turns) * kTurn;
+    w.way = way_of(of_one, static_cast<int>(n_head_kv), padded(d), io_bytes, max_len);
+    const size_t slots = static_cast<size_t>(w.way.turns) * kTurn;
     w.n_split = max_len ? static_cast<int>((max_len + slots - 1) / slots) : 1;
     if (w.n_split == 1) return w;
     const size_t recs = rows * n_head * static_cast<size_t>(w.n_split);
@@ -553,8 +988,12 @@ Attend8Ws attend_ws(size_t rows, size_t max_new, size_t n_head, size_t n_head_kv
 template <typename IO>
 int launch_attend(const Attend8Args &a, size_t seqs, int tiles, hipStream_t s) {
     const int dp = padded(static_cast<size_t>(a.c.d));
-    if (dp == 64) return tiles == 1 ? launch_attend<IO, 64, 1>(a, seqs, s) : tiles == 2 ? launch_attend<IO, 64, 2>(a, seqs, s) : launch_attend<IO, 64, 4>(a, seqs, s);
-    if (dp == 128) return tiles == 1 ? launch_attend<IO, 128, 1>(a, seqs, s) : tiles == 2 ? launch_attend<IO, 128, 2>(a, seqs, s) : launch_attend<IO, 128, 4>(a, seqs, s);
+    // bf16 rows two tiles a wavefront; fp32 queries take twice the registers, and one
+    // tile (two sequences' 1024 rows over 16384 slots: 745 us, two tiles 754)
+    constexpr int RT = sizeof(IO) == 2 ? 2 : 1;
+    if (tiles == 0) return dp == 64 ? launch_rows<IO, 64, RT>(a, seqs, s) : launch_rows<IO, 128, RT>(a, seqs, s);
+    if (dp == 64) return tiles == 1 ? launch_attend<IO, 64, 1>(a, seqs, s) : launch_attend<IO, 64, 2>(a, seqs, s);
+    if (dp == 128) return tiles == 1 ? launch_attend<IO, 128, 1>(a, seqs, s) : launch_attend<IO, 128, 2>(a, seqs, s);
     if (dp == 192) return tiles == 1 ? launch_attend<IO, 192, 1>(a, seqs, s) : launch_attend<IO, 192, 2>(a, seqs, s);
     return tiles == 1 ? launch_attend<IO, 256, 1>(a, seqs, s) : launch_attend<IO, 256, 2>(a, seqs, s);
 }
@@ -567,7 +1006,10 @@ using namespace ouro;
 extern "C" {
 
 size_t ouro_kv8_attend_workspace_bytes(size_t, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t head_dim, size_t max_len) {
-    return attend_ws(rows, max_new, n_head, n_head_kv, head_dim, max_len).bytes;
+    // for rows of either type: the way may differ, and with it the splits
+    const size_t a = attend_ws(rows, max_new, n_head, n_head_kv, head_dim, max_len, 2).bytes;
+    const size_t b = attend_ws(rows, max_new, n_head, n_head_kv, head_dim, max_len, 4).bytes;
+    return a > b ? a : b;
 }
 
 int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride, const int32_t *lens, const int32_t *cu,
@@ -602,9 +1044,9 @@ int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
     a.q = q, a.gate = gate, a.mask = mask, a.out = out, a.lse = lse;
     a.q_stride = static_cast<int64_t>(q_stride), a.out_stride = static_cast<int64_t>(out_stride);
     a.mask_stride = static_cast<int64_t>(mask_stride);
-    a.n_head = static_cast<int>(n_head), a.window = most(window), a.sinks = most(sinks), a.scale = scale;
-    const Attend8Ws w = attend_ws(rows, max_new, n_head, hkv, d, max_len);
-    a.n_split = w.n_split, a.turns = w.turns;
+    a.n_head = static_cast<int>(n_head), a.window = window ? most(window) : 1 << 30, a.sinks = most(sinks), a.scale = scale;
+    const Attend8Ws w = attend_ws(rows, max_new, n_head, hkv, d, max_len, dtype == OURO_DT_F32 ? 4 : 2);
+    a.n_split = w.n_split, a.turns = w.way.turns;
     const size_t most_new = static_cast<size_t>(a.r.max_new);
     if (seqs * hkv >= (1u << 24) || most_new * (n_head / hkv) > (1u << 20) || most_new * n_head >= (1u << 24))
         return fail(OURO_ERR_SHAPE, "%s: %zu rows of one sequence of %zu heads, %zu sequences", me, most_new, n_head, seqs);
@@ -613,7 +1055,7 @@ int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
         a.ml = static_cast<float2 *>(ws);
         a.part = reinterpret_cast<float *>(static_cast<unsigned char *>(ws) + w.part);
     }
-    return dtype == OURO_DT_F32 ? launch_attend<float>(a, seqs, w.tiles, as_stream(stream)) : launch_attend<uint16_t>(a, seqs, w.tiles, as_stream(stream));
+    return dtype == OURO_DT_F32 ? launch_attend<float>(a, seqs, w.way.tiles, as_stream(stream)) : launch_attend<uint16_t>(a, seqs, w.way.tiles, as_stream(stream));
 }
 
 }  // extern "C"

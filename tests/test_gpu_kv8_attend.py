@@ -11,6 +11,11 @@ weight times the largest scale, at most n 2^-39 max |v| over n slots.  So the ou
 (2 ds + 600 U) sum p |v| + n 2^-39 max |v|, lse within ds + 600 U + 2 U |lse|.  A
 bf16 output adds its rounding, 2^-8 of its size, the gate 8 U.
 
+Where a sequence has more than 256 rows of a kv head (and heads of up to 128 dims)
+the queries are two fp16 operands, 2^-22 = 4 U of each value, and the sums over the
+dims are made in fp32: 2 * 128 products at most, and six roundings more, so that
+ds = (4 + 256 + 6) U |scale| sum |q k| there, the largest over the slots.
+
 A slot left out, or counted twice, moves the output by its weight, at 1 / n on
 average many times the bar at the lengths here."""
 import numpy as np
@@ -26,8 +31,8 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-def plain(q, k, v, seen, scale):
-    """(out, lse, S, sum p |v|) of one row's heads: q [hq][d], k and v [slots][hkv][d], seen [slots]."""
+def plain(q, k, v, seen, scale, many=False):
+    """(out, lse, ds / 8 U, sum p |v|) of one row's heads: q [hq][d], k and v [slots][hkv][d], seen [slots]."""
     hq, d = q.shape
     hkv = k.shape[1]
     out, lse, size, spread = np.zeros((hq, d)), np.full(hq, -np.inf), np.zeros(hq), np.zeros((hq, d))
@@ -42,7 +47,7 @@ def plain(q, k, v, seen, scale):
         lse[h] = m + np.log(p.sum())
         p /= p.sum()
         out[h], spread[h] = p @ v[:, g], p @ np.abs(v[:, g])
-        size[h] = abs(scale) * np.abs(q[h]).max() * np.abs(k[:, g]).sum(1).max()
+        size[h] = abs(scale) * (266 / 8 * (np.abs(k[:, g]) @ np.abs(q[h])).max() if many else np.abs(q[h]).max() * np.abs(k[:, g]).sum(1).max())
     return out, lse, size, spread
 
 
@@ -89,7 +94,7 @@ def check(seed, lens, counts, hq, hkv, d, page, block, *, bf16=False, layout="to
             if mask is not None:
                 seen &= mask[b, :n] != 0
             with np.errstate(invalid="ignore"):
-                o, l, size, spread = plain(dec(q[r, :hq * d]).reshape(hq, d), k, v, seen, sc)
+                o, l, size, spread = plain(dec(q[r, :hq * d]).reshape(hq, d), k, v, seen, sc, most * (hq // hkv) > 256 and d <= 128)
             ds = 8 * U * size
             got_o, got_l = dec(raw_o[r, :hq * d]).reshape(hq, d), raw_l[r].astype(np.float64)
             assert np.array_equal(np.isneginf(got_l), np.isneginf(l)), (b, i)
@@ -132,6 +137,34 @@ def test_drafted_tokens(gpu, bf16, hq, hkv, d, page, block):
 def test_prompts(gpu, bf16, hq, hkv, d):
     """Whole prompts and pieces of them, over many tiles of rows."""
     check(d, (150, 333, 70, 1), (150, 60, 33, 1), hq, hkv, d, 64, 64, bf16=bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hq,hkv,d,page,block,layout", [(4, 1, 64, 64, 64, "token"), (6, 2, 128, 16, 16, "head"), (8, 1, 80, 128, 32, "token"),
+                                                        (5, 1, 96, 32, 32, "head"), (3, 1, 16, 64, 16, "token"), (9, 3, 112, 256, 256, "token")])
+def test_many_rows(gpu, bf16, hq, hkv, d, page, block, layout):
+    """More than 256 rows of a kv head: whole prompts, pieces behind a context, a last tile of one row, sequences with few and none."""
+    G = hq // hkv
+    n = 257 // G + 1
+    check(d, (n, 700, 64 * 3, 1, 90, 0), (n, n - 1, 65, 1, 90, 0), hq, hkv, d, page, block, bf16=bf16, layout=layout, gate=True, gap=1, extra=1)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (33, 4), (200, 70), (1500, 0)])
+def test_many_rows_behind_windows(gpu, bf16, window, sinks):
+    """Stages that no row sees are not walked; masks and holes in those that some do."""
+    rng = np.random.default_rng(window)
+    mask = (rng.random((2, 2300)) < 0.8).astype(np.uint8)
+    mask[1, :400] = 0
+    check(window, (2300, 500), (70, 130), 8, 2, 64, 32, 16, window=window, sinks=sinks, bf16=bf16, mask=mask, holes=((0, 60, -1), (1, 13, -5)))
+    check(window + 1, (2300, 500), (70, 130), 4, 1, 128, 64, 64, window=window, sinks=sinks, bf16=bf16)
+
+
+def test_many_splits(gpu):
+    """Splits beyond those that one group of lanes joins at a time, of one row, of some and of many."""
+    check(40, (9000, 100), (1, 1), 2, 1, 64, 256, 256)
+    check(41, (9000, 5200), (9, 2), 2, 1, 64, 256, 64)
+    check(42, (17000,), (140,), 2, 1, 64, 256, 256, bf16=True)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 0), (17, 4), (100, 16), (64, 70), (300, 5), (5000, 3), (1 << 40, 0)])
