@@ -137,8 +137,15 @@ __device__ __forceinline__ bool sees(const Attend8Args &a, int at, int j0, int j
 // multiply-add, which takes the offset off: exact.  A weight, times its slot's
 // scale of V against the largest so far, is held in two fp16 (2^-22 of it, or 2^-40
 // of the largest); sums, maxima and outputs are fp32.
+//
+// Bound by memory where the splits fill the chip (128 sequences of 8192 slots, 4 kv
+// heads of 128: 228 us, 4.7 TB/s), below that by what a workgroup does before its
+// first products and after its last: one sequence of 300 slots takes 9 us. Four
+// wavefronts a SIMD instead of three (128 dims, 16 rows) spill and take 24 us for 64
+// sequences of 1024 slots instead of 19; 256 dims are held to two (51 -> 48 us for 32
+// of 4096); loads that bypass the caches take 59 us for 64 of 4096 instead of 51.
 template <typename IO, int DP, int NT>
-__global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 && NT == 1 ? 2 : 1))) void kv8_attend_kernel(Attend8Args a) {
     constexpr int NJ = DP / 64;                   // steps of the first product over the dims
     constexpr int CH = DP / 16;                   // adjacent dims of V a lane
     constexpr int VW = CH / 4;                    // and their dwords
