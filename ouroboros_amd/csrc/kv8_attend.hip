@@ -22,7 +22,6 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTurn = 256;  // slots that a workgroup's four wavefronts take in turn: 2 tiles of 32 each
-constexpr int kJoin = 8;    // rows that the wavefronts' outputs are joined for at a time
 
 struct Attend8Args {
     Kv8View c;
@@ -118,6 +117,9 @@ __device__ __forceinline__ bool sees(const Attend8Args &a, int at, int j0, int j
     return j0 <= at && (at + 1 - a.window < j1 || j0 < a.sinks);
 }
 
+// As many as fit 40 KiB.
+constexpr int joined_rows(int dp) { return dp <= 128 ? 16 : 8; }
+
 // One workgroup takes 16 NT rows (token by token, each token's query heads of one
 // kv head) of a sequence and kv head against a split of its slots, its four
 // wavefronts on alternate tiles of 32 slots, each with its own running maxima,
@@ -151,10 +153,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
     constexpr int VW = CH / 4;                    // and their dwords
     constexpr int LPR = NJ == 1 ? 4 : NJ == 2 ? 8 : 16;  // lanes that make a row's digits
     constexpr int OS = DP + 4;                    // floats of an output row in LDS: rows start in different banks
+    constexpr int kJoin = joined_rows(DP);        // rows that the wavefronts' outputs are joined for at a time
     constexpr int kRows = 16 * NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // digits [3][NT][NJ][64 lanes] of 16 bytes; later the outputs
     __shared__ float row_scale[kRows];
     __shared__ float sm[4][kRows], sl[4][kRows], sf[4];
+    __shared__ int2 place[kRows];                 // packed row and head of each
     typedef uint32_t vch_t __attribute__((ext_vector_type(VW)));
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -252,6 +256,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         load_v(j, 0, tile_bits(0) != 0);
     }
 
+    if (tid < kRows && row0 + tid < R) place[tid] = make_int2(s.first + (row0 + tid) / G, kvh * G + (row0 + tid) % G);
     // The rows' digits.  A negative scale goes into their sign, so that a row's
     // largest score is that of its largest sum.
     const bool negative = a.scale < 0.f;
@@ -296,7 +301,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int rho = row0 + 16 * t + r;
-        at[t] = rho < R ? before + rho / G : -1;
+        at[t] = rho < R ? before + place[16 * t + r].x - s.first : -1;
         m[t] = -INFINITY, l[t] = 0.f, qs[t] = row_scale[16 * t + r];
 #pragma unroll
         for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -439,48 +444,65 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         }
     }
 
-    // the four wavefronts' outputs joined, kJoin rows at a time
+    // The four wavefronts' outputs joined, kJoin rows at a time: first what each
+    // wavefront's are to be taken by, a row a thread, then four dims a thread.
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const float sum = quad_sum(l[t]);
         if (g == 0) sm[wave][16 * t + r] = m[t], sl[wave][16 * t + r] = sum;
     }
     if (lane == 0) sf[wave] = v_top * 0.015625f;
+    __syncthreads();  // and the digits have been read
+    if (tid < kRows && row0 + tid < R) {
+        const float M = fmaxf(fmaxf(sm[0][tid], sm[1][tid]), fmaxf(sm[2][tid], sm[3][tid])), ref = M == -INFINITY ? 0.f : M;
+        float L = 0.f, f[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(sm[w][tid] - ref);
+            L += f[w] * sl[w][tid];
+        }
+        const int64_t row = place[tid].x;
+        const int h = place[tid].y;
+        const float norm = !whole ? 1.f : L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sm[w][tid] = f[w] * sf[w] * norm;
+        if (whole)
+            store_lse(a, row, h, M, L);
+        else
+            a.ml[(row * a.n_head + h) * a.n_split + split] = make_float2(M, L);
+    }
     float *const ob = reinterpret_cast<float *>(lds);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int q0 = 16 * t + kJoin * half;
+        for (int k = 0; k < 16 / kJoin; ++k) {
+            const int q0 = 16 * t + kJoin * k;
             if (row0 + q0 >= R) continue;  // whole workgroup
-            __syncthreads();  // the digits, or the rows before, have been read
-            if (r / kJoin == half) {
+            if (q0) __syncthreads();  // the rows before have been read
+            if (r / kJoin == k) {
                 float *row = ob + (wave * kJoin + r % kJoin) * OS + 4 * g;
 #pragma unroll
                 for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * e) = o[t][e];
             }
             __syncthreads();
-            for (int i = tid; i < kJoin * DP; i += 256) {
-                const int q = q0 + i / DP, dim = i % DP, rho = row0 + q;
-                if (dim >= d || rho >= R) continue;
-                const float M = fmaxf(fmaxf(sm[0][q], sm[1][q]), fmaxf(sm[2][q], sm[3][q]));
-                float L = 0.f, x = 0.f;
+            for (int i = tid; i < kJoin * DP / 4; i += 256) {
+                const int q = q0 + i / (DP / 4), dim = i % (DP / 4) * 4;
+                if (dim >= d || row0 + q >= R) continue;
+                f32x4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(sm[w][q] - (M == -INFINITY ? 0.f : M));
-                    L += f * sl[w][q];
-                    x += f * sf[w] * ob[(w * kJoin + q - q0) * OS + dim % CH * 16 + dim / CH];
+                    const float f = sm[w][q];
+                    const float *from = ob + (w * kJoin + q - q0) * OS;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] += f * from[(dim + e) % CH * 16 + (dim + e) / CH];
                 }
-                const int64_t row = s.first + rho / G;
-                const int h = kvh * G + rho % G;
-                if (whole) {
-                    store_out<IO>(a, row, h, dim, L == 0.f ? 0.f : x / L);
-                    if (dim == 0) store_lse(a, row, h, M, L);
-                } else {
-                    const int64_t rec = (row * a.n_head + h) * a.n_split + split;
-                    if (dim == 0) a.ml[rec] = make_float2(M, L);
-                    a.part[rec * d + dim] = x;
-                }
+                const int64_t row = place[q].x;
+                const int h = place[q].y;
+                if (whole)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, x[e]);
+                else
+                    *reinterpret_cast<f32x4_t *>(a.part + ((row * a.n_head + h) * a.n_split + split) * d + dim) = x;
             }
         }
 }
@@ -909,7 +931,7 @@ int launch_rows(const Attend8Args &a, size_t seqs, hipStream_t s) {
 
 template <typename IO, int DP, int NT>
 int launch_attend(const Attend8Args &a, size_t seqs, hipStream_t s) {
-    constexpr size_t digits = 3 * NT * (DP / 64) * 1024, outputs = 4 * kJoin * (DP + 4) * sizeof(float);
+    constexpr size_t digits = 3 * NT * (DP / 64) * 1024, outputs = 4 * joined_rows(DP) * (DP + 4) * sizeof(float);
     constexpr size_t lds = digits > outputs ? digits : outputs;
     static_assert(lds + 4096 <= 65536, "more LDS than a launch gets unasked");
     const int64_t rows = static_cast<int64_t>(a.r.max_new) * (a.n_head / a.c.n_head_kv);
