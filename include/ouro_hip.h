@@ -669,8 +669,8 @@ typedef struct ouro_kv8_cache {
  * came, and a row's error is at most half a step when it is written and less
  * than half of the present step more by later growth.  A NaN is held as 0, an
  * infinity as +-127 steps of what finite values need (as 0 where all are 0), a
- * block of zeros has scale 0.  Other slots keep their codes.  Two sequences must
- * not write to one page in a call; rows of a hole are dropped. */
+ * block of zeros has scale 0.  Other slots keep their codes.  A page that gets
+ * rows in a call stands once in the page table; rows of a hole are dropped. */
 int ouro_kv8_write(const ouro_kv8_cache *cache, const void *k_new,
                    const void *v_new, size_t new_stride, int dtype,
                    const int32_t *lens, const int32_t *cu, size_t seqs,

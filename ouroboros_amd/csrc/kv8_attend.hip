@@ -516,6 +516,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 // (2^-22 of a value), and the scores are summed in fp32: the codes' exact products
 // of three digits cost a third more matrix instructions and four conversions a
 // score.
+//
+// Bound by issue: of 512 us for two pieces of 1024 bf16 rows over up to 16384 slots
+// (250 GFLOP, 0.49 PFLOP/s) the matrix instructions are 149 and the others 215 (138
+// for each 16 rows and 32 slots, 45 of them the staging), and on the two wavefronts
+// of a SIMD they hardly overlap: a form that interleaves one half's products with the
+// other's weights took 67 registers too many and 669 us, one that reads operands ahead
+// 593, a raised priority around the products changed nothing.
 template <typename IO, int DP, int RT>
 __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
     constexpr int NC = DP / 32;                // steps of the first product over the dims
@@ -588,13 +595,17 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
                                       : 0;
             const uint32_t step = there ? static_cast<uint32_t>(a.c.token_stride) : 0u;
             if (wave >= 2) {
+                const int8_t *const base = kp + row;
+                const uint32_t off = static_cast<uint32_t>(r) * step;
 #pragma unroll
                 for (int i = 0; i < NJ; ++i)
-                    raw[u * NJ + i] = *reinterpret_cast<const u32x4_t *>(kp + row + (static_cast<uint32_t>(r) * step + static_cast<uint32_t>(min(16 * (4 * i + g), d - 16))));
+                    raw[u * NJ + i] = *reinterpret_cast<const u32x4_t *>(base + (off + static_cast<uint32_t>(min(16 * (4 * i + g), d - 16))));
             } else {
+                const int8_t *const base = vp + row;
+                const uint32_t off = 4 * static_cast<uint32_t>(g) * step + static_cast<uint32_t>(min(CH * r, d - CH));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const vch_t v = *reinterpret_cast<const vch_t *>(vp + row + (static_cast<uint64_t>(4 * g + i) * step + static_cast<uint32_t>(min(CH * r, d - CH))));
+                    const vch_t v = *reinterpret_cast<const vch_t *>(base + static_cast<uint64_t>(i) * step + off);
 #pragma unroll
                     for (int w = 0; w < VW; ++w) raw[(VW * (4 * u + i) + w) / 4][(VW * (4 * u + i) + w) % 4] = v[w];
                 }
@@ -983,13 +994,14 @@ Way way_of(int64_t rows, int n_head_kv, int dp, int io_bytes, size_t max_len) {
         // and 96 rows 58 (kv8_rows_kernel 56), 4 of 4096 and 256 rows 42 (45)
         w = {2, dp <= 128 ? 4 : 8};
     } else {
-        // splits until some 512 workgroups of a sequence's have work, of four to eight
-        // turns: one sequence of 16384 slots and 1024 rows 99 us with four (eight 119), one
-        // prompt of 4096 with 16384 rows 217 with eight (sixteen 250)
+        // splits until some 512 workgroups of a sequence's have work, and four at least, of
+        // four to sixteen turns: one sequence of 16384 slots and 1024 rows 99 us with four
+        // turns (eight 119), two of 4096 rows 528 with sixteen (eight 547, thirty-two 512),
+        // one prompt of 4096 tokens, 16384 rows, 211 with four (eight 217, sixteen 250)
         const int64_t groups = (rows + (io_bytes == 2 ? 127 : 63)) / (io_bytes == 2 ? 128 : 64) * n_head_kv;
-        const int64_t splits = groups < 512 ? 512 / groups : 1, all = static_cast<int64_t>((max_len + kTurn - 1) / kTurn);
+        const int64_t splits = groups < 128 ? 512 / groups : 4, all = static_cast<int64_t>((max_len + kTurn - 1) / kTurn);
         const int64_t turns = (all + splits - 1) / splits;
-        w = {0, static_cast<int>(turns < 4 ? 4 : turns > 8 ? 8 : turns)};
+        w = {0, static_cast<int>(turns < 4 ? 4 : turns > 16 ? 16 : turns)};
     }
     // at most 1024 splits
     while ((max_len + static_cast<size_t>(w.turns) * kTurn - 1) / (static_cast<size_t>(w.turns) * kTurn) > 1024) w.turns *= 2;

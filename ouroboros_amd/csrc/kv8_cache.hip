@@ -108,6 +108,10 @@ __device__ __forceinline__ uint32_t code_of(float x, float r) {
 // head and of keys or values: its new rows into registers, NC pieces of eight
 // values a thread, their largest magnitude, the scale, the codes.  Only where the
 // block holds older rows and its scale grew are they read and written.
+//
+// 32 prompts of up to 2048 rows, bf16, blocks of 16: 32 us, 3.9 TB/s where a copy has
+// 5 (a wavefront a block; four blocks a workgroup 33).  64 single rows 4.5 us on the
+// GPU: lengths, page, old scale and rows are loads that wait for each other.
 template <typename T, int U, int NC>
 __global__ __launch_bounds__(U) void kv8_write_kernel(WriteArgs a) {
     __shared__ float top[U / 64];
@@ -208,7 +212,8 @@ struct ReadArgs {
 static_assert(sizeof(ReadArgs) == 144, "ReadArgs: kernel argument layout");
 
 // A thread makes 16 bytes of the output, four or eight codes of a row and head, of
-// kReadRows rows, whose loads are on their way together.
+// kReadRows rows, whose loads are on their way together: 48 contexts of up to 2048
+// rows to bf16 38 us, 4.4 TB/s where a copy has 5 (one row at a time 52).
 constexpr int kReadRows = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a, int per_row) {

@@ -99,6 +99,11 @@ __device__ __forceinline__ void store(T *p, const float (&x)[E]) {
 // past n_rot two pieces in a row.  The angles of a token are the same for all of
 // its heads: they are made once, by as many threads as it has pairs, and a group
 // of G lanes stays with one token and keeps its angles and gains in registers.
+//
+// 16385 rows of 20 heads of 128, bf16: 47 us, 3.6 TB/s where a copy has 5, bound by
+// the five wavefronts a SIMD that 95 registers leave (eight tokens a workgroup; with
+// the angles and a division a head made anew 73).  64 fp32 rows take 4.6 us, a part of
+// a token's heads a workgroup: three dependent loads and the angles.
 template <typename T, int E, int G>
 __global__ __launch_bounds__(kThreads) void qk_rope_kernel(RopeArgs a) {
     __shared__ __attribute__((aligned(16))) float cs[kMaxTokens][kMaxHalf], sn[kMaxTokens][kMaxHalf];
