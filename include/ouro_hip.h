@@ -700,7 +700,8 @@ int ouro_kv8_read(const ouro_kv8_cache *cache, const int32_t *lens,
  *   max_len bounds lens, at most 2^30.
  * A stride of 0 stands for rows without a gap.  `workspace`:
  * ouro_kv8_attend_workspace_bytes() device bytes, 16-byte aligned; NULL takes
- * the library's. */
+ * the library's.  The bytes are enough for every call of the same heads with no
+ * more sequences, rows, new rows of a sequence or slots. */
 size_t ouro_kv8_attend_workspace_bytes(size_t seqs, size_t rows, size_t max_new,
                                        size_t n_head, size_t n_head_kv,
                                        size_t head_dim, size_t max_len);

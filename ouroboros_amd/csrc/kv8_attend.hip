@@ -30,14 +30,20 @@ struct Attend8Args {
     const uint8_t *mask;
     void *out;
     float *lse;
-    float *part;  // [rows][n_head][n_split][d]: the splits' outputs, not normalised
-    float2 *ml;   // [rows][n_head][n_split]: their maxima (of scores times log2 e) and sums
+    float *part;  // [records][n_head][n_split][d]: the splits' outputs, not normalised
+    float2 *ml;   // [records][n_head][n_split]: their maxima (of scores times log2 e) and sums
     int64_t q_stride, mask_stride, out_stride;
     int32_t n_head, window, sinks;  // window 2^30: every slot
     float scale;
     int32_t n_split, turns;  // turns of a split
+    int32_t by_seq;          // records: max_new of each sequence, or else one of each packed row
 };
-static_assert(sizeof(Attend8Args) == 224, "Attend8Args: kernel argument layout");
+static_assert(sizeof(Attend8Args) == 232, "Attend8Args: kernel argument layout");
+
+// What a packed row of sequence b is off from its record.
+__device__ __forceinline__ int64_t record_shift(const Attend8Args &a, int64_t b, const SeqRows &s) {
+    return a.by_seq ? b * a.r.max_new - s.first : 0;
+}
 
 template <typename T>
 __device__ __forceinline__ float load1(const T *p, int64_t i) {
@@ -446,6 +452,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 
     // The four wavefronts' outputs joined, kJoin rows at a time: first what each
     // wavefront's are to be taken by, a row a thread, then four dims a thread.
+    const int64_t shift = record_shift(a, b, s);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const float sum = quad_sum(l[t]);
@@ -469,7 +476,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         if (whole)
             store_lse(a, row, h, M, L);
         else
-            a.ml[(row * a.n_head + h) * a.n_split + split] = make_float2(M, L);
+            a.ml[((row + shift) * a.n_head + h) * a.n_split + split] = make_float2(M, L);
     }
     float *const ob = reinterpret_cast<float *>(lds);
 #pragma unroll
@@ -502,7 +509,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 #pragma unroll
                     for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, x[e]);
                 else
-                    *reinterpret_cast<f32x4_t *>(a.part + ((row * a.n_head + h) * a.n_split + split) * d + dim) = x;
+                    *reinterpret_cast<f32x4_t *>(a.part + (((row + shift) * a.n_head + h) * a.n_split + split) * d + dim) = x;
             }
         }
 }
@@ -823,6 +830,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
         k_sc = k_raw, v_sc = v_raw;
         __syncthreads();
     }
+    const int64_t shift = record_shift(a, b, s);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const float L = quad_sum(l[t]);
@@ -831,7 +839,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
         const int64_t row = s.first + rho / G;
         const int h = kvh * G + rho % G;
         const float unit = v_top * 0.015625f;  // outputs are in units of V's largest scale, times 2^6
-        const int64_t rec = (row * a.n_head + h) * a.n_split + split;
+        const int64_t rec = ((row + shift) * a.n_head + h) * a.n_split + split;
         if (g == 0) {
             if (whole)
                 store_lse(a, row, h, m[t], L);
@@ -877,7 +885,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
     const bool live = who < PER && i < s.count;
     if (PER == 1 && !live) return;  // whole workgroup
     const int at = s.n - s.count + i, d = a.c.d;
-    const int64_t row = s.first + i, rec = (row * a.n_head + h) * a.n_split;
+    const int64_t row = s.first + i, rec = ((row + record_shift(a, b, s)) * a.n_head + h) * a.n_split;
     f32x4_t x = {0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
     if (live)
@@ -980,50 +988,95 @@ int padded(size_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 && d % 12
 // times query heads of it): never by how many sequences there are, so that a
 // sequence's bits do not depend on the batch it is in.
 struct Way {
-    int tiles;  // of 16 rows of a workgroup, or 0: kv8_rows_kernel
-    int turns;  // of 256 slots of a split
+    int tiles;   // of 16 rows of a workgroup, or 0: kv8_rows_kernel
+    int turns;   // of 256 slots of a split
+    int splits;  // no more for any shorter max_len
 };
+constexpr int kFewRows = 16, kSomeRows = 256, kMostSplits = 1024;
+// kv8_rows_kernel: of a kv head's rows a workgroup has, and how often its grid is split
+constexpr int group_rows(int io_bytes) { return io_bytes == 2 ? 128 : 64; }
+constexpr int kManyGroups = 512, kLeastSplits = 4;
 Way way_of(int64_t rows, int n_head_kv, int dp, int io_bytes, size_t max_len) {
     Way w;
-    if (rows <= 16) {
+    const int64_t all = static_cast<int64_t>((max_len + kTurn - 1) / kTurn);
+    if (rows <= kFewRows) {
         // two turns: 64 sequences of 1024 slots 19 us (one turn 22, four 17), one of 16384
         // 14.3 (13.0, 18.6); wider heads four: 32 of 4096 and 256 dims 51 us (two turns 61)
-        w = {1, dp <= 128 ? 2 : 4};
-    } else if (rows <= 256 || dp > 128) {
+        w = {1, dp <= 128 ? 2 : 4, 0};
+    } else if (rows <= kSomeRows || dp > 128) {
         // 64 sequences of 2048 slots and 20 rows 38 us (one tile at best 43), 48 of 4096
         // and 96 rows 58 (kv8_rows_kernel 56), 4 of 4096 and 256 rows 42 (45)
-        w = {2, dp <= 128 ? 4 : 8};
+        w = {2, dp <= 128 ? 4 : 8, 0};
     } else {
         // splits until some 512 workgroups of a sequence's have work, and four at least, of
         // four to sixteen turns: one sequence of 16384 slots and 1024 rows 99 us with four
         // turns (eight 119), two of 4096 rows 528 with sixteen (eight 547, thirty-two 512),
         // one prompt of 4096 tokens, 16384 rows, 211 with four (eight 217, sixteen 250)
-        const int64_t groups = (rows + (io_bytes == 2 ? 127 : 63)) / (io_bytes == 2 ? 128 : 64) * n_head_kv;
-        const int64_t splits = groups < 128 ? 512 / groups : 4, all = static_cast<int64_t>((max_len + kTurn - 1) / kTurn);
-        const int64_t turns = (all + splits - 1) / splits;
-        w = {0, static_cast<int>(turns < 4 ? 4 : turns > 16 ? 16 : turns)};
+        const int64_t groups = (rows + group_rows(io_bytes) - 1) / group_rows(io_bytes) * n_head_kv;
+        const int64_t splits = groups * kLeastSplits < kManyGroups ? kManyGroups / groups : kLeastSplits;
+        const int64_t turns = (all + splits - 1) / splits, least = (all + 15) / 16, most = (all + 3) / 4;
+        w = {0, static_cast<int>(turns < 4 ? 4 : turns > 16 ? 16 : turns), 0};
+        // turns go up in whole ones, and the splits of a longer max_len can be fewer
+        const int64_t bound = splits > least ? splits : least;
+        w.splits = static_cast<int>(bound < most ? bound : most);
     }
-    // at most 1024 splits
-    while ((max_len + static_cast<size_t>(w.turns) * kTurn - 1) / (static_cast<size_t>(w.turns) * kTurn) > 1024) w.turns *= 2;
+    if (w.tiles) w.splits = static_cast<int>((all + w.turns - 1) / w.turns);
+    if (w.splits > kMostSplits) w.splits = kMostSplits;
+    while ((all + w.turns - 1) / w.turns > kMostSplits) w.turns *= 2;
     return w;
 }
 struct Attend8Ws {
     Way way;
     int n_split;
+    bool by_seq;
     size_t part, bytes;
 };
-Attend8Ws attend_ws(size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len, int io_bytes) {
+// Records are of the packed rows or of max_new rows of each sequence, whichever are fewer.
+size_t records_bytes(size_t rows, size_t seqs, size_t max_new, size_t n_head, size_t d, int splits, size_t *part) {
+    if (splits < 2) return 0;
+    const size_t recs = (seqs * max_new < rows ? seqs * max_new : rows) * n_head * static_cast<size_t>(splits);
+    *part = (recs * sizeof(float2) + 255) & ~size_t{255};
+    return *part + recs * d * sizeof(float);
+}
+// A sequence's rows of a kv head, of the caller's max_new, whatever rows there are: a
+// sequence alone goes the way that it goes with others.
+int64_t rows_of_one(size_t max_new, size_t n_head, size_t n_head_kv) {
+    return static_cast<int64_t>((max_new < (1u << 24) ? max_new : 1u << 24) * (n_head / n_head_kv));
+}
+Attend8Ws attend_ws(size_t seqs, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len, int io_bytes) {
     Attend8Ws w{};
-    // by the caller's max_new, whatever rows there are: a sequence alone goes the way that it goes with others
-    const int64_t of_one = n_head_kv ? static_cast<int64_t>((max_new < (1u << 24) ? max_new : 1u << 24) * (n_head / n_head_kv)) : 0;
-    w.way = way_of(of_one, static_cast<int>(n_head_kv), padded(d), io_bytes, max_len);
+    w.way = way_of(rows_of_one(max_new, n_head, n_head_kv), static_cast<int>(n_head_kv), padded(d), io_bytes, max_len);
     const size_t slots = static_cast<size_t>(w.way.turns) * kTurn;
     w.n_split = max_len ? static_cast<int>((max_len + slots - 1) / slots) : 1;
-    if (w.n_split == 1) return w;
-    const size_t recs = rows * n_head * static_cast<size_t>(w.n_split);
-    w.part = (recs * sizeof(float2) + 255) & ~size_t{255};
-    w.bytes = w.part + recs * d * sizeof(float);
+    if (max_new > rows) max_new = rows;
+    w.by_seq = seqs * max_new < rows;
+    w.bytes = records_bytes(rows, seqs, max_new, n_head, d, w.n_split, &w.part);
     return w;
+}
+
+// The most that a call of no more rows, new ones of a sequence or slots can take, in
+// either type: fewer rows of a sequence can go a way of more splits.  Records grow
+// with max_new while the way's splits are the same, so what counts is the largest
+// max_new of each: of few rows, of some, of each number of groups that is split anew.
+size_t attend_most(size_t seqs, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len) {
+    if (!n_head_kv || n_head < n_head_kv || seqs > 65535 || rows > (1u << 23)) return 0;
+    const size_t G = n_head / n_head_kv;
+    size_t most = 0;
+    auto see = [&](size_t of_one, int io_bytes) {  // rows of a kv head
+        const size_t t = of_one / G < max_new ? of_one / G : max_new;
+        size_t part;
+        const Way w = way_of(rows_of_one(t, n_head, n_head_kv), static_cast<int>(n_head_kv), padded(d), io_bytes, max_len);
+        const size_t b = records_bytes(rows, seqs, t < rows ? t : rows, n_head, d, w.splits, &part);
+        if (b > most) most = b;
+    };
+    for (int io_bytes : {2, 4}) {
+        see(kFewRows, io_bytes);
+        see(kSomeRows, io_bytes);
+        for (size_t g = 1; g * n_head_kv * kLeastSplits < kManyGroups + n_head_kv * kLeastSplits; ++g)
+            see(g * static_cast<size_t>(group_rows(io_bytes)), io_bytes);
+        see(max_new < (1u << 24) ? max_new * G : static_cast<size_t>(1u << 24) * G, io_bytes);
+    }
+    return most;
 }
 
 template <typename IO>
@@ -1046,11 +1099,9 @@ using namespace ouro;
 
 extern "C" {
 
-size_t ouro_kv8_attend_workspace_bytes(size_t, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t head_dim, size_t max_len) {
-    // for rows of either type: the way may differ, and with it the splits
-    const size_t a = attend_ws(rows, max_new, n_head, n_head_kv, head_dim, max_len, 2).bytes;
-    const size_t b = attend_ws(rows, max_new, n_head, n_head_kv, head_dim, max_len, 4).bytes;
-    return a > b ? a : b;
+size_t ouro_kv8_attend_workspace_bytes(size_t seqs, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t head_dim,
+                                       size_t max_len) {
+    return attend_most(seqs, rows, max_new, n_head, n_head_kv, head_dim, max_len);
 }
 
 int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride, const int32_t *lens, const int32_t *cu,
@@ -1086,8 +1137,8 @@ int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
     a.q_stride = static_cast<int64_t>(q_stride), a.out_stride = static_cast<int64_t>(out_stride);
     a.mask_stride = static_cast<int64_t>(mask_stride);
     a.n_head = static_cast<int>(n_head), a.window = window ? most(window) : 1 << 30, a.sinks = most(sinks), a.scale = scale;
-    const Attend8Ws w = attend_ws(rows, max_new, n_head, hkv, d, max_len, dtype == OURO_DT_F32 ? 4 : 2);
-    a.n_split = w.n_split, a.turns = w.way.turns;
+    const Attend8Ws w = attend_ws(seqs, rows, max_new, n_head, hkv, d, max_len, dtype == OURO_DT_F32 ? 4 : 2);
+    a.n_split = w.n_split, a.turns = w.way.turns, a.by_seq = w.by_seq;
     const size_t most_new = static_cast<size_t>(a.r.max_new);
     if (seqs * hkv >= (1u << 24) || most_new * (n_head / hkv) > (1u << 20) || most_new * n_head >= (1u << 24))
         return fail(OURO_ERR_SHAPE, "%s: %zu rows of one sequence of %zu heads, %zu sequences", me, most_new, n_head, seqs);

@@ -125,7 +125,8 @@ class KVCache8:
 
 def attend8_workspace_bytes(seqs: int, rows: int, max_new: int, n_head: int, n_head_kv: int, head_dim: int,
                             max_len: int) -> int:
-    """Bytes of scratch that KVCache8.attend takes (0 = none)."""
+    """Bytes of scratch that KVCache8.attend takes (0 = none), enough also for calls of fewer sequences, rows, new rows
+    of a sequence or slots."""
     return int(_lib.lib().ouro_kv8_attend_workspace_bytes(seqs, rows, max_new, n_head, n_head_kv, head_dim, max_len))
 
 

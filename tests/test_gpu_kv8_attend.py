@@ -52,13 +52,14 @@ def plain(q, k, v, seen, scale, many=False):
 
 
 def check(seed, lens, counts, hq, hkv, d, page, block, *, bf16=False, layout="token", window=0, sinks=0, mask=None, gate=False, holes=(),
-          gap=0, extra=0, uniform=False, max_len=None, q_scale=1.0, v_size=1.0, scale=None, workspace=False, stream=None):
+          gap=0, extra=0, uniform=False, max_len=None, q_scale=1.0, v_size=1.0, scale=None, workspace=0, behind=0, stream=None):
     B, L = len(lens), max(max(lens), 1) if max_len is None else max_len
     t = Cache8(seed, B, L, hkv, d, page, block, layout, holes, gap)
     t.fill([min(n, L) for n in lens], v_size)
     rng, unit = t.rng, 8 if bf16 else 4
     cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
-    rows, most = int(cu[-1]), max(counts)
+    used, most = int(cu[-1]), max(counts)
+    rows = used + behind
     qs, os_ = hq * d + extra * unit, hq * d + 2 * extra * unit
     q = enc(q_scale * rng.standard_normal((rows + 1, qs)), bf16)
     gt = enc(rng.standard_normal((rows + 1, qs)), bf16)
@@ -68,7 +69,7 @@ def check(seed, lens, counts, hq, hkv, d, page, block, *, bf16=False, layout="to
     up = DeviceBuffer.from_host
     mb = None if mask is None else up(np.ascontiguousarray(np.pad(mask, ((0, 0), (0, 5)), constant_values=1), np.uint8))
     held = up(q), up(gt), up(np.array(lens, np.int32)), up(cu)
-    need = attend8_workspace_bytes(B, rows, most, hq, hkv, d, L)
+    need = workspace if workspace > 1 else attend8_workspace_bytes(B, rows, most, hq, hkv, d, L)
     ws = DeviceBuffer.from_host(np.full(max(need, 1) + 256, 0xa5, np.uint8)) if workspace else None
     c.attend(held[0], out, held[2], B, rows, most, L, hq, cu=None if uniform else held[3], dtype=name(bf16), window=window,
              sinks=sinks, mask=mb, mask_stride=L + 5 if mask is not None else 0, gate=held[1] if gate else None, lse=lse, scale=scale,
@@ -78,7 +79,7 @@ def check(seed, lens, counts, hq, hkv, d, page, block, *, bf16=False, layout="to
     raw_o, raw_l = out.download(), lse.download()
     if ws is not None:
         assert (ws.download()[max(need, 1):] == 0xa5).all(), "past its workspace"
-    assert (raw_o[rows:] == 9).all() and (raw_l[rows:] == 9).all() and (raw_o[:, hq * d:] == 9).all()
+    assert (raw_o[used:] == 9).all() and (raw_l[used:] == 9).all() and (raw_o[:, hq * d:] == 9).all()
     sc = d ** -0.5 if scale is None else scale
     worst = 0.0
     for b in range(B):
@@ -202,6 +203,19 @@ def test_gate_strides_and_workspace(gpu, bf16):
     for counts in ((1, 1, 1), (3, 2, 4), (100, 20, 90)):
         check(9, (400, 20, 900), counts, 8, 2, 64, 64, 32, bf16=bf16, gate=True, gap=1, extra=1, workspace=True)
         check(10, (400, 20, 900), counts, 4, 4, 128, 64, 64, bf16=bf16, workspace=True, max_len=1000, stream=s.handle)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_one_workspace_for_shorter_calls(gpu, bf16):
+    """A workspace of the most rows and slots serves fewer, also where the packed arrays stay as long as for the most."""
+    for hq, hkv, d, most in ((8, 2, 64, 5), (4, 2, 128, 140), (4, 1, 192, 70)):
+        need = attend8_workspace_bytes(3, 3 * most, most, hq, hkv, d, 2300)
+        for counts in ((1, 1, 1), (4, 2, 4), (5, 5, 1), (70, 1, 30), (most, 1, most)):
+            if max(counts) > most:
+                continue
+            for L in (2300, 1100):
+                for behind in (0, 3 * most - sum(counts)):
+                    check(21, (L, 5, L - 40), counts, hq, hkv, d, 64, 32, bf16=bf16, workspace=need, max_len=L, behind=behind)
 
 
 @pytest.mark.parametrize("q_scale,size,scale", [(30.0, 1.0, None), (1e20, 1e-20, None), (1e-18, 1e18, None), (1.0, 1.0, -0.3), (2.0, 1.0, 0.0)])

@@ -40,3 +40,20 @@ def test_attend_workspace(seqs, rows, max_new, heads, kv, d, max_len):
     most = -(-max_len // 256)
     assert got <= rows * heads * most * (d + 2) * 4 + 256
     assert got == 0 if max_len <= 256 or not rows else got >= rows * heads * 2 * (d + 2) * 4
+
+
+@pytest.mark.parametrize("heads,kv,d", [(16, 4, 128), (32, 2, 64), (4, 4, 192), (8, 1, 128), (48, 1, 64)])
+def test_attend_workspace_serves_shorter_calls(heads, kv, d):
+    """Never less for more sequences, rows, new rows of a sequence or slots."""
+    def need(seqs, rows, new, slots):
+        return kvcache.attend8_workspace_bytes(seqs, rows, new, heads, kv, d, slots)
+
+    for slots in (300, 5000, 40000):
+        for grow in (lambda n: (3, 500, n, slots), lambda n: (3, 3 * n, n, slots)):
+            sizes = [need(*grow(n)) for n in [*range(0, 400), *range(400, 3000, 37)]]
+            assert sizes == sorted(sizes)
+    for new in (1, 4, 5, 64, 300, 1024):
+        sizes = [need(2, 2 * new, new, n) for n in [*range(0, 3000, 61), *range(3000, 300000, 1777)]]
+        assert sizes == sorted(sizes)
+        sizes = [need(n, 700, new, 9000) for n in range(0, 900)]
+        assert sizes == sorted(sizes)
