@@ -123,6 +123,15 @@ __device__ __forceinline__ bool sees(const Attend8Args &a, int at, int j0, int j
     return j0 <= at && (at + 1 - a.window < j1 || j0 < a.sinks);
 }
 
+// Of the slots j0 .. j1 - 1 of a split, seen by some of the rows in slots at_min ..
+// at_max: the last that is walked through, and the first, a multiple of `step` away.
+__device__ __forceinline__ int seen_end(const Attend8Args &a, int at_min, int at_max, int j1) {
+    return min(at_min + 1 - a.window >= j1 ? min(j1, a.sinks) : j1, at_max + 1);
+}
+__device__ __forceinline__ int seen_begin(const Attend8Args &a, int at_min, int j0, int step) {
+    return j0 < a.sinks ? j0 : j0 + max(at_min + 1 - a.window - j0, 0) / step * step;
+}
+
 // As many as fit 40 KiB.
 constexpr int joined_rows(int dp) { return dp <= 128 ? 16 : 8; }
 
@@ -171,7 +180,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
     const int kvh = static_cast<int>(blockIdx.x) % a.c.n_head_kv;
     const int64_t b = static_cast<int64_t>(blockIdx.x) / a.c.n_head_kv;
     const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
-    const int split = blockIdx.z, first_slot = split * a.turns * kTurn;
+    const int split = blockIdx.z, split_first = split * a.turns * kTurn;
     // Lane l of wavefront w stands for slot 32 (w + 4 (l / 32)) + l % 32 of a turn:
     // the wavefront's own tiles, whose pages, scales and visible slots stay in its
     // registers.  A turn's page ids and mask are read without waiting for the length.
@@ -185,16 +194,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         id = pages[j >> a.c.page_shift];
         if (a.mask) kept = a.mask[b * a.mask_stride + j];
     };
-    fetch(first_slot + mine);
+    fetch(split_first + mine);
     const SeqRows s = seq_rows(a.r, b);
     const int R = s.count * G, row0 = static_cast<int>(blockIdx.y) * kRows;
     if (row0 >= R) return;  // whole workgroup
     const int before = s.n - s.count;  // slots ahead of the new rows
     const int at_min = before + row0 / G, at_max = before + (min(row0 + kRows, R) - 1) / G;
-    const int split_end = min(first_slot + a.turns * kTurn, s.n);
+    const int split_end = min(split_first + a.turns * kTurn, s.n);
     const bool whole = s.n <= a.turns * kTurn;  // the sequence's only split
-    if (whole ? split > 0 : !sees(a, at_max, first_slot, split_end) && !sees(a, at_min, first_slot, split_end)) return;
-    const int end = min(split_end, at_max + 1);  // the slots taken are first_slot .. end - 1, of those that are seen
+    if (whole ? split > 0 : !sees(a, at_max, split_first, split_end) && !sees(a, at_min, split_first, split_end)) return;
+    // the slots taken are first_slot .. end - 1, of those that are seen; turns behind every row's window are left out
+    const int end = seen_end(a, at_min, at_max, split_end), first_slot = seen_begin(a, at_min, split_first, kTurn);
+    if (first_slot != split_first) fetch(first_slot + mine);
 
     // The rows' queries are on their way while the cache is looked at: 16 dims a lane,
     // LPR lanes a row.
@@ -553,9 +564,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
     const int at_min = before + group0 / G, at_max = before + (min(group0 + 64 * RT, R) - 1) / G;
     const bool whole = s.n <= slots;  // the sequence's only split
     if (whole ? split > 0 : !sees(a, at_max, split_first, split_end) && !sees(a, at_min, split_first, split_end)) return;
-    const int end = min(split_end, at_max + 1);
-    // what lies behind every row's window is not walked through, but where the first slots are seen
-    const int first = split_first < a.sinks ? split_first : max(split_first, (at_min + 1 - a.window) & ~(kStage - 1));
+    const int end = seen_end(a, at_min, at_max, split_end), first = seen_begin(a, at_min, split_first, kStage);
     const int stages = end > first ? (end - first + kStage - 1) / kStage : 0;
     const int row0 = group0 + 16 * RT * wave;  // the wavefront's
     const int mine_min = before + min(row0, R - 1) / G, mine_max = before + (min(row0 + 16 * RT, R) - 1) / G;
