@@ -541,7 +541,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 // of a SIMD they hardly overlap: a form that interleaves one half's products with the
 // other's weights took 67 registers too many and 669 us, one that reads operands ahead
 // 593, a raised priority around the products changed nothing.  64 dims and bf16 rows
-// are held to three wavefronts a SIMD (two such pieces of 32 heads over 2: 778 -> 664 us).
+// are held to three wavefronts a SIMD (two such pieces of 32 heads over 4: 778 -> 664 us).
 template <typename IO, int DP, int RT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8Args a) {
     constexpr int NC = DP / 32;                // steps of the first product over the dims
