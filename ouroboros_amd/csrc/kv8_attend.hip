@@ -535,8 +535,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 // of three digits cost a third more matrix instructions and four conversions a
 // score.
 //
-// Bound by issue: of 512 us for two pieces of 1024 bf16 rows over up to 16384 slots
-// (250 GFLOP, 0.49 PFLOP/s) the matrix instructions are 149 and the others 215 (138
+// Bound by issue: of 520 us for two pieces of 1024 bf16 rows over up to 16384 slots
+// (250 GFLOP, 0.48 PFLOP/s) the matrix instructions are 149 and the others 215 (138
 // for each 16 rows and 32 slots, 45 of them the staging), and on the two wavefronts
 // of a SIMD they hardly overlap: a form that interleaves one half's products with the
 // other's weights took 67 registers too many and 669 us, one that reads operands ahead
