@@ -168,11 +168,11 @@ __device__ __forceinline__ void segment(const VerifyArgs &a, int which, int64_t 
             for (int e = 0; e < VL; ++e) sum += x.raw(v[k], e) == m ? 1.0 : 0.0;
         sum = wave_sum(sum);
     } else if (m > -INFINITY) {
-        const double c = kLog2e / static_cast<double>(t), mc = -static_cast<double>(m) * c;
+        const double c = kLog2e / static_cast<double>(t), md = static_cast<double>(m);
 #pragma unroll
         for (int k = 0; k < kVec; ++k)
 #pragma unroll
-            for (int e = 0; e < VL; ++e) sum += exp2_64(fma(static_cast<double>(x.raw(v[k], e)), c, mc));
+            for (int e = 0; e < VL; ++e) sum += exp2_64((static_cast<double>(x.raw(v[k], e)) - md) * c);
         sum = wave_sum(sum);
     }
     if (lane == 0) *out = Seg{sum, m, at};
@@ -274,17 +274,19 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs &a, const SeqRows &s,
     return Verdict{};  // no rows: not reached
 }
 
-// A distribution's values, e^((x - m) / T) / z.
+// A distribution's values, e^((x - m) / T) / z.  The difference comes first here as in
+// the sums: x c - m c with either product rounded is off by 2^-53 |m| / T, which is
+// anything where the largest of many logits is a mask's 1e30 or T is 1e-18.
 struct Share {
-    double c, mc, z;  // log2 e / T, -m c, 1 / z
+    double c, m, z;  // log2 e / T, the maximum, 1 / z
     float top;        // +inf where m is: the mass is that of the +inf logits, else NaN
     __device__ __forceinline__ Share() {}
-    __device__ __forceinline__ Share(const Sums &s, double scale) : c(scale), mc(-static_cast<double>(s.m) * scale), z(1.0 / s.z), top(s.m == INFINITY ? INFINITY : NAN) {}
+    __device__ __forceinline__ Share(const Sums &s, double scale) : c(scale), m(static_cast<double>(s.m)), z(1.0 / s.z), top(s.m == INFINITY ? INFINITY : NAN) {}
     // Of a logit as it lies there: 0 for NaN and -inf.
     __device__ __forceinline__ double of(float x) const {
 #pragma clang fp contract(off)
         if (top == INFINITY) return x == top ? z : 0.0;
-        return exp2_64(__builtin_fma(static_cast<double>(x), c, mc)) * z;
+        return exp2_64((static_cast<double>(x) - m) * c) * z;
     }
 };
 
