@@ -656,7 +656,9 @@ typedef struct ouro_kv8_cache {
  * max_new rows each, rows = seqs * max_new) and lens [seqs] are on the device;
  * `rows` is the packed arrays' length (up to 2^23) and max_new bounds T.  What is out of
  * range is not followed: cu is read as 0 .. rows, T as 0 .. max_new, lens as 0
- * .. the slots of max_pages pages; a row before slot 0 has no slot.
+ * .. the slots of max_pages pages; a row before slot 0 has no slot.  cu ascends:
+ * what is written for a row that two sequences have may be either's or, of
+ * ouro_verify_drafts, a next of -1.
  *
  * New keys and values into the cache, `dtype` rows [n_head_kv][head_dim],
  * new_stride elements apart (0: no gap).  For each block and kv head that gets

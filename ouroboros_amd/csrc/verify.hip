@@ -459,6 +459,7 @@ __global__ __launch_bounds__(kThreads) void verify_next_kernel(VerifyArgs a) {
             if (part[i] > 0.0) from = i, start = cum, passed = cum + part[i] > want;
             cum += part[i];
         }
+        if (from < 0 && tid == 0) a.next[b] = -1;  // as below
 #pragma unroll
         for (int k = 0; k < kVec; ++k)
             if (from == wave * kVec + k) {
@@ -479,6 +480,9 @@ __global__ __launch_bounds__(kThreads) void verify_next_kernel(VerifyArgs a) {
             }
         return;
     }
+    // Not reached where sequences have rows of their own: p has its maximum's mass.  Rows
+    // that two share hold the sums of one, which may have been greedy and made none.
+    if (tid == 0) a.next[b] = -1;
 }
 
 template <typename T, typename D>
