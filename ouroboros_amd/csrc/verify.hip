@@ -76,12 +76,15 @@ __device__ __forceinline__ double exp2_64(double y) {
     s = fma(s, f, 1.0);
     return __builtin_amdgcn_ldexp(s, static_cast<int>(k));
 }
-// e^((x - m) / T), c = log2 e / T, x <= m: 1 where x = m, infinite or not, and 0
-// below 2^-1000, so that a product of what is not 0 never is.
+// 2^y, 0 at 2^-1000 and below, so that a product of what is not 0 never is: the upper
+// half of y becomes that of -2000.  (A sum against its largest term does not see what
+// this leaves out, and does without: 2 us of verify_segments_kernel's 65.)
+__device__ __forceinline__ double exp2_held(double y) {
+    return exp2_64(__hiloint2double(y > -1000.0 ? __double2hiint(y) : static_cast<int>(0xc09f4000u), __double2loint(y)));
+}
+// e^((x - m) / T), c = log2 e / T, x <= m: 1 where x = m, infinite or not.
 __device__ __forceinline__ double weight(float x, float m, double c) {
-    if (x == m) return 1.0;
-    const double y = (static_cast<double>(x) - static_cast<double>(m)) * c;
-    return y > -1000.0 ? exp2_64(y) : 0.0;
+    return x == m ? 1.0 : exp2_held((static_cast<double>(x) - static_cast<double>(m)) * c);
 }
 // Lane `lane`'s value, the same lane for all.
 __device__ __forceinline__ double lane64(double v, int lane) {
@@ -286,7 +289,7 @@ struct Share {
     __device__ __forceinline__ double of(float x) const {
 #pragma clang fp contract(off)
         if (top == INFINITY) return x == top ? z : 0.0;
-        return exp2_64((static_cast<double>(x) - m) * c) * z;
+        return exp2_held((static_cast<double>(x) - m) * c) * z;
     }
 };
 
