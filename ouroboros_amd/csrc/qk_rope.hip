@@ -200,7 +200,8 @@ int launch(const RopeArgs &a, hipStream_t s) {
     RopeArgs b = a;
     unsigned parts = 1;
     if (a.rows >= kManyRows) {
-        while (b.token_shift < 3 && (kThreads / G) >> b.token_shift > 4) ++b.token_shift;
+        // four groups a token, and less than 2^32 threads: 2^24 rows take two tokens at least
+        while (b.token_shift < 3 && ((kThreads / G) >> b.token_shift > 4 || a.rows >> b.token_shift >= 1 << 24)) ++b.token_shift;
     } else {
         parts = static_cast<unsigned>((a.heads + kThreads / G - 1) / (kThreads / G));
     }
