@@ -691,9 +691,11 @@ int ouro_kv8_read(const ouro_kv8_cache *cache, const int32_t *lens,
  *   j <= r with r - j < window or j < sinks (window 0: every j <= r),
  * whose page is there and whose mask byte is not 0,
  *   s_j = scale q.k_j, out = softmax(s) v [* sigmoid(gate)], lse = ln sum e^s,
- * with kv head h / (n_head / n_head_kv).  Where no slot is visible, out = 0 and
- * lse = -inf; where a query holds an infinity or NaN, out and lse are NaN, and so
- * where a visible scale is negative or not finite (of V: out alone).  What lies
+ * with kv head h / (n_head / n_head_kv).  Where no slot is visible, or every
+ * visible one scores -inf, out = 0 and lse = -inf; where a query holds an infinity
+ * or NaN, out and lse are NaN, and so where a visible scale is negative or not
+ * finite (of V: out alone) and where a visible score passes fp32 (|scale| max |q|
+ * times K's scale past 2^127 is taken for that too, whatever the codes).  What lies
  * in slots that are not visible changes nothing.  The same call gives the same
  * bits, and a sequence's rows do not depend on the others in the call (max_new
  * and max_len being the same).

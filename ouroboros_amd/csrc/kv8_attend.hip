@@ -4,7 +4,8 @@
 // For query head h of the row in slot r, over its visible slots j:
 //   s_j = scale q.k_j,  m = max s_j,  l = sum e^(s_j - m),
 //   o = (1 / l) sum e^(s_j - m) v_j  [* sigmoid(gate)],  lse = m + ln l,
-// and o = 0, lse = -inf where no slot is visible.
+// and o = 0, lse = -inf where no slot is visible.  Scores are fp32: one of +inf makes o
+// and lse NaN, one of -inf weighs nothing.
 #include "kv_cache.hpp"
 
 #include <atomic>
@@ -372,7 +373,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 #pragma unroll
                         for (int i = 0; i < 4; ++i) sum[u][i] = __builtin_fmaf(static_cast<float>(hi[i]), 256.f, static_cast<float>(lo[i]));
                     }
-                    const float kq[2] = {qs[t] * ks[0], qs[t] * ks[1]};
+                    // The scores, rounded as the maxima are: fused with the subtraction the largest
+                    // one's distance is what the rounding left, whose e^ passes an fp16 from 2^24 on.
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float kq = qs[t] * ks[u];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+#pragma clang fp contract(off)
+                            sum[u][i] *= kq;
+                        }
+                    }
                     uint32_t vis = 0;  // bit 4 u + i: slot 16 u + i after the lane's first, j + 4 g, is seen
                     float top_s = -INFINITY;
                     if constexpr (Masked) {
@@ -385,12 +396,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                                 const int slot = 16 * u + i;
                                 const uint32_t in = static_cast<uint32_t>(slot <= last) & (static_cast<uint32_t>(slot > low) | static_cast<uint32_t>(slot < sinks));
                                 vis |= (in & (now >> (slot + 4 * g))) << (4 * u + i);
-                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? kq[u] * sum[u][i] : -INFINITY);
+                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? sum[u][i] : -INFINITY);
                             }
                     } else {
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
-                            top_s = fmaxf(top_s, kq[u] * fmaxf(fmaxf(sum[u][0], sum[u][1]), fmaxf(sum[u][2], sum[u][3])));
+                            top_s = fmaxf(top_s, fmaxf(fmaxf(sum[u][0], sum[u][1]), fmaxf(sum[u][2], sum[u][3])));
                     }
                     // the reference moves only where some row of the tile has a larger score
                     if (__any(top_s > m[t]) || grown != 1.f) {
@@ -407,7 +418,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                         float p[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sum[u][i], kq[u], -ref));
+                            p[i] = __builtin_amdgcn_exp2f(sum[u][i] - ref);
                             if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;
                             l[t] += p[i];
                             p[i] *= f[u];
@@ -764,7 +775,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                     }
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
-                    const float kq[2] = {qs[t] * ks[0], qs[t] * ks[1]};
+                    // The scores, rounded as the maxima are: fused with the subtraction the largest
+                    // one's distance is what the rounding left, whose e^ passes an fp16 from 2^24 on.
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float kq = qs[t] * ks[u];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+#pragma clang fp contract(off)
+                            sum[t][u][i] *= kq;
+                        }
+                    }
                     uint32_t vis = 0;
                     float top_s = -INFINITY;
                     if constexpr (Masked) {
@@ -776,12 +797,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                                 const int slot = 16 * u + i;
                                 const uint32_t in = static_cast<uint32_t>(slot <= last) & (static_cast<uint32_t>(slot > low) | static_cast<uint32_t>(slot < sinks));
                                 vis |= (in & (now >> (slot + 4 * g))) << (4 * u + i);
-                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? kq[u] * sum[t][u][i] : -INFINITY);
+                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? sum[t][u][i] : -INFINITY);
                             }
                     } else {
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
-                            top_s = fmaxf(top_s, kq[u] * fmaxf(fmaxf(sum[t][u][0], sum[t][u][1]), fmaxf(sum[t][u][2], sum[t][u][3])));
+                            top_s = fmaxf(top_s, fmaxf(fmaxf(sum[t][u][0], sum[t][u][1]), fmaxf(sum[t][u][2], sum[t][u][3])));
                     }
                     if (__any(top_s > m[t]) || grown != 1.f) {
                         const float mn = fmaxf(m[t], quad_max(top_s));
@@ -797,7 +818,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                         float p[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sum[t][u][i], kq[u], -ref));
+                            p[i] = __builtin_amdgcn_exp2f(sum[t][u][i] - ref);
                             if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;
                             l[t] += p[i];
                             p[i] *= f[u];
