@@ -696,7 +696,9 @@ int ouro_kv8_read(const ouro_kv8_cache *cache, const int32_t *lens,
  * or NaN, out and lse are NaN, and so where a visible scale is negative or not
  * finite (of V: out alone) and where a visible score passes fp32 (|scale| max |q|
  * times K's scale past 2^127 is taken for that too, whatever the codes).  What lies
- * in slots that are not visible changes nothing.  The same call gives the same
+ * in slots that are not visible changes nothing.  A slot's weight times its scale
+ * of V is held to 2^-22 of itself or 2^-31 of the row's largest such product,
+ * whichever is more, sums and scores to fp32.  The same call gives the same
  * bits, and a sequence's rows do not depend on the others in the call (max_new
  * and max_len being the same).
  *   q, out (rows q_stride, out_stride apart), gate, mask, lse as of

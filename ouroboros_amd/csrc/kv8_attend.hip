@@ -109,6 +109,121 @@ __device__ __forceinline__ int in_loop(int x) {
     return x;
 }
 
+// A row's weights against V, e^(s - m) times the scale of the slot's block, are held in
+// fp16 against a bound of the largest so far, z its log2: it is no more than the largest
+// scale of what the row itself sees, and at most kHead above the largest such weight, so
+// that neither a block that another row sees nor one of a large scale and little weight
+// takes their bits.  They are taken times 2^unit, to kFull at most.
+constexpr float kNoWeight = -112.f, kHead = 8.f, kFull = 32768.f;
+constexpr float kLow = 130.f;  // kFull / 2^kHead, and a little
+__device__ __forceinline__ int unit_of(float z) { return 15 - static_cast<int>(ceilf(z)); }
+__device__ __forceinline__ int unit_of_scale(float unit_scale) { return __builtin_amdgcn_frexp_expf(unit_scale) - 1; }
+// A scale times 2^unit where that is past fp32, which it can be only of slots whose
+// weights are below kFull / 2^127: what those are short of then is less than they are,
+// and a weight of 0 stays one.
+__device__ __forceinline__ float no_infinity(float f) { return f > 3.4028234663852886e38f ? 3.4028234663852886e38f : f; }
+
+// A tile of 32 slots of the row that a lane has: slots 4 g + i and 16 + 4 g + i of it are
+// s[0][i] and s[1][i].  Those that the row does not see score -inf from here on: of the
+// tile's slots `now`, it sees them up to `last`, but for what lies between `sinks` and the
+// window (all of them counted from the lane's first, j + 4 g).
+__device__ __forceinline__ void hide_unseen(f32x4_t (&s)[2], uint32_t now, int last, int window, int sinks) {
+    // the lowest n of 32 bits
+    auto below = [](int n) { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; };
+    const uint32_t seen = now & below(last + 1) & (~below(last - window + 1) | below(sinks));
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(seen), 16 * u + i, 1));  // all ones or none
+            s[u][i] = __uint_as_float((keep & __float_as_uint(s[u][i])) | (~keep & 0xff800000u));
+        }
+}
+
+// What a wavefront keeps of its N tiles of 16 rows, a lane of row r of each.
+template <int N, int CH>
+struct Rows {
+    f32x4_t o[N][CH];             // o[t][e][i]: dim CH (4 g + i) + e, times unit, of codes times 2^-9
+    float m[N], l[N];             // the row's maximum and sum so far
+    float z[N], unit[N];          // the bound of its weights, log2, and 2^unit_of(z)
+    float held_to[N];             // and what the largest is at least, log2
+    __device__ __forceinline__ Rows() {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            m[t] = held_to[t] = -INFINITY, l[t] = 0.f, z[t] = kNoWeight, unit[t] = ldexpf(1.0f, unit_of(kNoWeight));
+#pragma unroll
+            for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // Takes in the scores s of a tile of 32 slots, whose scales of V are vs: f is what its
+    // weights are taken by.  The references move only where some row has a larger score or
+    // weight, all of a row's four lanes alike.
+    __device__ __forceinline__ void take(const f32x4_t (&s)[N][2], const float (&vs)[2], float (&f)[N][2]) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            float top[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                top[u] = fmaxf(fmaxf(s[t][u][0], s[t][u][1]), fmaxf(s[t][u][2], s[t][u][3]));
+                f[t][u] = vs[u] * unit[t];
+            }
+            const bool wider = !(__builtin_elementwise_maximum(f[t][0], f[t][1]) <= kFull);  // or NaN
+            if (__any(wider || fmaxf(top[0], top[1]) > m[t])) move(t, top, vs, wider, f[t]);
+        }
+    }
+    // A tile's weights of rows t as two operands, h + w.
+    __device__ __forceinline__ void weigh(int t, const f32x4_t (&s)[2], const float (&f)[2], u32x4_t &h, u32x4_t &w) {
+        const float ref = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(s[u][i] - ref);
+                l[t] += p[i];
+                p[i] *= f[u];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f16x2_t a = __builtin_convertvector(f32x2_t{p[2 * i], p[2 * i + 1]}, f16x2_t);
+                // what a leaves, by an fma that takes it as it is: one instruction, not two
+                const f16x2_t b = __builtin_convertvector(
+                    f32x2_t{__builtin_fmaf(static_cast<float>(a[0]), -1.f, p[2 * i]), __builtin_fmaf(static_cast<float>(a[1]), -1.f, p[2 * i + 1])}, f16x2_t);
+                h[2 * u + i] = __builtin_bit_cast(uint32_t, a);
+                w[2 * u + i] = __builtin_bit_cast(uint32_t, b);
+            }
+        }
+    }
+    // Moves the references of rows t, whose largest scores in the tile are top.  A row's
+    // bound rises to a larger scale that it sees, which takes one times unit above kFull,
+    // and falls where a new maximum has left it more than kHead above that slot's weight,
+    // which takes one below kLow.  It goes by what the row itself sees, whatever the rows
+    // beside it do.
+    __device__ __forceinline__ void move(int t, const float (&top)[2], const float (&vs)[2], bool wider, float (&f)[2]) {
+        const float mn = fmaxf(m[t], quad_max(fmaxf(top[0], top[1]))), to = mn == -INFINITY ? 0.f : mn;  // no inf - inf
+        const float back = __builtin_amdgcn_exp2f(m[t] - to);
+        float by = back;
+        held_to[t] += m[t] - to;
+        if (__any(wider || (fminf(f[0], f[1]) < kLow && mn > m[t]))) {  // seldom
+            const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
+            const float most = quad_max(fmaxf(top[0] - to + lv[0], top[1] - to + lv[1]));
+            const float scale = quad_max(fmaxf(top[0] > -INFINITY ? lv[0] : -INFINITY, top[1] > -INFINITY ? lv[1] : -INFINITY));
+            if (scale > ceilf(z[t]) + 0.01f || (mn > m[t] && z[t] > most + kHead)) {
+                held_to[t] = fmaxf(held_to[t], most);
+                z[t] = fmaxf(fmaxf(fmaxf(z[t] + (m[t] - to), most), fminf(fmaxf(z[t], scale), held_to[t] + kHead)), kNoWeight);
+            }
+            by = ldexpf(back, unit_of(z[t]) - unit_of_scale(unit[t]));
+            unit[t] = ldexpf(1.0f, unit_of(z[t]));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) f[u] = top[u] > -INFINITY ? no_infinity(vs[u] * unit[t]) : 0.f;  // whatever the scale of what is not seen
+        }
+        m[t] = mn;
+        l[t] *= back;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) o[t][e] *= by;
+    }
+};
+
 // A head's joined output (normalised), through the gate to its place.
 template <typename IO>
 __device__ __forceinline__ void store_out(const Attend8Args &a, int64_t row, int h, int dim, float o) {
@@ -152,9 +267,10 @@ constexpr int joined_rows(int dp) { return dp <= 128 ? 16 : 8; }
 // are loaded, so the weights become the second operand without leaving their
 // registers.  V's codes become fp16 by a byte permute, which puts the offset code
 // of two slots into the low bytes of two fp16 as multiples of 2^-24, and one fused
-// multiply-add, which takes the offset off: exact.  A weight, times its slot's
-// scale of V against the largest so far, is held in two fp16 (2^-22 of it, or 2^-40
-// of the largest); sums, maxima and outputs are fp32.
+// multiply-add, which takes the offset off: exact.  A weight times its slot's scale of
+// V is held in two fp16 (2^-22 of it, or 2^-31 of the row's largest: 2^-25 at a power of
+// two that takes 2^kHead times the largest to 2^14 .. 2^15); sums, maxima and outputs are
+// fp32.
 //
 // Bound by memory where the splits fill the chip (128 sequences of 8192 slots, 4 kv
 // heads of 128: 228 us, 4.7 TB/s), below that by what a workgroup does before its
@@ -173,7 +289,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
     constexpr int kRows = 16 * NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // digits [3][NT][NJ][64 lanes] of 16 bytes; later the outputs
     __shared__ float row_scale[kRows];
-    __shared__ float sm[4][kRows], sl[4][kRows], sf[4];
+    __shared__ float sm[4][kRows], sl[4][kRows];
+    __shared__ int su[4][kRows];                  // what brings a wavefront's outputs to the codes' size
     __shared__ int2 place[kRows];                 // packed row and head of each
     typedef uint32_t vch_t __attribute__((ext_vector_type(VW)));
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -313,18 +430,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
     }
     __syncthreads();
 
-    f32x4_t o[NT][CH];  // o[t][e][i]: dim CH (4 g + i) + e of row r of tile t
-    float m[NT], l[NT], qs[NT];
+    Rows<NT, CH> rows;
+    float qs[NT];
     int at[NT];  // the row's own slot; -1 past the last row
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int rho = row0 + 16 * t + r;
         at[t] = rho < R ? before + place[16 * t + r].x - s.first : -1;
-        m[t] = -INFINITY, l[t] = 0.f, qs[t] = row_scale[16 * t + r];
-#pragma unroll
-        for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        qs[t] = row_scale[16 * t + r];
     }
-    float v_top = 0.f, v_inv = 1.f;  // the largest scale of V so far and its reciprocal; outputs are in units of it (times 2^6)
     const int turns = (end - first_slot + kTurn - 1) / kTurn;
     for (int turn = 0; turn < turns; ++turn) {
         const int t0 = first_slot + turn * kTurn;
@@ -337,22 +451,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
             const float ks[2] = {lane_float(k_sc, 32 * k), lane_float(k_sc, 32 * k + 16)};
             const float vs[2] = {lane_float(v_sc, 32 * k), lane_float(v_sc, 32 * k + 16)};
             const bool all = now == 0xffffffffu && j + 31 <= at_min && (j > at_max - a.window || j + 31 < a.sinks);
-            u32x4_t ph[NT], pl[NT];  // the weights' two operands
-            // A tile's scores, running maxima and weights.  Masked: some row does not
-            // see some slot.
-            auto weigh = [&](auto masked) {
-                constexpr bool Masked = decltype(masked)::value;
-                const float top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
-                float grown = 1.f;
-                if (top != v_top) {
-                    grown = v_top / top;
-                    v_top = top;
-                    v_inv = 1.0f / top;
-                }
-                const float f[2] = {vs[0] * v_inv * 32768.f, vs[1] * v_inv * 32768.f};
+            // The tile's scores, rounded as the maxima are: fused with the subtraction the largest
+            // one's distance is what the rounding left, whose e^ passes an fp16 from 2^24 on.
+            f32x4_t sum[NT][2];
+            if (now) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    float sum[2][4];
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         i32x4_t hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
@@ -370,75 +474,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                         for (int i = 0; i < NJ; ++i)
                             hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, kf[u][i]),
                                                                        __builtin_bit_cast(i32x4_t, dg[NT * NJ * 64 + i * 64]), hi, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[u][i] = __builtin_fmaf(static_cast<float>(hi[i]), 256.f, static_cast<float>(lo[i]));
-                    }
-                    // The scores, rounded as the maxima are: fused with the subtraction the largest
-                    // one's distance is what the rounding left, whose e^ passes an fp16 from 2^24 on.
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
                         const float kq = qs[t] * ks[u];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
 #pragma clang fp contract(off)
-                            sum[u][i] *= kq;
+                            sum[t][u][i] = __builtin_fmaf(static_cast<float>(hi[i]), 256.f, static_cast<float>(lo[i])) * kq;
                         }
                     }
-                    uint32_t vis = 0;  // bit 4 u + i: slot 16 u + i after the lane's first, j + 4 g, is seen
-                    float top_s = -INFINITY;
-                    if constexpr (Masked) {
-                        // it is up to `last`, but for what lies between `sinks` and the window
-                        const int last = at[t] - j - 4 * g, low = last - a.window, sinks = a.sinks - j - 4 * g;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int slot = 16 * u + i;
-                                const uint32_t in = static_cast<uint32_t>(slot <= last) & (static_cast<uint32_t>(slot > low) | static_cast<uint32_t>(slot < sinks));
-                                vis |= (in & (now >> (slot + 4 * g))) << (4 * u + i);
-                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? sum[u][i] : -INFINITY);
-                            }
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            top_s = fmaxf(top_s, fmaxf(fmaxf(sum[u][0], sum[u][1]), fmaxf(sum[u][2], sum[u][3])));
-                    }
-                    // the reference moves only where some row of the tile has a larger score
-                    if (__any(top_s > m[t]) || grown != 1.f) {
-                        const float mn = fmaxf(m[t], quad_max(top_s));
-                        const float back = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));  // no inf - inf
-                        m[t] = mn;
-                        l[t] *= back;
-#pragma unroll
-                        for (int e = 0; e < CH; ++e) o[t][e] *= back * grown;
-                    }
-                    const float ref = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float p[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[i] = __builtin_amdgcn_exp2f(sum[u][i] - ref);
-                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;
-                            l[t] += p[i];
-                            p[i] *= f[u];
-                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;  // whatever the scale of a slot that is not seen
-                        }
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const f16x2_t h = __builtin_convertvector(f32x2_t{p[2 * i], p[2 * i + 1]}, f16x2_t);
-                            const f16x2_t w = __builtin_convertvector(
-                                f32x2_t{p[2 * i] - static_cast<float>(h[0]), p[2 * i + 1] - static_cast<float>(h[1])}, f16x2_t);
-                            ph[t][2 * u + i] = __builtin_bit_cast(uint32_t, h);
-                            pl[t][2 * u + i] = __builtin_bit_cast(uint32_t, w);
-                        }
-                    }
-                }
-            };
-            if (all)
-                weigh(std::false_type{});
-            else if (now)
-                weigh(std::true_type{});
+            }
             // K's registers are free: the next tile's rows
             if (k == 0) {
                 load_k(j + 128, 1, tile_bits(1) != 0);
@@ -447,6 +490,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                 load_k(j + 128, 0, tile_bits(0) != 0);
             }
             if (now) {
+                u32x4_t ph[NT], pl[NT];  // the weights' two operands
+                if (!all)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) hide_unseen(sum[t], now >> (4 * g), in_loop(at[t] - j - 4 * g), a.window, a.sinks - j - 4 * g);  // a branch of its own
+                float f[NT][2];
+                rows.take(sum, vs, f);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) rows.weigh(t, sum[t], f[t], ph[t], pl[t]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -463,8 +514,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                         }
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, ph[t]), o[t][e], 0, 0, 0);
-                        o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, pl[t]), o[t][e], 0, 0, 0);
+                        rows.o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, ph[t]), rows.o[t][e], 0, 0, 0);
+                        rows.o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, pl[t]), rows.o[t][e], 0, 0, 0);
                     }
                 }
             }
@@ -477,10 +528,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
     const int64_t shift = record_shift(a, b, s);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const float sum = quad_sum(l[t]);
-        if (g == 0) sm[wave][16 * t + r] = m[t], sl[wave][16 * t + r] = sum;
+        const float sum = quad_sum(rows.l[t]);
+        if (g == 0) sm[wave][16 * t + r] = rows.m[t], sl[wave][16 * t + r] = sum, su[wave][16 * t + r] = 9 - unit_of_scale(rows.unit[t]);
     }
-    if (lane == 0) sf[wave] = v_top * 0.015625f;
     __syncthreads();  // and the digits have been read
     if (tid < kRows && row0 + tid < R) {
         const float M = fmaxf(fmaxf(sm[0][tid], sm[1][tid]), fmaxf(sm[2][tid], sm[3][tid])), ref = M == -INFINITY ? 0.f : M;
@@ -494,7 +544,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         const int h = place[tid].y;
         const float norm = !whole ? 1.f : L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) sm[w][tid] = f[w] * sf[w] * norm;
+        for (int w = 0; w < 4; ++w) sm[w][tid] = f[w] * norm;
         if (whole)
             store_lse(a, row, h, M, L);
         else
@@ -511,7 +561,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
             if (r / kJoin == k) {
                 float *row = ob + (wave * kJoin + r % kJoin) * OS + 4 * g;
 #pragma unroll
-                for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * e) = o[t][e];
+                for (int e = 0; e < CH; ++e) *reinterpret_cast<f32x4_t *>(row + 16 * e) = rows.o[t][e];
             }
             __syncthreads();
             for (int i = tid; i < kJoin * DP / 4; i += 256) {
@@ -523,7 +573,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                     const float f = sm[w][q];
                     const float *from = ob + (w * kJoin + q - q0) * OS;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] += f * from[(dim + e) % CH * 16 + (dim + e) / CH];
+                    for (int e = 0; e < 4; ++e) x[e] += ldexpf(f * from[(dim + e) % CH * 16 + (dim + e) / CH], su[w][q]);
                 }
                 const int64_t row = place[q].x;
                 const int h = place[q].y;
@@ -716,15 +766,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                             uint32_t, __builtin_convertvector(f32x2_t{x0 - static_cast<float>(hi[0]), x1 - static_cast<float>(hi[1])}, f16x2_t));
                 }
     }
-    f32x4_t o[RT][CH];  // o[t][e][i]: dim CH (4 g + i) + e of row r of tile t
-    float m[RT], l[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        m[t] = -INFINITY, l[t] = 0.f;
-#pragma unroll
-        for (int e = 0; e < CH; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    float v_top = 0.f, v_inv = 1.f;
+    Rows<RT, CH> rows;
     look(0);
     load(0);
     fetch(1);
@@ -746,17 +788,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
             const bool all = now == 0xffffffffu && j + 31 <= mine_min && (j > mine_max - a.window || j + 31 < a.sinks);
             const float ks[2] = {lane_float(k_sc, 32 * half), lane_float(k_sc, 32 * half + 16)};
             const float vs[2] = {lane_float(v_sc, 32 * half), lane_float(v_sc, 32 * half + 16)};
-            u32x4_t ph[RT], pl[RT];
-            auto weigh = [&](auto masked) {
-                constexpr bool Masked = decltype(masked)::value;
-                const float top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
-                float grown = 1.f;
-                if (top != v_top) {
-                    grown = v_top / top;
-                    v_top = top;
-                    v_inv = 1.0f / top;
-                }
-                const float f[2] = {vs[0] * v_inv * 32768.f, vs[1] * v_inv * 32768.f};
+            if (now) {
                 f32x4_t sum[RT][2];
 #pragma unroll
                 for (int t = 0; t < RT; ++t) sum[t][0] = sum[t][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -774,9 +806,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                                 sum[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k[u]), __builtin_bit_cast(f16x8_t, qf[t][n][c]), sum[t][u], 0, 0, 0);
                     }
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    // The scores, rounded as the maxima are: fused with the subtraction the largest
-                    // one's distance is what the rounding left, whose e^ passes an fp16 from 2^24 on.
+                for (int t = 0; t < RT; ++t)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const float kq = qs[t] * ks[u];
@@ -786,73 +816,24 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                             sum[t][u][i] *= kq;
                         }
                     }
-                    uint32_t vis = 0;
-                    float top_s = -INFINITY;
-                    if constexpr (Masked) {
-                        const int last = at[t] - j - 4 * g, low = last - a.window, sinks = a.sinks - j - 4 * g;
+                if (!all)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
+                    for (int t = 0; t < RT; ++t) hide_unseen(sum[t], now >> (4 * g), in_loop(at[t] - j - 4 * g), a.window, a.sinks - j - 4 * g);  // a branch of its own
+                float f[RT][2];
+                rows.take(sum, vs, f);
+                u32x4_t w[CH];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int slot = 16 * u + i;
-                                const uint32_t in = static_cast<uint32_t>(slot <= last) & (static_cast<uint32_t>(slot > low) | static_cast<uint32_t>(slot < sinks));
-                                vis |= (in & (now >> (slot + 4 * g))) << (4 * u + i);
-                                top_s = fmaxf(top_s, vis >> (4 * u + i) & 1 ? sum[t][u][i] : -INFINITY);
-                            }
-                    } else {
+                for (int e = 0; e < CH; ++e) w[e] = from[kK + (half * CH + e) * 64 + lane];
+                // one tile's weights beside the other's products
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            top_s = fmaxf(top_s, fmaxf(fmaxf(sum[t][u][0], sum[t][u][1]), fmaxf(sum[t][u][2], sum[t][u][3])));
-                    }
-                    if (__any(top_s > m[t]) || grown != 1.f) {
-                        const float mn = fmaxf(m[t], quad_max(top_s));
-                        const float back = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));  // no inf - inf
-                        m[t] = mn;
-                        l[t] *= back;
-#pragma unroll
-                        for (int e = 0; e < CH; ++e) o[t][e] *= back * grown;
-                    }
-                    const float ref = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float p[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[i] = __builtin_amdgcn_exp2f(sum[t][u][i] - ref);
-                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;
-                            l[t] += p[i];
-                            p[i] *= f[u];
-                            if constexpr (Masked) p[i] = vis >> (4 * u + i) & 1 ? p[i] : 0.f;  // whatever the scale of a slot that is not seen
-                        }
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const f16x2_t h = __builtin_convertvector(f32x2_t{p[2 * i], p[2 * i + 1]}, f16x2_t);
-                            const f16x2_t w = __builtin_convertvector(
-                                f32x2_t{__builtin_fmaf(static_cast<float>(h[0]), -1.f, p[2 * i]), __builtin_fmaf(static_cast<float>(h[1]), -1.f, p[2 * i + 1])}, f16x2_t);
-                            ph[t][2 * u + i] = __builtin_bit_cast(uint32_t, h);
-                            pl[t][2 * u + i] = __builtin_bit_cast(uint32_t, w);
-                        }
-                    }
-                }
-            };
-            if (all)
-                weigh(std::false_type{});
-            else if (now)
-                weigh(std::true_type{});
-            if (now) {
-                // four dims at a time: no product waits for the one before it
-#pragma unroll
-                for (int e0 = 0; e0 < CH; e0 += 4) {
-                    u32x4_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = from[kK + (half * CH + e0 + e) * 64 + lane];
+                for (int t = 0; t < RT; ++t) {
+                    u32x4_t p[2];
+                    rows.weigh(t, sum[t], f[t], p[0], p[1]);
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int t = 0; t < RT; ++t)
-                                o[t][e0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[e]), __builtin_bit_cast(f16x8_t, n ? pl[t] : ph[t]), o[t][e0 + e], 0, 0, 0);
+                        for (int e = 0; e < CH; ++e)
+                            rows.o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[e]), __builtin_bit_cast(f16x8_t, p[n]), rows.o[t][e], 0, 0, 0);
                 }
             }
         }
@@ -864,18 +845,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
     const int64_t shift = record_shift(a, b, s);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const float L = quad_sum(l[t]);
+        const float L = quad_sum(rows.l[t]);
         const int rho = row0 + 16 * t + r;
         if (rho >= R) continue;
         const int64_t row = s.first + rho / G;
         const int h = kvh * G + rho % G;
-        const float unit = v_top * 0.015625f;  // outputs are in units of V's largest scale, times 2^6
         const int64_t rec = ((row + shift) * a.n_head + h) * a.n_split + split;
         if (g == 0) {
             if (whole)
-                store_lse(a, row, h, m[t], L);
+                store_lse(a, row, h, rows.m[t], L);
             else
-                a.ml[rec] = make_float2(m[t], L);
+                a.ml[rec] = make_float2(rows.m[t], L);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -885,7 +865,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
             for (int e = 0; e < CH; e += 4) {
                 f32x4_t x;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = o[t][e + k][i] * unit;
+                for (int k = 0; k < 4; ++k) x[k] = ldexpf(rows.o[t][e + k][i], 9 - unit_of_scale(rows.unit[t]));
                 if (whole) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) store_out<IO>(a, row, h, dim + e + k, L == 0.f ? 0.f : x[k] / L);
