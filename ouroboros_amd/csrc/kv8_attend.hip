@@ -102,6 +102,26 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
     return __builtin_bit_cast(uint32_t, c);
 }
 
+// N adjacent dwords of a row of codes, at a multiple of 4 bytes for N = 3 (12 dims a
+// lane), of 4 N else.  A vector of three is no type to read them by: it has the size
+// and the alignment of four, so that the last lane of a pool's last row could read 4
+// bytes past its end.
+template <int N>
+struct Dwords {
+    uint32_t w[N];
+};
+template <int N>
+__device__ __forceinline__ auto load_dwords(const int8_t *p) {
+    typedef uint32_t vec_t __attribute__((ext_vector_type(N)));
+    if constexpr (N == 3) {
+        static_assert(sizeof(Dwords<3>) == 12 && alignof(Dwords<3>) == 4, "Dwords: what is read of a row");
+        const Dwords<3> d = *reinterpret_cast<const Dwords<3> *>(p);
+        return vec_t{d.w[0], d.w[1], d.w[2]};
+    } else {
+        static_assert(sizeof(vec_t) == 4 * N, "Dwords: what is read of a row");
+        return *reinterpret_cast<const vec_t *>(p);
+    }
+}
 // x, as a value that is made where this stands: what is read by it stays in the
 // loop.  The asm holds no instruction, so that no wait state is owed around it.
 __device__ __forceinline__ int in_loop(int x) {
@@ -380,7 +400,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
             const uint32_t step = there ? row_bytes : 0u, off = 4 * static_cast<uint32_t>(in_loop(g)) * step;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                vf[u][i] = *reinterpret_cast<const vch_t *>(base + static_cast<uint64_t>(i) * step + (off + static_cast<uint32_t>(min(CH * r, d - CH))));
+                vf[u][i] = load_dwords<VW>(base + static_cast<uint64_t>(i) * step + (off + static_cast<uint32_t>(min(CH * r, d - CH))));
         }
     };
     auto tile_bits = [&](int k) { return static_cast<uint32_t>(bits >> (32 * k)); };
@@ -683,7 +703,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                 const uint32_t off = 4 * static_cast<uint32_t>(g) * step + static_cast<uint32_t>(min(CH * r, d - CH));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const vch_t v = *reinterpret_cast<const vch_t *>(base + static_cast<uint64_t>(i) * step + off);
+                    const vch_t v = load_dwords<VW>(base + static_cast<uint64_t>(i) * step + off);
 #pragma unroll
                     for (int w = 0; w < VW; ++w) raw[(VW * (4 * u + i) + w) / 4][(VW * (4 * u + i) + w) % 4] = v[w];
                 }
