@@ -913,8 +913,9 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
     const int i = static_cast<int>(item / a.n_head), h = static_cast<int>(item % a.n_head);
     const int slots = a.turns * kTurn;
     if (s.n <= slots) return;  // its only split wrote it
+    if (static_cast<int64_t>(blockIdx.x) * PER >= static_cast<int64_t>(s.count) * a.n_head) return;  // whole workgroup
+    // threads past the last whole head (of 192 dims 16 or 64) have no work but the barrier
     const bool live = who < PER && i < s.count;
-    if (PER == 1 && !live) return;  // whole workgroup
     const int at = s.n - s.count + i, d = a.c.d;
     const int64_t row = s.first + i, rec = ((row + record_shift(a, b, s)) * a.n_head + h) * a.n_split;
     f32x4_t x = {0.f, 0.f, 0.f, 0.f};
