@@ -244,11 +244,12 @@ struct Rows {
     }
 };
 
-// A head's joined output (normalised), through the gate to its place.
+// A head's joined output (normalised; its sum l) through the gate to its place: 0 where
+// nothing was visible, whatever the gate is.
 template <typename IO>
-__device__ __forceinline__ void store_out(const Attend8Args &a, int64_t row, int h, int dim, float o) {
+__device__ __forceinline__ void store_out(const Attend8Args &a, int64_t row, int h, int dim, float o, float l) {
     const int64_t i = static_cast<int64_t>(h) * a.c.d + dim;
-    if (a.gate) o *= 1.0f / (1.0f + expf(-load1(static_cast<const IO *>(a.gate), row * a.q_stride + i)));
+    if (a.gate && l != 0.f) o *= 1.0f / (1.0f + expf(-load1(static_cast<const IO *>(a.gate), row * a.q_stride + i)));
     store1(static_cast<IO *>(a.out), row * a.out_stride + i, o);
 }
 __device__ __forceinline__ void store_lse(const Attend8Args &a, int64_t row, int h, float m, float l) {
@@ -565,6 +566,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         const float norm = !whole ? 1.f : L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
         for (int w = 0; w < 4; ++w) sm[w][tid] = f[w] * norm;
+        sl[0][tid] = L;
         if (whole)
             store_lse(a, row, h, M, L);
         else
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
                 const int h = place[q].y;
                 if (whole)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, x[e]);
+                    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, x[e], sl[0][q]);
                 else
                     *reinterpret_cast<f32x4_t *>(a.part + (((row + shift) * a.n_head + h) * a.n_split + split) * d + dim) = x;
             }
@@ -888,7 +890,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
                 for (int k = 0; k < 4; ++k) x[k] = ldexpf(rows.o[t][e + k][i], 9 - unit_of_scale(rows.unit[t]));
                 if (whole) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) store_out<IO>(a, row, h, dim + e + k, L == 0.f ? 0.f : x[k] / L);
+                    for (int k = 0; k < 4; ++k) store_out<IO>(a, row, h, dim + e + k, L == 0.f ? 0.f : x[k] / L, L);
                 } else {
                     *reinterpret_cast<f32x4_t *>(a.part + rec * d + dim + e) = x;
                 }
@@ -960,7 +962,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
     }
     if (!live || dim >= d) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, L == 0.f ? 0.f : x[e] / L);
+    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, L == 0.f ? 0.f : x[e] / L, L);
     if (dim == 0) store_lse(a, row, h, M, L);
 }
 
