@@ -1161,6 +1161,8 @@ int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
     if (!mask_stride) mask_stride = max_len;
     if (q_stride < n_head * d || out_stride < n_head * d || mask_stride < max_len)
         return fail(OURO_ERR_SHAPE, "%s: a stride shorter than its row", me);
+    if (q_stride > (size_t{1} << 40) || out_stride > (size_t{1} << 40) || mask_stride > (size_t{1} << 40))
+        return fail(OURO_ERR_SHAPE, "%s: a stride past 2^40", me);
     const size_t unit = dtype == OURO_DT_F32 ? 4 : 8;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(gate)) & 15 ||
         q_stride % unit || out_stride % unit)
