@@ -31,7 +31,7 @@ struct Attend8Args {
     const uint8_t *mask;
     void *out;
     float *lse;
-    float *part;  // [records][n_head][n_split][d]: the splits' outputs, not normalised
+    float *part;  // [records][n_head][n_split][d]: the splits' outputs, averages by their own sums
     float2 *ml;   // [records][n_head][n_split]: their maxima (of scores times log2 e) and sums
     int64_t q_stride, mask_stride, out_stride;
     int32_t n_head, window, sinks;  // window 2^30: every slot
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
         }
         const int64_t row = place[tid].x;
         const int h = place[tid].y;
-        const float norm = !whole ? 1.f : L == 0.f ? 0.f : 1.0f / L;
+        const float norm = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
         for (int w = 0; w < 4; ++w) sm[w][tid] = f[w] * norm;
         sl[0][tid] = L;
@@ -873,6 +873,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
         const int64_t row = s.first + rho / G;
         const int h = kvh * G + rho % G;
         const int64_t rec = ((row + shift) * a.n_head + h) * a.n_split + split;
+        const float norm = L == 0.f ? 0.f : 1.0f / L;
+        const int to = 9 - unit_of_scale(rows.unit[t]);
         if (g == 0) {
             if (whole)
                 store_lse(a, row, h, rows.m[t], L);
@@ -887,10 +889,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
             for (int e = 0; e < CH; e += 4) {
                 f32x4_t x;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = ldexpf(rows.o[t][e + k][i], 9 - unit_of_scale(rows.unit[t]));
+                for (int k = 0; k < 4; ++k) x[k] = ldexpf(rows.o[t][e + k][i] * norm, to);
                 if (whole) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) store_out<IO>(a, row, h, dim + e + k, L == 0.f ? 0.f : x[k] / L, L);
+                    for (int k = 0; k < 4; ++k) store_out<IO>(a, row, h, dim + e + k, x[k], L);
                 } else {
                     *reinterpret_cast<f32x4_t *>(a.part + rec * d + dim + e) = x;
                 }
@@ -899,9 +901,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8
     }
 }
 
+__device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l); }
 // The splits of a row and head joined by NG groups of DP / 4 lanes, each with
 // every NG-th split and four dims a lane, kAhead splits on their way at a time;
-// 256 / (NG DP / 4) heads a workgroup.
+// 256 / (NG DP / 4) heads a workgroup.  What is joined stays an average at every step (its
+// rounding 3 U, of at most 64 + NG steps), so that values up to fp32's last do not pass it.
 constexpr int kAhead = 4;
 template <typename IO, int DP, int NG>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
@@ -939,10 +943,10 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const float mn = fmaxf(M, ml[k].x), ref = mn == -INFINITY ? 0.f : mn;
-                const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml[k].x - ref);
-                L = L * f + ml[k].y * w;
-                x = x * f + w * part[k];
-                M = mn;
+                const float f = L * __builtin_amdgcn_exp2f(M - ref), w = ml[k].y * __builtin_amdgcn_exp2f(ml[k].x - ref);
+                L = f + w, M = mn;
+                const float inv = reciprocal(L);
+                x = f * inv * x + w * inv * part[k];
             }
         }
     if constexpr (NG > 1) {
@@ -954,15 +958,15 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
         for (int k = 1; k < NG; ++k) {
             const float2 ml = rml[tid + k * DL];
             const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-            const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml.x - ref);
-            L = L * f + ml.y * w;
-            x = x * f + w * red[tid + k * DL];
-            M = mn;
+            const float f = L * __builtin_amdgcn_exp2f(M - ref), w = ml.y * __builtin_amdgcn_exp2f(ml.x - ref);
+            L = f + w, M = mn;
+            const float inv = reciprocal(L);
+            x = f * inv * x + w * inv * red[tid + k * DL];
         }
     }
     if (!live || dim >= d) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, L == 0.f ? 0.f : x[e] / L, L);
+    for (int e = 0; e < 4; ++e) store_out<IO>(a, row, h, dim + e, x[e], L);
     if (dim == 0) store_lse(a, row, h, M, L);
 }
 
