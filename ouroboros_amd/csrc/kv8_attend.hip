@@ -300,7 +300,7 @@ constexpr int joined_rows(int dp) { return dp <= 128 ? 16 : 8; }
 // sequences of 1024 slots instead of 19; 256 dims are held to two (51 -> 48 us for 32
 // of 4096); loads that bypass the caches take 59 us for 64 of 4096 instead of 51.
 template <typename IO, int DP, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 && NT == 1 ? 2 : 1))) void kv8_attend_kernel(Attend8Args a) {
+__global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
     constexpr int NJ = DP / 64;                   // steps of the first product over the dims
     constexpr int CH = DP / 16;                   // adjacent dims of V a lane
     constexpr int VW = CH / 4;                    // and their dwords
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 256 &
 // 593, a raised priority around the products changed nothing.  64 dims and bf16 rows
 // are held to three wavefronts a SIMD (two such pieces of 32 heads over 4: 778 -> 664 us).
 template <typename IO, int DP, int RT>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void kv8_rows_kernel(Attend8Args a) {
+__global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
     constexpr int NC = DP / 32;                // steps of the first product over the dims
     constexpr int CH = DP / 16, VW = CH / 4;   // adjacent dims of V a lane, and their dwords
     constexpr int NQ = sizeof(IO) == 4 ? 2 : 1;

@@ -59,11 +59,10 @@ struct VerifyArgs {
 };
 static_assert(sizeof(VerifyArgs) == 160, "VerifyArgs: kernel argument layout");
 
-// 2^y: y = k + f, |f| <= 1/2, and the polynomial of degree 8 that equals 2^f at
-// the nine Chebyshev points of [-1/2, 1/2], within 1.1e-12 of it between them
-// and 1 at 0.  Below 2^-1074, and for NaN, it is 0.
-__device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -2000.0);
+// 2^y, y finite: y = k + f, |f| <= 1/2, and the polynomial of degree 8 that equals 2^f
+// at the nine Chebyshev points of [-1/2, 1/2], within 1.1e-12 of it between them and 1
+// at 0.
+__device__ __forceinline__ double exp2_finite(double y) {
     const double k = rint(y), f = y - k;
     double s = 0x1.63d136366db24p-20;
     s = fma(s, f, 0x1.00dc4a532fb8ep-16);
@@ -76,11 +75,13 @@ __device__ __forceinline__ double exp2_64(double y) {
     s = fma(s, f, 1.0);
     return __builtin_amdgcn_ldexp(s, static_cast<int>(k));
 }
-// 2^y, 0 at 2^-1000 and below, so that a product of what is not 0 never is: the upper
-// half of y becomes that of -2000.  (A sum against its largest term does not see what
-// this leaves out, and does without: 2 us of verify_segments_kernel's 65.)
+// 2^y, 0 below 2^-1074 and for NaN.
+__device__ __forceinline__ double exp2_64(double y) { return exp2_finite(fmax(y, -2000.0)); }
+// 2^y, 0 at 2^-1000 and below and for NaN, so that a product of what is not 0 never is: the
+// upper half of y becomes that of -2000.  (A sum against its largest term does not see
+// what this leaves out, and does without: 2 us of verify_segments_kernel's 65.)
 __device__ __forceinline__ double exp2_held(double y) {
-    return exp2_64(__hiloint2double(y > -1000.0 ? __double2hiint(y) : static_cast<int>(0xc09f4000u), __double2loint(y)));
+    return exp2_finite(__hiloint2double(y > -1000.0 ? __double2hiint(y) : static_cast<int>(0xc09f4000u), __double2loint(y)));
 }
 // e^((x - m) / T), c = log2 e / T, x <= m: 1 where x = m, infinite or not.
 __device__ __forceinline__ double weight(float x, float m, double c) {
