@@ -294,11 +294,10 @@ constexpr int joined_rows(int dp) { return dp <= 128 ? 16 : 8; }
 // fp32.
 //
 // Bound by memory where the splits fill the chip (128 sequences of 8192 slots, 4 kv
-// heads of 128: 228 us, 4.7 TB/s), below that by what a workgroup does before its
-// first products and after its last: one sequence of 300 slots takes 9 us. Four
-// wavefronts a SIMD instead of three (128 dims, 16 rows) spill and take 24 us for 64
-// sequences of 1024 slots instead of 19; 256 dims are held to two (51 -> 48 us for 32
-// of 4096); loads that bypass the caches take 59 us for 64 of 4096 instead of 51.
+// heads of 128: 226 us, 4.8 TB/s), below that by what a workgroup does before its
+// first products and after its last: one sequence of 300 slots takes 9 us.  Four
+// wavefronts a SIMD instead of three (128 dims, 16 rows) take 18.4 us for 64 sequences
+// of 1024 slots and 227 for 128 of 8192 instead of 18.2 and 226.
 template <typename IO, int DP, int NT>
 __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
     constexpr int NJ = DP / 64;                   // steps of the first product over the dims
@@ -608,8 +607,8 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
         }
 }
 
-// The same for many rows of a sequence and kv head: 64 RT of them a workgroup, 16 RT
-// a wavefront, which takes them through all slots of the split, so that nothing is
+// The same for many rows of a sequence and kv head: 128 of them a workgroup, two tiles
+// of 16 a wavefront, which takes them through all slots of the split, so that nothing is
 // joined but splits.  64 slots at a time of K and V are turned to fp16 operands
 // once for all of them and go through LDS, a buffer being filled while the other
 // is read; wavefronts 0 and 1 make V's operands, 2 and 3 K's.  A query is one fp16
@@ -618,15 +617,16 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Attend8Args a) {
 // of three digits cost a third more matrix instructions and four conversions a
 // score.
 //
-// Bound by issue: of 520 us for two pieces of 1024 bf16 rows over up to 16384 slots
-// (250 GFLOP, 0.48 PFLOP/s) the matrix instructions are 149 and the others 215 (138
-// for each 16 rows and 32 slots, 45 of them the staging), and on the two wavefronts
-// of a SIMD they hardly overlap: a form that interleaves one half's products with the
-// other's weights took 67 registers too many and 669 us, one that reads operands ahead
-// 593, a raised priority around the products changed nothing.  64 dims and bf16 rows
-// are held to three wavefronts a SIMD (two such pieces of 32 heads over 4: 778 -> 664 us).
-template <typename IO, int DP, int RT>
+// Bound by issue: two pieces of 1024 bf16 rows over up to 16384 slots take 487 us (250
+// GFLOP, 0.51 PFLOP/s), of which a SIMD is busy for 1.00 million cycles (some 2.1 GHz
+// under this load). Matrix instructions take 0.36 of them, the others 0.49 (130 for each
+// 16 rows and 32 slots, some 45 of them the staging), and the two wavefronts that the LDS
+// leaves a SIMD overlap little of that.  One tile's weights stand beside the other's
+// products (after both 549); one tile a wavefront takes 667 us for fp32 rows, two 542.
+constexpr int kRowTiles = 2, kGroupRows = 64 * kRowTiles;
+template <typename IO, int DP>
 __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
+    constexpr int RT = kRowTiles;
     constexpr int NC = DP / 32;                // steps of the first product over the dims
     constexpr int CH = DP / 16, VW = CH / 4;   // adjacent dims of V a lane, and their dwords
     constexpr int NQ = sizeof(IO) == 4 ? 2 : 1;
@@ -641,11 +641,11 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Attend8Args a) {
     const int64_t b = static_cast<int64_t>(blockIdx.x) / a.c.n_head_kv;
     const int G = a.n_head / a.c.n_head_kv, d = a.c.d;
     const SeqRows s = seq_rows(a.r, b);
-    const int R = s.count * G, group0 = static_cast<int>(blockIdx.y) * 64 * RT;
+    const int R = s.count * G, group0 = static_cast<int>(blockIdx.y) * kGroupRows;
     if (group0 >= R) return;  // whole workgroup
     const int before = s.n - s.count;  // slots ahead of the new rows
     const int slots = a.turns * kTurn, split = blockIdx.z, split_first = split * slots, split_end = min(split_first + slots, s.n);
-    const int at_min = before + group0 / G, at_max = before + (min(group0 + 64 * RT, R) - 1) / G;
+    const int at_min = before + group0 / G, at_max = before + (min(group0 + kGroupRows, R) - 1) / G;
     const bool whole = s.n <= slots;  // the sequence's only split
     if (whole ? split > 0 : !sees(a, at_max, split_first, split_end) && !sees(a, at_min, split_first, split_end)) return;
     const int end = seen_end(a, at_min, at_max, split_end), first = seen_begin(a, at_min, split_first, kStage);
@@ -974,14 +974,14 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attend8Args a) {
 template <typename IO, int DP>
 int launch_join(const Attend8Args &a, size_t seqs, hipStream_t s);
 
-template <typename IO, int DP, int RT>
+template <typename IO, int DP>
 int launch_rows(const Attend8Args &a, size_t seqs, hipStream_t s) {
     constexpr size_t lds = 2 * (4 * (DP / 32) + 2 * (DP / 16)) * 1024;
     static_assert(lds <= 65536, "more LDS than a launch gets unasked");
     const int64_t rows = static_cast<int64_t>(a.r.max_new) * (a.n_head / a.c.n_head_kv);
-    const dim3 grid(static_cast<unsigned>(seqs * static_cast<size_t>(a.c.n_head_kv)), static_cast<unsigned>((rows + 64 * RT - 1) / (64 * RT)),
+    const dim3 grid(static_cast<unsigned>(seqs * static_cast<size_t>(a.c.n_head_kv)), static_cast<unsigned>((rows + kGroupRows - 1) / kGroupRows),
                     static_cast<unsigned>(a.n_split));
-    hipLaunchKernelGGL((kv8_rows_kernel<IO, DP, RT>), grid, dim3(256), lds, s, a);
+    hipLaunchKernelGGL((kv8_rows_kernel<IO, DP>), grid, dim3(256), lds, s, a);
     const int st = check_launch("kv8_rows_kernel");
     return st ? st : launch_join<IO, DP>(a, seqs, s);
 }
@@ -1031,26 +1031,26 @@ struct Way {
     int splits;  // no more for any shorter max_len
 };
 constexpr int kFewRows = 16, kSomeRows = 256, kMostSplits = 1024;
-// kv8_rows_kernel: of a kv head's rows a workgroup has, and how often its grid is split
-constexpr int group_rows(int io_bytes) { return io_bytes == 2 ? 128 : 64; }
+// how often the grid of kv8_rows_kernel is split
 constexpr int kManyGroups = 512, kLeastSplits = 4;
-Way way_of(int64_t rows, int n_head_kv, int dp, int io_bytes, size_t max_len) {
+Way way_of(int64_t rows, int n_head_kv, int dp, size_t max_len) {
     Way w;
     const int64_t all = static_cast<int64_t>((max_len + kTurn - 1) / kTurn);
     if (rows <= kFewRows) {
-        // two turns: 64 sequences of 1024 slots 19 us (one turn 22, four 17), one of 16384
-        // 14.3 (13.0, 18.6); wider heads four: 32 of 4096 and 256 dims 51 us (two turns 61)
+        // two turns: 64 sequences of 1024 slots 18.2 us (one turn 21.2, four 15.7), one of
+        // 16384 13.9 (12.7, 17.9); wider heads four: 32 of 4096 and 256 dims 47.0 us (two 48.5)
         w = {1, dp <= 128 ? 2 : 4, 0};
     } else if (rows <= kSomeRows || dp > 128) {
-        // 64 sequences of 2048 slots and 20 rows 38 us (one tile at best 43), 48 of 4096
-        // and 96 rows 58 (kv8_rows_kernel 56), 4 of 4096 and 256 rows 42 (45)
+        // 64 sequences of 2048 slots and 20 rows 35.0 us (one tile at best 44.9), 48 of 4096
+        // and 96 rows 77 (kv8_rows_kernel 89; of 64 dims 53 and 54), 4 of 4096 and 256 rows
+        // 38 (48); wider heads eight turns: 32 of 4096, 24 rows of 256 dims 62 (four 73)
         w = {2, dp <= 128 ? 4 : 8, 0};
     } else {
         // splits until some 512 workgroups of a sequence's have work, and four at least, of
-        // four to sixteen turns: one sequence of 16384 slots and 1024 rows 99 us with four
-        // turns (eight 119), two of 4096 rows 528 with sixteen (eight 547, thirty-two 512),
-        // one prompt of 4096 tokens, 16384 rows, 211 with four (eight 217, sixteen 250)
-        const int64_t groups = (rows + group_rows(io_bytes) - 1) / group_rows(io_bytes) * n_head_kv;
+        // four to sixteen turns: one sequence of 16384 slots and 1024 rows 92 us with four
+        // turns (eight 122), two of 4096 rows 499 with sixteen (eight 518, thirty-two 474),
+        // one prompt of 4096 tokens, 16384 rows, 194 with four (eight 206, sixteen 231)
+        const int64_t groups = (rows + kGroupRows - 1) / kGroupRows * n_head_kv;
         const int64_t splits = groups * kLeastSplits < kManyGroups ? kManyGroups / groups : kLeastSplits;
         const int64_t turns = (all + splits - 1) / splits, least = (all + 15) / 16, most = (all + 3) / 4;
         w = {0, static_cast<int>(turns < 4 ? 4 : turns > 16 ? 16 : turns), 0};
@@ -1081,9 +1081,9 @@ size_t records_bytes(size_t rows, size_t seqs, size_t max_new, size_t n_head, si
 int64_t rows_of_one(size_t max_new, size_t n_head, size_t n_head_kv) {
     return static_cast<int64_t>((max_new < (1u << 24) ? max_new : 1u << 24) * (n_head / n_head_kv));
 }
-Attend8Ws attend_ws(size_t seqs, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len, int io_bytes) {
+Attend8Ws attend_ws(size_t seqs, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len) {
     Attend8Ws w{};
-    w.way = way_of(rows_of_one(max_new, n_head, n_head_kv), static_cast<int>(n_head_kv), padded(d), io_bytes, max_len);
+    w.way = way_of(rows_of_one(max_new, n_head, n_head_kv), static_cast<int>(n_head_kv), padded(d), max_len);
     const size_t slots = static_cast<size_t>(w.way.turns) * kTurn;
     w.n_split = max_len ? static_cast<int>((max_len + slots - 1) / slots) : 1;
     if (max_new > rows) max_new = rows;
@@ -1092,38 +1092,31 @@ Attend8Ws attend_ws(size_t seqs, size_t rows, size_t max_new, size_t n_head, siz
     return w;
 }
 
-// The most that a call of no more rows, new ones of a sequence or slots can take, in
-// either type: fewer rows of a sequence can go a way of more splits.  Records grow
+// The most that a call of no more rows, new ones of a sequence or slots can take: fewer rows of a sequence can go a way of more splits.  Records grow
 // with max_new while the way's splits are the same, so what counts is the largest
 // max_new of each: of few rows, of some, of each number of groups that is split anew.
 size_t attend_most(size_t seqs, size_t rows, size_t max_new, size_t n_head, size_t n_head_kv, size_t d, size_t max_len) {
     if (!n_head_kv || n_head < n_head_kv || seqs > 65535 || rows > (1u << 23)) return 0;
     const size_t G = n_head / n_head_kv;
     size_t most = 0;
-    auto see = [&](size_t of_one, int io_bytes) {  // rows of a kv head
+    auto see = [&](size_t of_one) {  // rows of a kv head
         const size_t t = of_one / G < max_new ? of_one / G : max_new;
         size_t part;
-        const Way w = way_of(rows_of_one(t, n_head, n_head_kv), static_cast<int>(n_head_kv), padded(d), io_bytes, max_len);
+        const Way w = way_of(rows_of_one(t, n_head, n_head_kv), static_cast<int>(n_head_kv), padded(d), max_len);
         const size_t b = records_bytes(rows, seqs, t < rows ? t : rows, n_head, d, w.splits, &part);
         if (b > most) most = b;
     };
-    for (int io_bytes : {2, 4}) {
-        see(kFewRows, io_bytes);
-        see(kSomeRows, io_bytes);
-        for (size_t g = 1; g * n_head_kv * kLeastSplits < kManyGroups + n_head_kv * kLeastSplits; ++g)
-            see(g * static_cast<size_t>(group_rows(io_bytes)), io_bytes);
-        see(max_new < (1u << 24) ? max_new * G : static_cast<size_t>(1u << 24) * G, io_bytes);
-    }
+    see(kFewRows);
+    see(kSomeRows);
+    for (size_t g = 1; g * n_head_kv * kLeastSplits < kManyGroups + n_head_kv * kLeastSplits; ++g) see(g * kGroupRows);
+    see(max_new < (1u << 24) ? max_new * G : static_cast<size_t>(1u << 24) * G);
     return most;
 }
 
 template <typename IO>
 int launch_attend(const Attend8Args &a, size_t seqs, int tiles, hipStream_t s) {
     const int dp = padded(static_cast<size_t>(a.c.d));
-    // bf16 rows two tiles a wavefront; fp32 queries take twice the registers, and one
-    // tile (two sequences' 1024 rows over 16384 slots: 745 us, two tiles 754)
-    constexpr int RT = sizeof(IO) == 2 ? 2 : 1;
-    if (tiles == 0) return dp == 64 ? launch_rows<IO, 64, RT>(a, seqs, s) : launch_rows<IO, 128, RT>(a, seqs, s);
+    if (tiles == 0) return dp == 64 ? launch_rows<IO, 64>(a, seqs, s) : launch_rows<IO, 128>(a, seqs, s);
     if (dp == 64) return tiles == 1 ? launch_attend<IO, 64, 1>(a, seqs, s) : launch_attend<IO, 64, 2>(a, seqs, s);
     if (dp == 128) return tiles == 1 ? launch_attend<IO, 128, 1>(a, seqs, s) : launch_attend<IO, 128, 2>(a, seqs, s);
     if (dp == 192) return tiles == 1 ? launch_attend<IO, 192, 1>(a, seqs, s) : launch_attend<IO, 192, 2>(a, seqs, s);
@@ -1177,7 +1170,7 @@ int ouro_kv8_attend(const ouro_kv8_cache *cache, const void *q, size_t q_stride,
     a.q_stride = static_cast<int64_t>(q_stride), a.out_stride = static_cast<int64_t>(out_stride);
     a.mask_stride = static_cast<int64_t>(mask_stride);
     a.n_head = static_cast<int>(n_head), a.window = window ? most(window) : 1 << 30, a.sinks = most(sinks), a.scale = scale;
-    const Attend8Ws w = attend_ws(seqs, rows, max_new, n_head, hkv, d, max_len, dtype == OURO_DT_F32 ? 4 : 2);
+    const Attend8Ws w = attend_ws(seqs, rows, max_new, n_head, hkv, d, max_len);
     a.n_split = w.n_split, a.turns = w.way.turns, a.by_seq = w.by_seq;
     const size_t most_new = static_cast<size_t>(a.r.max_new);
     if (seqs * hkv >= (1u << 24) || most_new * (n_head / hkv) > (1u << 20) || most_new * n_head >= (1u << 24))
