@@ -35,7 +35,7 @@ static_assert(sizeof(RopeArgs) == 184, "RopeArgs: kernel argument layout");
 
 // cos and sin of pos * freq.  In quarter turns u = pos freq 2/pi: its nearest
 // integer says which of cos, sin, -cos, -sin, and of what is left, within 1/2,
-// the series of x = (pi/2) rest, |x| <= pi/4, leave out less than 2^-31.  The
+// the series of x = (pi/2) rest, |x| <= pi/4, leave out less than 2^-29.  The
 // product is exact but for one rounding in 64 bits and 2/pi is held in two
 // parts, so that far positions keep their angle; single precision begins at x.
 __device__ __forceinline__ float2 cos_sin(int pos, float freq) {
@@ -101,9 +101,10 @@ __device__ __forceinline__ void store(T *p, const float (&x)[E]) {
 // of G lanes stays with one token and keeps its angles and gains in registers.
 //
 // 16385 rows of 20 heads of 128, bf16: 47 us, 3.6 TB/s where a copy has 5, bound by
-// the five wavefronts a SIMD that 95 registers leave (eight tokens a workgroup; with
-// the angles and a division a head made anew 73).  64 fp32 rows take 4.6 us, a part of
-// a token's heads a workgroup: three dependent loads and the angles.
+// the five wavefronts a SIMD that two pieces of eight values a lane leave (95 registers;
+// eight tokens a workgroup; with the angles and a division a head made anew 73).  64 fp32
+// rows take 4.4 us, a part of a token's heads a workgroup: three dependent loads and the
+// angles.
 template <typename T, int E, int G>
 __global__ __launch_bounds__(kThreads) void qk_rope_kernel(RopeArgs a) {
     __shared__ __attribute__((aligned(16))) float cs[kMaxTokens][kMaxHalf], sn[kMaxTokens][kMaxHalf];

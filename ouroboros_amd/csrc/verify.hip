@@ -8,8 +8,9 @@
 //
 // Which token is drawn hangs on sums over the whole vocabulary: at 248320 tokens
 // a sum that is off by 1e-9 gives another token once in some thousand draws.  So
-// exponentials, sums and comparisons are made in 64 bits, where it is once in 1e9
-// or rarer; the logits are read in their own type and their differences are exact.
+// exponentials, sums and comparisons are made in 64 bits, exponentials within 1.1e-12:
+// once in some million.  The logits are read in their own type, and it is their
+// differences that are scaled.
 #include "logits.hpp"
 
 #include "kv_cache.hpp"
@@ -184,9 +185,10 @@ __device__ __forceinline__ void segment(const VerifyArgs &a, int which, int64_t 
 
 // A wavefront a segment, of the target's rows and then of the drafter's.  No
 // barrier and no LDS: what a wavefront waits for is its 8 KiB of logits.  64
-// sequences of up to four drafted tokens over 248320 logits, 340 MB: 66 us at 5.1 TB/s,
-// the rate of a copy (17 instructions in 64 bits a logit are some 35 of it; workgroups
-// of 8192 logits and a polynomial of degree 11 took 107).
+// sequences of up to four drafted tokens over 248320 logits, 308 MB (the drafter's rows of
+// greedy sequences are not read): 65 us at 4.7 TB/s where a copy has 5 (18 instructions in
+// 64 bits a logit are some 35 of it; workgroups of 8192 logits and a polynomial of degree
+// 11 took 107).
 template <typename T, typename D>
 __global__ __launch_bounds__(kThreads) void verify_segments_kernel(VerifyArgs a) {
     const int which = static_cast<int>(blockIdx.y) / a.r.max_new, i = static_cast<int>(blockIdx.y) % a.r.max_new;
@@ -361,8 +363,8 @@ __device__ __forceinline__ void say(const VerifyArgs &a, int64_t b, const SeqRow
 // Every workgroup of a sequence judges its rows (all wait for the same few
 // kilobytes); where a token was refused each wavefront then sums max(p - q, 0)
 // over a segment of that row.  64 sequences of up to four drafted tokens over
-// 248320 logits, some 90 MB of refusing rows: 33 us; the judging in a launch of
-// its own 8 + 25 us and one launch more, two segments a wavefront 43.
+// 248320 logits, some 90 MB of refusing rows: 34 us; the judging in a launch of
+// its own 8 + 25 us where this took 33, and one launch more, two segments a wavefront 43.
 template <typename T, typename D>
 __global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a) {
     constexpr int VL = Left<T, D>::VL;
