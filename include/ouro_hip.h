@@ -668,7 +668,8 @@ typedef struct ouro_kv8_cache {
  *   code = x / scale rounded to nearest even;
  * and where the scale grew, the codes of the slots before are rounded to it.
  * So a block's scale is the largest that its rows need, in whatever pieces they
- * came, and a row's error is at most half a step when it is written and less
+ * came (rows written and taken back since, while older ones are there, among them),
+ * and a row's error is at most half a step when it is written and less
  * than half of the present step more by later growth.  A NaN is held as 0, an
  * infinity as +-127 steps of what finite values need (as 0 where all are 0), a
  * block of zeros has scale 0.  Other slots keep their codes.  A page that gets

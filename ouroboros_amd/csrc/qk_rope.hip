@@ -103,7 +103,7 @@ __device__ __forceinline__ void store(T *p, const float (&x)[E]) {
 // 16385 rows of 20 heads of 128, bf16: 47 us, 3.6 TB/s where a copy has 5, bound by
 // the five wavefronts a SIMD that two pieces of eight values a lane leave (95 registers;
 // eight tokens a workgroup; with the angles and a division a head made anew 73).  64 fp32
-// rows take 4.4 us, a part of a token's heads a workgroup: three dependent loads and the
+// rows take 4.5 us, a part of a token's heads a workgroup: three dependent loads and the
 // angles.
 template <typename T, int E, int G>
 __global__ __launch_bounds__(kThreads) void qk_rope_kernel(RopeArgs a) {
